@@ -1,0 +1,489 @@
+"""Operators of ztcp_b200.kvcache on the GPU against plain 64-bit forms, at the sizes and masks where they can go
+wrong: pages that end inside a tile, odd page sizes, rows that see nothing, empty sequences, stale NaN in unused page
+rows, table entries outside the pool, strided queries, streams, graphs and prepared calls."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kvcache_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+F16, BF16 = torch.float16, torch.bfloat16
+ids = lambda x: str(x).replace("torch.", "").replace(" ", "")  # noqa: E731
+
+
+def cpu(t):
+    return None if t is None else t.cpu()
+
+
+def queries(rows, heads, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn((rows, heads, D), generator=g).to(dtype).to(DEV)
+
+
+def run_attend(q, k, v, tables, lens, q_lens, *, scale=None, causal=True, rope_dim=0, decode=False, **kw):
+    from ztcp_b200 import kvcache
+
+    dv = k.shape[3] - (rope_dim if v is None else 0)
+    out = torch.full((q.shape[0], q.shape[1], dv), 7.0, dtype=q.dtype, device=DEV)
+    lse = torch.full(q.shape[:2], 7.0, dtype=torch.float32, device=DEV)
+    starts = None if decode else ref.starts_of(q_lens)
+    status = kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=starts, max_q_len=max(max(q_lens), 1),
+                                  rope_dim=rope_dim, scale=scale, causal=causal, **kw)
+    torch.cuda.synchronize()
+    return out, lse, status
+
+
+def check_attend(kv, q_lens, T, H, G, D, dtype, *, mla_rope=None, causal=True, decode=False, seed=1, scale=None):
+    mla = mla_rope is not None
+    k, v, tables, lens = ref.make_cache(kv, T, H, D, dtype, seed, mla)
+    q = queries(sum(q_lens), H * G, D, dtype, seed + 1)
+    out, lse, status = run_attend(q, k, v, tables, lens, q_lens, causal=causal, rope_dim=mla_rope or 0, decode=decode,
+                                  scale=scale)
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv, q_lens, D ** -0.5 if scale is None else scale,
+                                     causal, mla_rope or 0)
+    assert not status.any()
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+
+
+# ---- attention --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("H,G,D", [(8, 4, 128), (2, 1, 64), (1, 16, 128), (3, 5, 80), (2, 2, 16), (1, 3, 256), (2, 4, 176)])
+def test_decode(dtype, H, G, D):
+    kv = [1, 64, 65, 0, 200, 127, 333]
+    check_attend(kv, [1] * len(kv), 64, H, G, D, dtype, decode=True)
+
+
+@pytest.mark.parametrize("T", [1, 5, 16, 48, 64, 100, 256])
+def test_decode_page_sizes(T):
+    kv = [300, 1, T, T + 1, 2 * T - 1]
+    check_attend(kv, [1] * len(kv), T, 2, 4, 64, BF16, decode=True)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("heads,D,rope", [(16, 576, 64), (5, 96, 32), (40, 576, 64), (8, 320, 0), (4, 272, 16)])
+def test_single_buffer(dtype, heads, D, rope):
+    kv = [1, 70, 0, 257]
+    check_attend(kv, [1] * len(kv), 64, 1, heads, D, dtype, mla_rope=rope, decode=True)
+    check_attend([90, 33], [7, 2], 16, 1, heads, D, dtype, mla_rope=rope)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D,T", [(128, 64), (64, 16), (128, 128), (96, 32), (128, 8), (64, 256), (112, 24), (48, 64)])
+def test_chunk(dtype, causal, D, T):
+    kv, q_lens = [200, 5, 0, 130, 64, 385], [50, 5, 0, 129, 1, 3]
+    check_attend(kv, q_lens, T, 2, 4, D, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("H,G", [(1, 1), (8, 1), (1, 8), (4, 3), (1, 32), (2, 7)])
+def test_chunk_head_layouts(H, G):
+    check_attend([300, 77, 140], [40, 77, 9], 64, H, G, 128, BF16)
+
+
+def test_rows_that_see_nothing():
+    # more query rows than tokens: the first rows see nothing; sequences without tokens or without rows between
+    check_attend([3, 0, 10, 0, 70], [8, 4, 0, 0, 200], 64, 2, 4, 128, BF16)
+    check_attend([3, 0, 10], [8, 4, 0], 64, 2, 4, 128, F16, causal=False)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_batches(seed):
+    kv, q_lens = ref.ragged(seed, 9, 700, 1 if seed % 3 == 0 else 60)
+    q_lens[0] = max(q_lens[0], 1)
+    check_attend(kv, q_lens, [64, 16, 32][seed % 3], [8, 2, 1][seed % 3], [4, 8, 6][seed % 3], [128, 64][seed % 2],
+                 [F16, BF16][seed // 3], seed=seed)
+
+
+def test_long_context_splits():
+    check_attend([9000], [1], 64, 1, 2, 64, F16, decode=True)
+    check_attend([6000, 4500], [33, 2], 64, 1, 4, 128, BF16)
+    check_attend([5000], [1], 64, 1, 16, 576, BF16, mla_rope=64, decode=True)
+
+
+def test_large_scores():
+    # a scale of 1 on 128 columns: scores of tens, one weight near 1
+    check_attend([500, 260], [3, 100], 64, 2, 4, 128, BF16, scale=1.0)
+
+
+def test_rows_behind_the_last_sequence_stay():
+    from ztcp_b200 import kvcache
+
+    k, v, tables, lens = ref.make_cache([100, 40], 64, 2, 128, BF16)
+    q = queries(60, 8, 128, BF16, 3)
+    out = torch.full((60, 8, 128), 5.0, dtype=BF16, device=DEV)
+    lse = torch.full((60, 8), 5.0, device=DEV)
+    kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=ref.starts_of([30, 20]), max_q_len=30)
+    torch.cuda.synchronize()
+    assert bool((out[50:] == 5).all()) and bool((lse[50:] == 5).all())
+    assert bool((out[:50] != 5).any()) and not bool((lse[:50] == 5).any())
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_bad_blocks_count_as_masked(q_len):
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = [200, 130, 64], [q_len] * 3
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 5)
+    tables[0, 1] = -1
+    tables[1, 0] = k.shape[0]
+    q = queries(sum(q_lens), 8, 128, BF16, 6)
+    with pytest.raises(RuntimeError, match="block_tables entries must lie"):
+        run_attend(q, k, v, tables, lens, q_lens)
+    out, lse, status = run_attend(q, k, v, tables, lens, q_lens, check_block_table=False)
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv, q_lens, 128 ** -0.5)
+    assert status.tolist() == [kvcache.SEQ_BAD_BLOCK, kvcache.SEQ_BAD_BLOCK, kvcache.SEQ_OK]
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+
+
+def test_bad_lengths_are_clamped():
+    from ztcp_b200 import kvcache
+
+    k, v, tables, lens = ref.make_cache([128, 128, 128], 64, 2, 64, F16, 5)
+    q = queries(3, 4, 64, F16, 6)
+    lens.copy_(torch.tensor([-5, 1 << 30, 100], dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="kv_lens entries must lie"):
+        run_attend(q, k, v, tables, lens, [1] * 3)
+    out, lse, status = run_attend(q, k, v, tables, lens, [1] * 3, check_block_table=False)
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), [0, 128, 100], [1] * 3, 64 ** -0.5)
+    assert status.tolist() == [kvcache.SEQ_BAD_LENGTH, kvcache.SEQ_BAD_LENGTH, kvcache.SEQ_OK]
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+    # starts that run backwards or past the rows
+    starts = torch.tensor([0, 2, 1, 9], dtype=torch.int32, device=DEV)
+    lens.fill_(100)
+    status = kvcache.attend_pages(q, k, v, tables, lens, out, q_starts=starts, max_q_len=3)
+    torch.cuda.synchronize()
+    assert status.tolist() == [kvcache.SEQ_OK, kvcache.SEQ_BAD_LENGTH, kvcache.SEQ_BAD_LENGTH]
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [50, 3, 20]])
+def test_strided_queries(q_lens):
+    kv = [100, 65, 300]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    fused = queries(sum(q_lens), 8 + 2 + 2, 128, BF16, 9)  # one projection: query heads, then key and value heads
+    q = fused[:, :8]
+    out, lse, _ = run_attend(q, k, v, tables, lens, q_lens)
+    out2, lse2, _ = run_attend(q.contiguous(), k, v, tables, lens, q_lens)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("q_lens", [[1] * 4, [70, 1, 33, 8]])
+def test_prepared_call_streams_and_graph(q_lens):
+    """A prepared call reads its tensors at every call, on any stream and from a graph, and repeats bit for bit."""
+    from ztcp_b200 import kvcache
+
+    kv = [700, 65, 300, 9]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8, poison=False)
+    q = queries(sum(q_lens), 8, 128, BF16, 9)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    call = kvcache.prepare_attend(q, k, v, tables, lens, out, lse=lse, q_starts=ref.starts_of(q_lens), max_q_len=70)
+    call()
+    torch.cuda.synchronize()
+    first = out.clone()
+    side = torch.cuda.Stream(DEV)
+    out.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    call(side)
+    side.synchronize()
+    assert torch.equal(out, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    kv2 = [130, 64, 1, 9]
+    lens.copy_(torch.tensor(kv2, dtype=torch.int32))
+    q.copy_(queries(sum(q_lens), 8, 128, BF16, 10))
+    graph.replay()
+    torch.cuda.synchronize()
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv2, q_lens, 128 ** -0.5)
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+
+
+def test_one_shot_calls_on_another_stream():
+    kv = [400, 65]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    q = queries(2, 8, 128, BF16, 9)
+    want, _, _ = run_attend(q, k, v, tables, lens, [1, 1])
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (side, side.cuda_stream):
+        out, _, _ = run_attend(q, k, v, tables, lens, [1, 1], stream=stream)
+        assert torch.equal(out, want)
+
+
+# ---- attention weight per page ----------------------------------------------------------------------------------
+def check_mass(kv, q_lens, T, H, G, D, dtype, *, causal=True, seed=1, decay=0.75, empty=True, bad=()):
+    from ztcp_b200 import kvcache
+
+    k, v, tables, lens = ref.make_cache(kv, T, H, D, dtype, seed, mla=True, extra_pages=2)
+    for b, p in bad:
+        tables[b, p] = -7
+    q = queries(sum(q_lens), H * G, D, dtype, seed + 1)
+    _, lse, _, _ = ref.attend(cpu(q), cpu(k), None, cpu(tables), kv, q_lens, D ** -0.5, causal)
+    lse = lse.float().to(DEV)
+    before = None if empty else torch.rand(tables.shape, device=DEV)
+    out = torch.full(tables.shape, 9.0, device=DEV)
+    status = kvcache.page_mass(q, k, tables, lens, lse, before, out, decay=decay, q_starts=ref.starts_of(q_lens),
+                               max_q_len=max(max(q_lens), 1), causal=causal, check_block_table=False)
+    torch.cuda.synchronize()
+    want, tol = ref.mass(cpu(q), cpu(k), cpu(tables), kv, q_lens, cpu(lse), cpu(before), decay, D ** -0.5, causal)
+    assert [s != 0 for s in status.tolist()] == [any(b == i for b, _ in bad) for i in range(len(kv))]
+    ref.assert_close(out, want, tol, "mass")
+    if before is not None:  # in place
+        kvcache.page_mass(q, k, tables, lens, lse, before, before, decay=decay, q_starts=ref.starts_of(q_lens),
+                          max_q_len=max(max(q_lens), 1), causal=causal, check_block_table=False)
+        assert torch.equal(before, out)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("T,H,G,D", [(64, 8, 4, 128), (16, 2, 1, 64), (5, 1, 3, 48), (100, 2, 8, 128), (256, 1, 4, 64),
+                                     (64, 1, 16, 576), (64, 2, 4, 256), (128, 4, 2, 128), (8, 2, 4, 64)])
+def test_mass_decode(dtype, T, H, G, D):
+    check_mass([1, 64, 0, 300, 129], [1, 1, 1, 1, 1], T, H, G, D, dtype, empty=dtype == F16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("T,D", [(64, 128), (16, 64), (48, 128), (128, 64), (64, 112)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_mass_window(dtype, T, D, causal):
+    check_mass([200, 0, 70, 33, 513], [32, 3, 70, 0, 64], T, 2, 4, D, dtype, causal=causal, empty=False)
+
+
+def test_mass_more_rows_than_tokens():
+    check_mass([3, 10], [40, 200], 16, 1, 4, 64, F16)
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_mass_bad_blocks(q_len):
+    check_mass([200, 130, 64], [q_len] * 3, 64, 2, 4, 128, BF16, bad=[(0, 1), (1, 0)])
+
+
+def test_mass_sums_to_the_rows():
+    """Without earlier weight, a sequence's pages add up to its rows times heads: every row's weights sum to 1."""
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = [900, 64, 1], [40, 1, 1]
+    k, v, tables, lens = ref.make_cache(kv, 64, 4, 128, BF16, 4)
+    q = queries(42, 16, 128, BF16, 5)
+    _, lse, _ = run_attend(q, k, v, tables, lens, q_lens)
+    out = torch.empty(tables.shape, device=DEV)
+    kvcache.page_mass(q, k, tables, lens, lse, None, out, q_starts=ref.starts_of(q_lens), max_q_len=40)
+    for total, rows in zip(out.double().sum(1).tolist(), q_lens):
+        # a weight is off by the errors of its score and of lse: scores of at most 2^4, 2^4 * 140 half steps each
+        assert abs(total / (rows * 16) - 1) <= 2 * 16 * 140 * ref.U32
+
+
+# ---- append -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("n,Hq,H,D,R,interleaved,norm_from,weights,mla", [
+    (1, 32, 8, 128, 128, False, 0, True, False),
+    (37, 8, 2, 128, 64, True, 0, True, False),
+    (300, 4, 1, 64, 64, False, 0, True, False),
+    (5, 16, 1, 576, 64, False, 64, True, True),
+    (5, 3, 2, 48, 16, True, 0, True, False),
+    (9, 6, 3, 96, 96, False, 32, False, False),
+    (4, 2, 2, 256, 256, False, 0, True, False),
+    (4, 2, 1, 1024, 256, True, 0, True, False),
+    (3, 5, 1, 80, 0, False, 16, True, False),
+    (2, 1, 1, 16, 16, False, 0, True, True),
+])
+def test_append(dtype, n, Hq, H, D, R, interleaved, norm_from, weights, mla):
+    from ztcp_b200 import kvcache
+
+    g = torch.Generator().manual_seed(n * D)
+    T, pages = 16, n // 16 + 3
+    split = [Hq * D, H * D, 0 if mla else H * D]
+    qkv = torch.randn((n, sum(split) + 8), generator=g).to(dtype)  # rows with a gap behind them
+    q, k, v = (t.unflatten(1, (-1, D)) if t.shape[1] else None for t in qkv[:, :sum(split)].split(split, dim=1))
+    qw, kw = ((1 + 0.2 * torch.randn(D - norm_from, generator=g)) if weights else None for _ in range(2))
+    table = kvcache.rope_table(500, R, device="cpu") if R else None
+    pos = torch.randint(0, 500, (n,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(pages * T, generator=g)[:n].clone()
+    if n > 2:
+        slots[1] = -1
+    kp = torch.full((pages, T, H, D), 3.0, dtype=dtype, device=DEV)
+    vp = None if mla else kp.clone()
+    dq = qkv.to(DEV)
+    dq, dk, dv = (t.unflatten(1, (-1, D)) if t.shape[1] else None for t in dq[:, :sum(split)].split(split, dim=1))
+    qo = torch.empty((n, Hq, D), dtype=dtype, device=DEV)
+    dev = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    status = kvcache.append_tokens(dq, dk, dv, kp, vp, dev(slots), dev(pos), dev(table), qo, q_weight=dev(qw),
+                                   k_weight=dev(kw), norm_from=norm_from, eps=1e-5, interleaved=interleaved)
+    assert not status.any()
+    want, tol = ref.norm_rotate(q, qw, norm_from, 1e-5, table, pos, interleaved)
+    ref.assert_close(qo, want, tol, "q")
+    want, tol = ref.norm_rotate(k, kw, norm_from, 1e-5, table, pos, interleaved)
+    written = slots >= 0
+    ref.assert_close(kp.view(-1, H, D)[dev(slots[written])], want[written], tol[written], "k")
+    rest = torch.ones(pages * T, dtype=torch.bool)
+    rest[slots[written]] = False
+    assert bool((kp.view(-1, H, D)[dev(rest)] == 3).all())
+    if not mla:
+        assert torch.equal(vp.view(-1, H, D)[dev(slots[written])].cpu(), v[written])
+        assert bool((vp.view(-1, H, D)[dev(rest)] == 3).all())
+
+
+def test_append_bad_slots_and_positions():
+    from ztcp_b200 import kvcache
+
+    n, H, D, T = 6, 2, 64, 16
+    k, v, q = (queries(n, h, D, BF16, s) for h, s in ((H, 1), (H, 2), (4, 3)))
+    kp = torch.full((2, T, H, D), 3.0, dtype=BF16, device=DEV)
+    vp = kp.clone()
+    table = kvcache.rope_table(50, 64)
+    slots = torch.tensor([0, 32, -2, 5, 6, 1 << 40], dtype=torch.int64, device=DEV)
+    pos = torch.tensor([0, 1, 2, 50, -1, 3], dtype=torch.int32, device=DEV)
+    qo = torch.full_like(q, 9.0)
+    status = kvcache.append_tokens(q, k, v, kp, vp, slots, pos, table, qo)
+    bad = kvcache.SEQ_BAD_BLOCK
+    assert status.tolist() == [0, bad, bad, bad, bad, bad]
+    assert bool((qo[3:5] == 9).all())                       # a position outside the table: nothing is written
+    assert not bool((qo[[0, 1, 2, 5]] == 9).all(-1).any())  # a slot outside the pool: the query only
+    assert bool((kp.view(-1, H, D)[1:] == 3).all()) and not bool((kp.view(-1, H, D)[0] == 3).all())
+    assert torch.equal(vp.view(-1, H, D)[0], v[0]) and bool((vp.view(-1, H, D)[1:] == 3).all())
+
+
+def test_append_in_place_and_without_queries():
+    from ztcp_b200 import kvcache
+
+    n, H, D, T = 33, 2, 128, 64
+    k, v, q = (queries(n, h, D, F16, s) for h, s in ((H, 1), (H, 2), (8, 3)))
+    kp, vp = (torch.zeros((1, T, H, D), dtype=F16, device=DEV) for _ in range(2))
+    table, pos = kvcache.rope_table(64, 128), torch.arange(n, dtype=torch.int32, device=DEV)
+    slots = torch.arange(n, device=DEV)
+    qo = torch.empty_like(q)
+    kvcache.append_tokens(q, k, v, kp, vp, slots, pos, table, qo)
+    kp2, vp2 = torch.zeros_like(kp), torch.zeros_like(vp)
+    kvcache.append_tokens(q, k, v, kp2, vp2, slots, pos, table, q)
+    assert torch.equal(q, qo) and torch.equal(kp, kp2)
+    kp2.zero_()
+    kvcache.append_tokens(None, k, v, kp2, vp2, slots, pos, table, None)
+    assert torch.equal(kp, kp2) and torch.equal(vp, vp2)
+
+
+# ---- eviction ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kv,T,keep,sink,recent", [
+    ([640], 64, 4, 1, 1),
+    ([0, 1, 64, 65, 1000, 5000, 4999], 16, 20, 2, 3),
+    ([3000, 2000], 1, 100, 0, 1),
+    ([500, 20], 16, 0, 0, 1),
+    ([500, 20], 16, 1000, 3, 5),
+    ([500, 48], 16, 2, 40, 40),
+    ([70000], 16, 4000, 4, 8),
+])
+def test_select(kv, T, keep, sink, recent):
+    from ztcp_b200 import kvcache
+
+    P = max(-(-n // T) for n in kv) + 1
+    g = torch.Generator().manual_seed(len(kv) * T)
+    mass = torch.rand((len(kv), P), generator=g)
+    mass[torch.rand(mass.shape, generator=g) < 0.4] = 0.25   # ties
+    mass[torch.rand(mass.shape, generator=g) < 0.05] = float("nan")
+    mass[torch.rand(mass.shape, generator=g) < 0.05] = float("inf")
+    mass[torch.rand(mass.shape, generator=g) < 0.1] = 0.0
+    mass[torch.rand(mass.shape, generator=g) < 0.1] = -0.0
+    mass[torch.rand(mass.shape, generator=g) < 0.05] = -1.5
+    tables = torch.randint(0, 1 << 20, (len(kv), P), generator=g, dtype=torch.int32)
+    want = ref.select(mass.numpy(), tables, kv, T, keep, sink, recent)
+    sel = kvcache.select_cold_pages(mass.to(DEV), tables.to(DEV), torch.tensor(kv, dtype=torch.int32, device=DEV),
+                                    page_tokens=T, keep=keep, sink=sink, recent=recent)
+    for got, exp, name in zip(sel, want, sel._fields):
+        if name == "kept_mass":
+            assert torch.equal(got.cpu().nan_to_num(nan=77.0), torch.tensor(exp).nan_to_num(nan=77.0)), name
+        else:
+            assert got.tolist() == exp, name
+    assert not sel.status.any()
+
+
+def test_select_clamps_lengths():
+    from ztcp_b200 import kvcache
+
+    mass = torch.rand((2, 8), device=DEV)
+    tables = torch.arange(16, dtype=torch.int32, device=DEV).view(2, 8)
+    lens = torch.tensor([-3, 1 << 20], dtype=torch.int32, device=DEV)
+    sel = kvcache.select_cold_pages(mass, tables, lens, page_tokens=16, keep=5)
+    want = ref.select(mass.cpu().numpy(), tables.cpu(), [0, 128], 16, 5, 1, 1)
+    assert sel.status.tolist() == [kvcache.SEQ_BAD_LENGTH] * 2
+    assert sel.cold_blocks.tolist() == want[0] and sel.kept_tables.tolist() == want[3] and sel.kept_lens.tolist() == want[5]
+
+
+# ---- together ---------------------------------------------------------------------------------------------------
+def test_append_attend_mass_select_egress_ingress():
+    """A serving loop over one layer: prompt chunks are appended and attended to, the pages with the least attention
+    weight are chosen, encrypted from their pool slots and restored into fresh ones; attention over the compacted
+    tables sees exactly the pages that stayed, over the restored ones what the codec gives back."""
+    from ztcp_b200 import capi, codec, kvcache, workload
+
+    T, H, Hq, D, R, pool = 64, 8, 32, 128, 64, 40
+    prompts, q_scale = [700, 430], D ** -0.5
+    g = torch.Generator().manual_seed(3)
+    table = kvcache.rope_table(1024, R)
+    w = (1 + 0.1 * torch.randn(D, generator=g)).to(DEV)
+    kp, vp = (torch.zeros((pool, T, H, D), dtype=F16, device=DEV) for _ in range(2))
+    tables = torch.randperm(pool, generator=g)[:2 * 12].view(2, 12).to(torch.int32).to(DEV)
+    starts = ref.starts_of(prompts)
+    n = sum(prompts)
+    qkv = torch.randn((n, Hq + 2 * H, D), generator=g).to(F16).to(DEV)
+    pos = torch.cat([torch.arange(m) for m in prompts])
+    seq = torch.cat([torch.full((m,), b) for b, m in enumerate(prompts)])
+    slots = tables.cpu()[seq, pos // T].long() * T + pos % T
+    q = torch.empty((n, Hq, D), dtype=F16, device=DEV)
+    st = kvcache.append_tokens(qkv[:, :Hq], qkv[:, Hq:Hq + H], qkv[:, Hq + H:], kp, vp, slots.to(DEV),
+                               pos.to(torch.int32).to(DEV), table, q, q_weight=w, k_weight=w, interleaved=True)
+    lens = torch.tensor(prompts, dtype=torch.int32, device=DEV)
+    out, lse = torch.empty_like(q), torch.empty((n, Hq), device=DEV)
+    st2 = kvcache.attend_pages(q, kp, vp, tables, lens, out, lse=lse, q_starts=starts, max_q_len=700)
+    torch.cuda.synchronize()
+    assert not st.any() and not st2.any()
+    rows = torch.tensor([0, 5, 64, 699, 700, 1129])  # some rows against the plain form
+    for r in rows.tolist():
+        b, i = (0, r) if r < 700 else (1, r - 700)
+        want, _, tol, _ = ref.attend(cpu(q[r:r + 1]), cpu(kp), cpu(vp), cpu(tables[b:b + 1]), [i + 1], [1], q_scale)
+        ref.assert_close(out[r:r + 1], want, tol, f"row {r}")
+
+    window = 16  # attention weight of each prompt's last rows
+    pick = torch.cat([torch.arange(m - window, m) + s for m, s in zip(prompts, [0, 700])]).to(DEV)
+    mass = torch.zeros(tables.shape, device=DEV)
+    kvcache.page_mass(q[pick], kp, tables, lens, lse[pick], mass, mass, q_starts=ref.starts_of([window] * 2),
+                      max_q_len=window)
+    sel = kvcache.select_cold_pages(mass, tables, lens, page_tokens=T, keep=6, sink=1, recent=2)
+    want = ref.select(mass.cpu().numpy(), tables.cpu(), prompts, T, 6, 1, 2)
+    assert sel.cold_blocks.tolist() == want[0] and sel.kept_lens.tolist() == [700 - 5 * 64, 430 - 64]
+
+    cold = int(sel.cold_starts[-1])
+    assert cold == 6
+    m = workload.session_material(5)
+    keys = capi.keys(*m["key"], *m["mac_key"])
+    hashes = torch.from_numpy(workload.token_hashes(24, 9)).to(DEV)[sel.cold_index[:cold].long()]
+    blobs = torch.empty((cold, 98352), dtype=torch.uint8, device=DEV)
+    kw = dict(rope_dim=64, tenant_id_hash=m["tenant"], model_id_hash=m["model"], layer_id=1, keys=keys)
+    blocks = sel.cold_blocks[:cold].clone()
+    codec.encode_pages(kp, vp, hashes, blobs, preset=1, rope_mode=1, expected_payload_bytes=98304, head_group_id=0,
+                       base_sequence_nonce=1, block_table=blocks, **kw)
+
+    # decode step over the compacted tables
+    q1 = queries(2, Hq, D, F16, 12)
+    o1 = torch.empty_like(q1)
+    kvcache.attend_pages(q1, kp, vp, sel.kept_tables, sel.kept_lens, o1)
+    want, _, tol, _ = ref.attend(cpu(q1), cpu(kp), cpu(vp), cpu(sel.kept_tables), sel.kept_lens.tolist(), [1, 1], q_scale)
+    ref.assert_close(o1, want, tol, "compacted")
+
+    # the cold pages come back into other pool pages
+    free = [p for p in range(pool) if p not in set(tables.flatten().tolist())][:cold]
+    back = torch.tensor(free, dtype=torch.int32, device=DEV)
+    status, fail = codec.decode_pages(blobs, hashes, kp, vp, is_mla=False, block_table=back, **kw)
+    codec.raise_for_status(status, fail)
+    restored = tables.clone()
+    restored.view(-1)[sel.cold_index[:cold].long()] = back
+    kvcache.attend_pages(q1, kp, vp, restored, lens, o1)
+    want, _, tol, _ = ref.attend(cpu(q1), cpu(kp), cpu(vp), cpu(restored), prompts, [1, 1], q_scale)
+    ref.assert_close(o1, want, tol, "restored")

@@ -3,6 +3,7 @@
 Modules:
   capi           -- ctypes binding of the C-ABI (include/ztcp_b200.h), loads libztcp_b200.so
   codec          -- GPU-native batch API: block tables, per-page metadata, stream-ordered
+  kvcache        -- operators on the hot pool: append, paged attention, attention weight per page, cold-page choice
   fused_ext      -- drop-in for the reference's native module (NativeCppFusedColdPageCodec._ext)
   cold_page_spec -- wire-format spec mirror (header, presets, geometry, payload sizes)
   session        -- GPU-native session codec: the reference wrapper's six methods on CUDA tensors
@@ -17,5 +18,5 @@ Modules:
 """
 from . import build, capi, cold_page_spec  # noqa: F401
 
-__all__ = ["build", "capi", "cold_page_spec", "codec", "errors", "fused_ext", "hooks", "keyring", "ledger", "offload",
+__all__ = ["build", "capi", "cold_page_spec", "codec", "errors", "fused_ext", "hooks", "keyring", "kvcache", "ledger", "offload",
            "session", "sharding", "workload"]

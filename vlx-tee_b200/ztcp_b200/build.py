@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libztcp_b200.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
 ]
 
 
@@ -31,7 +31,7 @@ def sources() -> list[str]:
 def _inputs() -> list[str]:
     return sources() + sorted(glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh"))) + [
         os.path.join(INCLUDE, "ztcp_b200.h"), os.path.join(INCLUDE, "ztcp_ledger.h"),
-        os.path.join(INCLUDE, "ztcp_measure.h")
+        os.path.join(INCLUDE, "ztcp_measure.h"), os.path.join(INCLUDE, "ztcp_kvcache.h")
     ]
 
 
