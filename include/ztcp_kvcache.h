@@ -36,6 +36,7 @@ extern "C" {
                                  [0, total_rows]: clamped to that range */
 #define ZTCP_SEQ_BAD_BLOCK 6  /* a block-table entry outside the pool: its page counts as masked; append: a slot
                                  or position out of range: the token is not written */
+#define ZTCP_SEQ_TIMEOUT 7    /* a wait inside the attention kernel did not end: the outputs are not valid */
 
 /* A paged KV cache as n_seqs sequences see it.  Sequence b holds kv_lens[b] tokens (its newest ones included);
  * token j lies in page block_tables[b * table_stride + j / num_tokens], row j % num_tokens.  Entries past the

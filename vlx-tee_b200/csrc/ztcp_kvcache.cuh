@@ -55,6 +55,11 @@ struct MassParams {
 void launch_attend(const AttendParams& P, bool bf16, cudaStream_t s);
 int attend_grid(const CacheParams& c);
 void attend_part_size(const CacheParams& c, int32_t* rows, int32_t* floats);
+// Tensor-core kernel for items of more than one MMA row block (ztcp_attend_tc.cu): whether the pool's pages fit its
+// loads, its grid and workspace bytes, and the launch (false: no tensor map could be made).
+bool attend_tc_fits(const CacheParams& c);
+int64_t attend_tc_workspace(const CacheParams& c, AttendParams* P);
+bool launch_attend_tc(const AttendParams& P, bool bf16, cudaStream_t s);
 void launch_page_mass(const MassParams& P, bool bf16, cudaStream_t s);
 
 // ------------------------------------------------------------------------------------------------

@@ -99,8 +99,15 @@ int32_t launched(const char* what) {
   return ZTCP_OK;
 }
 
-int64_t workspace_bytes(const ztcp::CacheParams& c, ztcp::AttendParams* P) {
+// One token's rows of a group fill at most one 16-row block: the general kernel reads K and V as fast as memory
+// gives them.  More rows go to the tensor-core kernel where the pool's pages fit its loads.
+bool use_tc(const ztcp::CacheParams& c, const ztcp_queries* q) {
+  return c.group * q->max_q_len > 16 && ztcp::attend_tc_fits(c);
+}
+
+int64_t workspace_bytes(const ztcp::CacheParams& c, const ztcp_queries* q, ztcp::AttendParams* P) {
   P->c = c;
+  if (use_tc(c, q)) return ztcp::attend_tc_workspace(c, P);
   P->grid = ztcp::attend_grid(c);
   ztcp::attend_part_size(c, &P->part_rows, &P->part_floats);
   return (int64_t)P->grid * 2 * P->part_floats * (int64_t)sizeof(float);
@@ -114,7 +121,7 @@ int64_t ztcp_attend_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queri
   ztcp::CacheParams c;
   ztcp::AttendParams P;
   if (to_params(cache, queries, &c) != ZTCP_OK || check_values(c) != ZTCP_OK) return -1;
-  const int64_t n = workspace_bytes(c, &P);
+  const int64_t n = workspace_bytes(c, queries, &P);
   if (n <= 0) {
     launched("ztcp_attend_workspace_bytes");
     return -1;
@@ -130,14 +137,17 @@ int32_t ztcp_attend_pages(const ztcp_kv_cache* cache, const ztcp_queries* querie
   if (rc != ZTCP_OK || (rc = check_values(c)) != ZTCP_OK) return rc;
   if (!out || !status || !workspace) return invalid("out, status and workspace must not be NULL");
   if (!aligned(out, 16) || !aligned(workspace, 16)) return invalid("out and workspace must be 16-byte aligned");
-  const int64_t need = workspace_bytes(c, &P);
+  const int64_t need = workspace_bytes(c, queries, &P);
   if (need <= 0) return launched("ztcp_attend_pages") != ZTCP_OK ? ZTCP_ECUDA : set_last_error(ZTCP_ECUDA, "no CUDA device");
   if (workspace_bytes_given < need) return invalid("workspace smaller than ztcp_attend_workspace_bytes");
   P.c.status = status;
   P.out = static_cast<uint16_t*>(out);
   P.lse = lse;
   P.part = static_cast<float*>(workspace);
-  ztcp::launch_attend(P, cache->dtype == ZTCP_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  const bool bf16 = cache->dtype == ZTCP_DTYPE_BF16;
+  if (!use_tc(c, queries)) ztcp::launch_attend(P, bf16, static_cast<cudaStream_t>(stream));
+  else if (!ztcp::launch_attend_tc(P, bf16, static_cast<cudaStream_t>(stream)))
+    return set_last_error(ZTCP_ECUDA, "cuTensorMapEncodeTiled failed");
   return launched("attend_kernel");
 }
 

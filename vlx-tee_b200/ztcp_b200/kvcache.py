@@ -28,6 +28,7 @@ from .codec import PreparedCall, _ptr, _require_cuda
 SEQ_OK = 0
 SEQ_BAD_LENGTH = 5  # ZTCP_SEQ_BAD_LENGTH
 SEQ_BAD_BLOCK = 6   # ZTCP_SEQ_BAD_BLOCK
+SEQ_TIMEOUT = 7     # ZTCP_SEQ_TIMEOUT: a wait inside the attention kernel did not end; the outputs are not valid
 
 # every symbol include/ztcp_kvcache.h declares
 KVCACHE_SYMBOLS = ("ztcp_attend_workspace_bytes", "ztcp_attend_pages", "ztcp_page_mass", "ztcp_append_tokens",
