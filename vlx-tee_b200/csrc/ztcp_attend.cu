@@ -16,6 +16,7 @@
 // masked tokens zero-filled so that whatever lies in unused rows of a page never enters a product).  QK^T: each warp
 // takes 8 of the tile's keys; scores cross shared memory; each warp then holds the softmax of all keys (one quad per
 // row pair) and multiplies P with its own slice of V's columns, so that no accumulator crosses warps.
+#include "../../include/ztcp_kvcache.h"
 #include "ztcp_kvcache.cuh"
 
 namespace ztcp {
@@ -23,7 +24,6 @@ namespace ztcp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kRows = 16;  // rows of a row tile: one MMA row block
 
 // ---- items and tiles ------------------------------------------------------------------------------
@@ -92,7 +92,10 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
   int64_t at;
   Spot spot;
   const SplitSpan S = locate(c.n_seqs, P.grid, [&](int b) { return seq_work(c, b, BK); }, [&](const SplitSpan& s) { return blockIdx.x < s.n ? s.begin(blockIdx.x) : (int64_t)-1; }, &at, &spot);
-  if (at < 0) return;
+  if (at < 0) {
+    if (tid == 0) P.cuts[blockIdx.x] = Cut{};
+    return;
+  }
   Cursor cons;
   cons.load(c, spot.seq, BK);
   cons.item = (int32_t)((at - spot.first) / cons.tiles);
@@ -147,6 +150,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
   bool fresh = true;
   bool whole = cons.tile == 0;  // the item's first tile is this CTA's
   int stage = 0;
+  Cut cut = {};
+  if (cons.tile > 0) cut.tiles[0] = (int32_t)(cons.left < cons.tiles - cons.tile ? cons.left : cons.tiles - cons.tile);
   while (cons.left > 0) {
     cp_async_wait<STAGES - 2>();
     __syncthreads();  // the tile has arrived; everyone is done with the stage that is refilled next
@@ -291,6 +296,15 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
           }
         }
       }
+      if (whole && !last) {  // the share ends inside the item
+        const int64_t end = S.begin(blockIdx.x + 1), start = end - cons.tile - 1;
+        cut.row0 = cons.s.row0;
+        cut.row = row;
+        cut.rows = rows;
+        cut.head = h;
+        cut.last = S.owner(start + cons.tiles - 1);
+        cut.tiles[1] = cons.tile + 1;
+      }
       fresh = true;
       whole = true;
     }
@@ -298,53 +312,110 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   cp_async_wait<0>();
+  if (tid == 0) P.cuts[blockIdx.x] = cut;
 }
 
-// Joins the partial results of each item that several CTAs share.  Block x looks at the border between CTAs x and
-// x + 1 and takes the item cut there if this is its first border; blocks y share its rows.  Also writes the
-// sequences' status.
+// Joins the partial results of the item that CTA x's share began and did not end (Cut): partial 1 of CTA x and
+// partial 0 of the CTAs behind it.  Blocks y share its rows.  A thread holds four value columns of one row; the
+// block's four groups of 64 threads take every fourth partial each, so that the loads of an item cut into many are
+// in flight together, and add up in shared memory in a fixed order.
+constexpr int kMergeThreads = 256, kMergeQuads = 64;
+
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads) attend_merge_kernel(const __grid_constant__ AttendParams P, int bk) {
+__global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __grid_constant__ AttendParams P) {
   const CacheParams& c = P.c;
-  int64_t w;
-  Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.grid, [&](int b) { return seq_work(c, b, bk); }, [&](const SplitSpan& s) { return (int)blockIdx.x + 1 < s.n ? s.begin(blockIdx.x + 1) : (int64_t)-1; }, &w, &spot);
-  if (blockIdx.y == 0)
-    for (int b = blockIdx.x * kWarps + (threadIdx.x >> 5); b < c.n_seqs; b += gridDim.x * kWarps)
-      write_seq_status(c, b, threadIdx.x & 31);
+  __shared__ float s_m[4][kMergeQuads], s_l[4][kMergeQuads];
+  __shared__ float4 s_o[4][kMergeQuads];
+  __shared__ int s_late;
+  const int tid = threadIdx.x, quad = tid & (kMergeQuads - 1), grp = tid / kMergeQuads;
+  const int x = blockIdx.x;
   cudaGridDependencySynchronize();
-  if (w < 0) return;
-  Cursor cur;
-  cur.load(c, spot.seq, bk);
-  cur.item = (int32_t)((w - spot.first) / cur.tiles);
-  const int64_t start = spot.first + (int64_t)cur.item * cur.tiles, end = start + cur.tiles;
-  if (w == start || S.begin(blockIdx.x) > start) return;
-  const int c0 = blockIdx.x, c1 = S.owner(end - 1);
-  const int rows = cur.rows(c), row = cur.row(c), h = cur.head(c);
-  const int64_t mo = (int64_t)P.part_rows * c.v_dim, lo = mo + P.part_rows;
-  // partial i of the item: CTA c0's second slot, then the first slots of the CTAs behind it
-  auto part = [&](int cta) { return P.part + (int64_t)(2 * cta + (cta == c0 ? 1 : 0)) * P.part_floats; };
-  const int half = c.v_dim / 2;
-  for (int i = blockIdx.y * kThreads + threadIdx.x; i < rows * half; i += gridDim.y * kThreads) {
-    const int r = i / half, col = (i - r * half) * 2;
-    float m = -INFINITY;
-    for (int k = c0; k <= c1; ++k) m = fmaxf(m, __ldcg(part(k) + mo + r));
-    const float z = m == -INFINITY ? 0.f : m;
-    float l = 0.f, a = 0.f, b = 0.f;
-#pragma unroll 4
-    for (int k = c0; k <= c1; ++k) {
-      const float* const q = part(k);
-      const float f = fast_exp2(__ldcg(q + mo + r) - z);
-      const float2 o = __ldcg(reinterpret_cast<const float2*>(q + r * c.v_dim + col));
-      l = fmaf(__ldcg(q + lo + r), f, l);
-      a = fmaf(o.x, f, a);
-      b = fmaf(o.y, f, b);
+  if (blockIdx.y == 0) {
+    if (tid == 0) s_late = 0;
+    __syncthreads();
+    for (int i = tid; i < P.grid; i += kMergeThreads)
+      if (__ldcg(&P.cuts[i].error)) s_late = 1;
+    __syncthreads();
+    for (int b = x * (kMergeThreads / 32) + (tid >> 5); b < c.n_seqs; b += gridDim.x * (kMergeThreads / 32)) {
+      if (!s_late) write_seq_status(c, b, tid & 31);
+      else if (tid % 32 == 0) c.status[b] = ZTCP_SEQ_TIMEOUT;
     }
-    const int tok = (row + r) / c.group, gh = (row + r) - tok * c.group;
-    const int64_t o = (cur.s.row0 + tok) * (int64_t)(c.kv_heads * c.group) + h * c.group + gh;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    *reinterpret_cast<uint32_t*>(P.out + o * c.v_dim + col) = pack2<BF16>(a * inv, b * inv);
-    if (col == 0 && P.lse) P.lse[o] = l == 0.f ? -INFINITY : fmaf(m, 0.693147180559945f, logf(l));
+  }
+  const int rows = __ldcg(&P.cuts[x].rows);
+  if (rows == 0) return;
+  const Cut cut = P.cuts[x];
+  const int n = cut.last - x + 1;
+  auto tiles = [&](int i) { return i == 0 ? cut.tiles[1] : __ldcg(&P.cuts[x + i].tiles[0]); };
+  // rounding to tiles may have left the whole item to one CTA, which has then written the result
+  int some = 0;
+  for (int i = tid; i < n; i += kMergeThreads) some += tiles(i) > 0;
+  if (__syncthreads_count(some > 0) < 2 && __syncthreads_count(some > 1) == 0) return;
+  const int64_t mo = (int64_t)P.part_rows * c.v_dim, lo = mo + P.part_rows;
+  auto part = [&](int i) { return P.part + (int64_t)(2 * (x + i) + (i == 0 ? 1 : 0)) * P.part_floats; };
+  const int quads = c.v_dim / 4;
+  for (int base = blockIdx.y * kMergeQuads; base < rows * quads; base += gridDim.y * kMergeQuads) {
+    const int i = base + quad;
+    const bool live = i < rows * quads;
+    const int r = live ? i / quads : 0, col = live ? (i - r * quads) * 4 : 0;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = grp; k0 < n; k0 += 16) {  // four partials in flight
+      float pm[4], pl[4];
+      float4 po[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = k0 + 4 * u;
+        pm[u] = -INFINITY;
+        pl[u] = 0.f;
+        po[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live && k < n && tiles(k) > 0) {
+          const float* const p = part(k);
+          pm[u] = __ldcg(p + mo + r);
+          pl[u] = __ldcg(p + lo + r);
+          po[u] = __ldcg(reinterpret_cast<const float4*>(p + (int64_t)r * c.v_dim + col));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float t = fmaxf(m, pm[u]);
+        const float z = t == -INFINITY ? 0.f : t;
+        const float f = fast_exp2(m - z), e = fast_exp2(pm[u] - z);
+        m = t;
+        l = l * f + pl[u] * e;
+        a.x = a.x * f + po[u].x * e;
+        a.y = a.y * f + po[u].y * e;
+        a.z = a.z * f + po[u].z * e;
+        a.w = a.w * f + po[u].w * e;
+      }
+    }
+    s_m[grp][quad] = m;
+    s_l[grp][quad] = l;
+    s_o[grp][quad] = a;
+    __syncthreads();
+    if (grp == 0 && live) {
+      float t = m;
+#pragma unroll
+      for (int u = 1; u < 4; ++u) t = fmaxf(t, s_m[u][quad]);
+      const float z = t == -INFINITY ? 0.f : t;
+      l = 0.f;
+      a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float f = fast_exp2(s_m[u][quad] - z);
+        const float4 o = s_o[u][quad];
+        l = fmaf(s_l[u][quad], f, l);
+        a.x = fmaf(o.x, f, a.x);
+        a.y = fmaf(o.y, f, a.y);
+        a.z = fmaf(o.z, f, a.z);
+        a.w = fmaf(o.w, f, a.w);
+      }
+      const int tok = (cut.row + r) / c.group, gh = (cut.row + r) - tok * c.group;
+      const int64_t o = (cut.row0 + tok) * (int64_t)(c.kv_heads * c.group) + cut.head * c.group + gh;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      *reinterpret_cast<uint2*>(P.out + o * c.v_dim + col) = make_uint2(pack2<BF16>(a.x * inv, a.y * inv), pack2<BF16>(a.z * inv, a.w * inv));
+      if (col == 0 && P.lse) P.lse[o] = l == 0.f ? -INFINITY : fmaf(t, 0.693147180559945f, logf(l));
+    }
+    __syncthreads();
   }
 }
 
@@ -377,36 +448,32 @@ void launch_kernel(const AttendParams& P, const Variant& v, cudaStream_t s) {
 
 }  // namespace
 
-int attend_grid(const CacheParams& c) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return sms * pick(c).per_sm;
-}
-
-void attend_part_size(const CacheParams& c, int32_t* rows, int32_t* floats) {
-  *rows = kRows;
-  *floats = kRows * (c.v_dim + 2);
-}
+AttendShape attend_shape(const CacheParams& c, int sms) { return {sms * pick(c).per_sm, kRows, kRows * (c.v_dim + 2)}; }
 
 void launch_attend(const AttendParams& P, bool bf16, cudaStream_t s) {
   const Variant v = pick(P.c);
   if (P.c.head_dim <= 128) bf16 ? launch_kernel<true, 2, 1, 3>(P, v, s) : launch_kernel<false, 2, 1, 3>(P, v, s);
   else if (P.c.head_dim <= 256) bf16 ? launch_kernel<true, 4, 1, 3>(P, v, s) : launch_kernel<false, 4, 1, 3>(P, v, s);
   else bf16 ? launch_kernel<true, 8, 2, 5>(P, v, s) : launch_kernel<false, 8, 2, 5>(P, v, s);
-  if (cudaPeekAtLastError() != cudaSuccess) return;
-  // The merge's prologue overlaps the end of the kernel before it (programmatic dependent launch).
+}
+
+void launch_attend_merge(const AttendParams& P, bool bf16, int64_t rows, cudaStream_t s) {
+  // One block per border and 64 quads of columns, at most 32 blocks a border.  The launch overlaps the end of the
+  // kernel before it (programmatic dependent launch).
+  const int64_t quads = (rows < P.part_rows ? rows : P.part_rows) * (P.c.v_dim / 4);
+  int64_t y = (quads + kMergeQuads - 1) / kMergeQuads;
+  if (y > 32) y = 32;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(P.grid > 1 ? P.grid - 1 : 1, 2);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(P.grid, (unsigned)y);
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (bf16) cudaLaunchKernelEx(&cfg, attend_merge_kernel<true>, P, v.bk);
-  else cudaLaunchKernelEx(&cfg, attend_merge_kernel<false>, P, v.bk);
+  if (bf16) cudaLaunchKernelEx(&cfg, attend_merge_kernel<true>, P);
+  else cudaLaunchKernelEx(&cfg, attend_merge_kernel<false>, P);
 }
 
 }  // namespace ztcp

@@ -34,13 +34,28 @@ struct CacheParams {
   int32_t* status;
 };
 
+// What a CTA leaves to join.  Its share of the line begins and ends inside items: the part of an item that began
+// before the share is its partial 0, the part of one that goes on behind it partial 1.
+struct alignas(16) Cut {
+  int64_t row0;                    // partial 1's item: the sequence's first row,
+  int32_t row, rows, head, last;   // its first packed row, rows (0: no such item), KV head, and last CTA
+  int32_t tiles[2];                // tiles in each partial (0: nothing was written)
+  int32_t error, reserved[5];      // a wait of the CTA ran out
+};
+
 struct AttendParams {
   CacheParams c;
   uint16_t* out;   // [total_rows, kv_heads * group, v_dim]
   float* lse;      // [total_rows, kv_heads * group] or null
-  float* part;     // partial results of items that several CTAs share (see SplitSpan)
-  int32_t part_rows, part_floats;  // rows of a partial, and its size in floats
+  Cut* cuts;       // one per CTA
+  float* part;     // two per CTA, part_floats each: o [part_rows][v_dim], m [part_rows], l [part_rows]
+  int32_t part_rows, part_floats;
   int32_t grid;    // CTAs that share the work
+};
+
+// Grid and partials of a kernel.
+struct AttendShape {
+  int32_t grid, part_rows, part_floats;
 };
 
 struct MassParams {
@@ -52,14 +67,18 @@ struct MassParams {
   int32_t unit_pages;  // whole pages per unit of work
 };
 
+// The attention kernels: whether they can take a call, their shape, and the launch (false: no tensor map could be
+// made).  ztcp_attend.cu takes every call; ztcp_attend_tc.cu items of many rows, ztcp_attend_decode.cu of few.
+AttendShape attend_shape(const CacheParams& c, int sms);
 void launch_attend(const AttendParams& P, bool bf16, cudaStream_t s);
-int attend_grid(const CacheParams& c);
-void attend_part_size(const CacheParams& c, int32_t* rows, int32_t* floats);
-// Tensor-core kernel for items of more than one MMA row block (ztcp_attend_tc.cu): whether the pool's pages fit its
-// loads, its grid and workspace bytes, and the launch (false: no tensor map could be made).
 bool attend_tc_fits(const CacheParams& c);
-int64_t attend_tc_workspace(const CacheParams& c, AttendParams* P);
+AttendShape attend_tc_shape(const CacheParams& c, int sms);
 bool launch_attend_tc(const AttendParams& P, bool bf16, cudaStream_t s);
+bool attend_decode_fits(const CacheParams& c);
+AttendShape attend_decode_shape(const CacheParams& c, int sms, int64_t rows);
+bool launch_attend_decode(const AttendParams& P, bool bf16, cudaStream_t s);
+// Joins what the kernel before it left to join, and writes the sequences' status; `rows`: of an item, at most.
+void launch_attend_merge(const AttendParams& P, bool bf16, int64_t rows, cudaStream_t s);
 void launch_page_mass(const MassParams& P, bool bf16, cudaStream_t s);
 
 // ------------------------------------------------------------------------------------------------

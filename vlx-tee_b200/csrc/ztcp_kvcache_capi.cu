@@ -99,18 +99,32 @@ int32_t launched(const char* what) {
   return ZTCP_OK;
 }
 
-// One token's rows of a group fill at most one 16-row block: the general kernel reads K and V as fast as memory
-// gives them.  More rows go to the tensor-core kernel where the pool's pages fit its loads.
-bool use_tc(const ztcp::CacheParams& c, const ztcp_queries* q) {
-  return c.group * q->max_q_len > 16 && ztcp::attend_tc_fits(c);
+// The kernel of a call.  Items of at most 64 rows (of one token or a few, and a group) leave the tensor cores idle
+// whatever is done, so the decode kernel turns the products over and reads K and V at memory speed; more rows take
+// the chunk kernel's 256-row items.  What their loads cannot take (odd page sizes, other head dims) goes to the
+// general kernel.
+enum class Kernel { general, chunk, decode };
+
+Kernel pick_kernel(const ztcp::CacheParams& c, const ztcp_queries* q) {
+  const int64_t rows = c.group * q->max_q_len;
+  if (ztcp::attend_decode_fits(c) && (rows <= 16 || !ztcp::attend_tc_fits(c))) return Kernel::decode;
+  return rows > 16 && ztcp::attend_tc_fits(c) ? Kernel::chunk : Kernel::general;
 }
 
-int64_t workspace_bytes(const ztcp::CacheParams& c, const ztcp_queries* q, ztcp::AttendParams* P) {
+// Fills the workspace-dependent part of P for a workspace at `base`; returns the bytes it takes, 0 without a device.
+int64_t plan(Kernel k, const ztcp::CacheParams& c, const ztcp_queries* q, void* base, ztcp::AttendParams* P) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  const ztcp::AttendShape s = k == Kernel::chunk    ? ztcp::attend_tc_shape(c, sms)
+                              : k == Kernel::decode ? ztcp::attend_decode_shape(c, sms, c.group * q->max_q_len)
+                                                    : ztcp::attend_shape(c, sms);
   P->c = c;
-  if (use_tc(c, q)) return ztcp::attend_tc_workspace(c, P);
-  P->grid = ztcp::attend_grid(c);
-  ztcp::attend_part_size(c, &P->part_rows, &P->part_floats);
-  return (int64_t)P->grid * 2 * P->part_floats * (int64_t)sizeof(float);
+  P->grid = s.grid;
+  P->part_rows = s.part_rows;
+  P->part_floats = s.part_floats;
+  P->cuts = static_cast<ztcp::Cut*>(base);
+  P->part = reinterpret_cast<float*>(P->cuts + s.grid);
+  return s.grid * ((int64_t)sizeof(ztcp::Cut) + 2 * (int64_t)s.part_floats * (int64_t)sizeof(float));
 }
 
 }  // namespace
@@ -121,7 +135,7 @@ int64_t ztcp_attend_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queri
   ztcp::CacheParams c;
   ztcp::AttendParams P;
   if (to_params(cache, queries, &c) != ZTCP_OK || check_values(c) != ZTCP_OK) return -1;
-  const int64_t n = workspace_bytes(c, queries, &P);
+  const int64_t n = plan(pick_kernel(c, queries), c, queries, nullptr, &P);
   if (n <= 0) {
     launched("ztcp_attend_workspace_bytes");
     return -1;
@@ -137,18 +151,22 @@ int32_t ztcp_attend_pages(const ztcp_kv_cache* cache, const ztcp_queries* querie
   if (rc != ZTCP_OK || (rc = check_values(c)) != ZTCP_OK) return rc;
   if (!out || !status || !workspace) return invalid("out, status and workspace must not be NULL");
   if (!aligned(out, 16) || !aligned(workspace, 16)) return invalid("out and workspace must be 16-byte aligned");
-  const int64_t need = workspace_bytes(c, queries, &P);
+  const Kernel kernel = pick_kernel(c, queries);
+  const int64_t need = plan(kernel, c, queries, workspace, &P);
   if (need <= 0) return launched("ztcp_attend_pages") != ZTCP_OK ? ZTCP_ECUDA : set_last_error(ZTCP_ECUDA, "no CUDA device");
   if (workspace_bytes_given < need) return invalid("workspace smaller than ztcp_attend_workspace_bytes");
   P.c.status = status;
   P.out = static_cast<uint16_t*>(out);
   P.lse = lse;
-  P.part = static_cast<float*>(workspace);
   const bool bf16 = cache->dtype == ZTCP_DTYPE_BF16;
-  if (!use_tc(c, queries)) ztcp::launch_attend(P, bf16, static_cast<cudaStream_t>(stream));
-  else if (!ztcp::launch_attend_tc(P, bf16, static_cast<cudaStream_t>(stream)))
-    return set_last_error(ZTCP_ECUDA, "cuTensorMapEncodeTiled failed");
-  return launched("attend_kernel");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  bool made = true;
+  if (kernel == Kernel::general) ztcp::launch_attend(P, bf16, s);
+  else made = kernel == Kernel::chunk ? ztcp::launch_attend_tc(P, bf16, s) : ztcp::launch_attend_decode(P, bf16, s);
+  if (!made) return set_last_error(ZTCP_ECUDA, "cuTensorMapEncodeTiled failed");
+  if ((rc = launched("attend_kernel")) != ZTCP_OK) return rc;
+  ztcp::launch_attend_merge(P, bf16, c.group * queries->max_q_len, s);
+  return launched("attend_merge_kernel");
 }
 
 int32_t ztcp_page_mass(const ztcp_kv_cache* cache, const ztcp_queries* queries, const float* lse, const float* mass,

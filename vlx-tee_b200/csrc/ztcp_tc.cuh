@@ -1,0 +1,277 @@
+// ztcp_tc.cuh -- what the tensor-core kernels of the paged cache share: PTX wrappers, shared-memory and instruction
+// descriptors, the line of items that CTAs share, and the pool's tensor maps.
+#pragma once
+#include <cuda.h>
+
+#include "ztcp_kvcache.cuh"
+
+namespace ztcp {
+
+constexpr int kKeys = 128;                           // keys per tile
+constexpr int kGroupBytes = kKeys * 128;             // a tile's 64-column group: 128 rows of 128 bytes
+constexpr long long kWaitCycles = 4000000000ll;      // bound of a wait, about two seconds
+
+// Boxes of the pool's TMA loads.
+struct PoolBoxes {
+  int32_t rows;       // rows of one box: a page, or 128 of a larger one (8 to 128, a power of two)
+  int32_t shift;      // its logarithm
+  int32_t pool_rows;  // rows of the tensor maps; a load at this row is filled with zeros
+};
+
+#if defined(__CUDACC__)
+
+// ---- PTX ------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok;
+}
+// False when the wait ran out, here or (dead set) elsewhere in the CTA.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try(bar, parity)) return true;
+  const long long start = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*dead) return false;
+    if (clock64() - start > kWaitCycles) {
+      *dead = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// The same for a whole warp: all lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, dead));
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr) : "memory");
+}
+// Waits for the thread's TMEM loads; the values pass through, so that no use of them can move above the wait.
+__device__ __forceinline__ void tmem_ready32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), 
+               "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle, descriptor version 1.  K-major operands (Q, K: 64 columns per
+// 128-byte row): 8-row groups 1,024 bytes apart.  MN-major operand (V: 64 output columns per row of a key): 8-key
+// groups 1,024 bytes apart, the next 64 columns `lbo` bytes on.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: fp32 accumulators, both operands of the pool's type, M = 128.
+__device__ __forceinline__ uint32_t inst_desc(bool bf16, int n, bool a_mn_major, bool b_mn_major) {
+  const uint32_t t = bf16 ? 1 : 0;
+  return 1u << 4 | t << 7 | t << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+// ---- the line of items ----------------------------------------------------------------------------
+// Items of up to ROWS (token, head-of-the-group) rows of one sequence and KV head form one line, sequence by
+// sequence, row tile by row tile, head by head, that the CTAs share evenly, in units of keys x group: an item's
+// length is what its last row sees plus its own rows, which sums over row tiles in closed form.  Shares are rounded
+// to tiles of 128 keys.
+template <int ROWS>
+struct Line {
+  int64_t head;  // units of row tile 0's items, without the rows' share
+  int64_t step;  // what each further row tile adds
+  int32_t row_tiles, heads;
+  __device__ __forceinline__ int64_t cost(int rt) const { return head + (rt + 1) * step + ROWS; }
+  __device__ __forceinline__ int64_t before(int rt) const {  // units of one head's row tiles [0, rt)
+    return rt * (head + ROWS) + step * ((int64_t)rt * (rt + 1) / 2);
+  }
+  __device__ __forceinline__ int64_t total() const { return before(row_tiles) * heads; }
+};
+template <int ROWS>
+__device__ __forceinline__ Line<ROWS> line_of(const CacheParams& c, const Seq& s) {
+  Line<ROWS> l;
+  l.row_tiles = (int)(((int64_t)s.q_len * c.group + ROWS - 1) / ROWS);
+  l.heads = c.kv_heads;
+  const int64_t seen = c.causal ? (s.kv_len > s.q_len ? s.kv_len - s.q_len : 0) : s.kv_len;
+  l.head = seen * c.group;
+  l.step = c.causal ? ROWS : 0;
+  return l;
+}
+template <int ROWS>
+__device__ __forceinline__ int64_t seq_work(const CacheParams& c, int b) {
+  return line_of<ROWS>(c, load_seq(c, b)).total();
+}
+
+// An item and the tiles [ta, tb) of its `nt` that a share [pos, end) of the line covers.
+template <int ROWS>
+struct Item {
+  Seq s;
+  Line<ROWS> line;
+  int64_t seq_start, start, cost;
+  int32_t b, rt, h, nt, ta, tb, rows, row;
+  bool inside;  // the share begins inside the item
+  __device__ __forceinline__ void load_seq_at(const CacheParams& c, int seq, int64_t first) {
+    b = seq;
+    seq_start = first;
+    s = load_seq(c, seq);
+    line = line_of<ROWS>(c, s);
+  }
+  __device__ __forceinline__ void find(const CacheParams& c, int64_t pos) {  // pos lies in sequence b
+    const int64_t x = pos - seq_start;
+    int lo = 0, hi = line.row_tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (line.before(mid) * line.heads <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    rt = lo;
+    cost = line.cost(rt);
+    h = (int)((x - line.before(rt) * line.heads) / cost);
+    start = seq_start + line.before(rt) * line.heads + h * cost;
+    row = rt * ROWS;
+    rows = min(s.q_len * c.group - row, ROWS);
+    const int vis = visible_keys(c, s, (row + rows - 1) / c.group);
+    nt = vis > 0 ? (vis + kKeys - 1) / kKeys : 1;
+  }
+  __device__ __forceinline__ int tile_at(int64_t pos) const { return (int)((pos - start) * nt / cost); }
+  __device__ __forceinline__ void clip(int64_t pos, int64_t end) {
+    inside = pos > start;
+    ta = tile_at(pos);
+    tb = end >= start + cost ? nt : tile_at(end);
+  }
+};
+
+// Walks the items of a share; every role of the CTA walks the same ones.
+template <int ROWS>
+struct Walk {
+  Item<ROWS> it;
+  int64_t pos, end;
+  __device__ __forceinline__ void begin(const CacheParams& c, const Spot& spot, int64_t p, int64_t e) {
+    pos = p;
+    end = e;
+    it.load_seq_at(c, spot.seq, spot.first);
+  }
+  __device__ __forceinline__ bool next(const CacheParams& c) {  // the next item with tiles, in `it`
+    while (pos < end) {
+      while (pos >= it.seq_start + it.line.total()) it.load_seq_at(c, it.b + 1, it.seq_start + it.line.total());
+      it.find(c, pos);
+      it.clip(pos, end);
+      pos = min(end, it.start + it.cost);
+      if (it.ta < it.tb) return true;
+    }
+    return false;
+  }
+};
+
+
+// The CTA's record of what it left to join (see Cut): the item that its share's end cuts, if that item began in the
+// share, and the tiles of its two partials.
+template <int ROWS>
+__device__ __forceinline__ void write_cut(const AttendParams& P, const SplitSpan& S, const CacheParams& c, const Spot& spot, int64_t begin,
+                                          int32_t error) {
+  Cut cut = {};
+  cut.error = error;
+  const int64_t end = S.begin(blockIdx.x + 1);
+  Item<ROWS> it;
+  it.load_seq_at(c, spot.seq, spot.first);
+  it.find(c, begin);
+  it.clip(begin, end);
+  if (it.inside) cut.tiles[0] = it.tb - it.ta;
+  if (end < S.total) {  // the item that holds the share's last unit
+    while (end - 1 >= it.seq_start + it.line.total()) it.load_seq_at(c, it.b + 1, it.seq_start + it.line.total());
+    it.find(c, end - 1);
+    if (it.start >= begin && it.start + it.cost > end) {
+      it.clip(it.start, end);
+      cut.tiles[1] = it.tb;
+      cut.row0 = it.s.row0;
+      cut.row = it.row;
+      cut.rows = it.rows;
+      cut.head = it.h;
+      cut.last = S.owner(it.start + it.cost - 1);
+    }
+  }
+  P.cuts[blockIdx.x] = cut;
+}
+
+#endif  // __CUDACC__
+
+// ---- host -----------------------------------------------------------------------------------------
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+inline EncodeTiled encode_tiled() {  // the driver's entry point, looked up once (the library links no libcuda)
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+
+// The pool as [rows][heads][head_dim], boxes of b.rows rows x one head x 64 columns.
+inline bool pool_map(CUtensorMap* map, const void* pool, const CacheParams& c, bool bf16, const PoolBoxes& b) {
+  const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.kv_heads, (cuuint64_t)b.pool_rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.kv_heads * c.head_dim * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)b.rows}, elem[3] = {1, 1, 1};
+  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(pool), dims, strides,
+                        box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+
+// Pages must fill TMA boxes of whole swizzle groups (8 rows) that fit a tile of 128 keys evenly.
+inline bool pages_fit(const CacheParams& c) {
+  const int T = c.page_tokens;
+  return T % 8 == 0 && (T <= kKeys ? kKeys % T == 0 : T % kKeys == 0) && c.pool_pages * T < ((int64_t)1 << 31) && encode_tiled() != nullptr;
+}
+inline PoolBoxes pool_boxes(const CacheParams& c) {
+  PoolBoxes b;
+  b.rows = c.page_tokens < kKeys ? c.page_tokens : kKeys;
+  b.shift = 0;
+  while (1 << b.shift < b.rows) ++b.shift;
+  b.pool_rows = (int32_t)(c.pool_pages * c.page_tokens);
+  return b;
+}
+
+}  // namespace ztcp
