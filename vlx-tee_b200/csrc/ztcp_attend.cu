@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
 
   int64_t at;
   Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.grid, [&](int b) { return seq_work(c, b, BK); }, [&](const SplitSpan& s) { return blockIdx.x < s.n ? s.begin(blockIdx.x) : (int64_t)-1; }, &at, &spot);
+  const SplitSpan S = locate(c.n_seqs, P.grid, [&](int b) { return seq_work(c, b, BK); }, &at, &spot);
   if (at < 0) {
     if (tid == 0) P.cuts[blockIdx.x] = Cut{};
     return;

@@ -10,10 +10,12 @@
 // tcgen05.mma by one thread: about 500 instructions per warp where a 16-row mma.sync tile needed 4,000 (measured:
 // 359 us for 48 sequences of up to 8,192 tokens, 32/8 heads of 128, against 144 us to read K and V once).
 //
-// Warps.  0-3: softmax, a thread per key; 4: one thread issues the products; 5: TMA.  K and V tiles pass a ring of
-// slots of up to 128 columns, one box per page.  A row's maximum over the tile is a redux per warp and an exchange
-// through shared memory; sums stay per thread until the item ends.  O^T is rescaled only when a maximum has grown
-// by more than 2^8 over the one in use.  For single-buffer pools V's columns are those of the K tile itself.
+// Warps.  0-3 and 4-7: softmax of every other tile, a thread per key, each group with its own O^T, maxima and sums (a
+// tile's softmax takes longer than its products and its share of the memory's time; two of them side by side do not);
+// 8: one thread issues the products; 9: TMA.  K and V tiles pass a ring of slots of up to 128 columns, one box per
+// page.  A row's maximum over the tile is a redux per warp and an exchange through shared memory; sums stay per
+// thread until the item ends.  O^T is rescaled only when a maximum has grown by more than 2^8 over the one in use.
+// For single-buffer pools V's columns are those of the K tile itself.
 //
 // Work, joining of shared items and bounded waits as in ztcp_attend_tc.cu.
 #include "ztcp_tc.cuh"
@@ -22,9 +24,10 @@ namespace ztcp {
 
 namespace {
 
-constexpr int kThreads = 192;
-constexpr int kMmaWarp = 4, kTmaWarp = 5;
-constexpr int kBars = 40;  // barrier slots at the start of shared memory
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kTurns = 4;
+constexpr int kBars = 48;  // barrier slots at the start of shared memory
 
 struct DecodeParams {
   AttendParams a;
@@ -34,25 +37,46 @@ struct DecodeParams {
 // KG: 64-column groups of K; MB: 128-column blocks of V; N: rows of an item.
 template <int KG, int MB, int N, bool SHARED>
 struct Shape {
+  // Keys of a tile.  A single-buffer pool's rows are wide: 64 keys, so that two tiles fit the ring; S^T then has 64
+  // rows, 16 in the first lanes of each warp's 32.
+  static constexpr int kTileKeys = SHARED ? 64 : kKeys;
+  static constexpr int kGroupBytes = kTileKeys * 128;                   // one column group of a tile
   static constexpr int kGroups = KG == 1 ? 1 : 2;                       // column groups of a slot
   static constexpr int kSlotBytes = kGroups * kGroupBytes;
   static constexpr int kKSlots = SHARED ? 1 + MB : (KG + 1) / 2;        // slots of a tile's K (shared: group 0, then V's pairs)
   static constexpr int kTileSlots = SHARED ? kKSlots : 2 * kKSlots;
   static constexpr int kQBytes = KG * N * 128;
-  static constexpr int kPBytes = N * kKeys * 2;
-  static constexpr int kSlots = (232448 - 4096 - kQBytes - kPBytes) / kSlotBytes;
-  static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kQBytes + kPBytes;
-  static constexpr int kCols = (2 + MB) * N <= 64 ? 64 : ((2 + MB) * N <= 128 ? 128 : 256);
-  static_assert(kSlots >= kTileSlots && 2 * kSlots + 8 <= kBars && (2 + MB) * N <= kCols, "shape");
+  static constexpr int kPBlock = kTileKeys * 32;                        // P^T of 16 rows
+  static constexpr int kPBytes = N / 16 * kPBlock;
+  static constexpr int kTail = 2 * kPBytes + kQBytes;
+  static constexpr int kSlots = (232448 - 8192 - kTail) / kSlotBytes;
+  static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kTail;
+  static constexpr int kCols = (2 + 2 * MB) * N <= 64 ? 64 : ((2 + 2 * MB) * N <= 128 ? 128 : ((2 + 2 * MB) * N <= 256 ? 256 : 512));
+  // the next tile's K and this tile's V share the ring
+  static_assert(kSlots >= (SHARED ? 2 * kTileSlots : kTileSlots + kKSlots) && 2 * kSlots + 12 + 2 * kJobs <= kBars && (2 + 2 * MB) * N <= kCols, "shape");
   // first column group, and number of groups, of slot s of a tile's K
-  static __device__ __forceinline__ int group(int s) { return SHARED ? (s == 0 ? 0 : 2 * s - 1) : s * kGroups; }
-  static __device__ __forceinline__ int groups(int s) { return SHARED && s == 0 ? 1 : kGroups; }
+  static __device__ __forceinline__ constexpr int group(int s) { return SHARED ? (s == 0 ? 0 : 2 * s - 1) : s * kGroups; }
+  static __device__ __forceinline__ constexpr int groups(int s) { return SHARED && s == 0 ? 1 : kGroups; }
 };
 
 __device__ __forceinline__ float warp_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Lane n gets the sum of v[n] over the warp.
+template <int N>
+__device__ __forceinline__ float lane_sums(float (&v)[N], int lane) {
+#pragma unroll
+  for (int d = N / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < d; ++i) {
+      const bool up = lane & d;
+      const float keep = up ? v[i + d] : v[i], send = up ? v[i] : v[i + d];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+    }
+  return N == 32 ? v[0] : v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
 
 template <int N>
@@ -78,21 +102,21 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t* r) {
                  "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
-// P^T, rows of the product contiguous per key: 32-byte swizzle, 8-key groups 256 bytes apart, the next 16 rows one
-// block of 128 keys (4,096 bytes) on.
-__device__ __forceinline__ uint64_t p_desc(uint32_t addr) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(kKeys * 32 >> 4) << 16 | (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)6 << 61;
-}
-
 template <bool BF16, int KG, int MB, int N, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Sh = Shape<KG, MB, N, SHARED>;
-  constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kKS = Sh::kKSlots;
+  constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kKS = Sh::kKSlots, kTileKeys = Sh::kTileKeys;
+  constexpr int kGroupBytes = Sh::kGroupBytes, kKGroups = Sh::kGroups;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
-  __shared__ float4 s_max[2][N], s_sum[N];  // per row: one value of each softmax warp
+  __shared__ float4 s_max[2][2][N], s_sum[2][N];  // per group (and tile, by turns) and row: one value of each warp
+  __shared__ float s_top[2][N];                   // per group and row: the maximum in use
+  __shared__ float2 s_mix[N];                     // per row: what the groups' O count
+  __shared__ int64_t s_row[kTurns][N];            // per item, by turns, and row: the row of the output,
+  __shared__ int32_t s_lim[2][kTurns][N];         // and (per group) the keys that it sees
+  __shared__ Job s_jobs[kJobs];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   volatile int* const dead = &dead_s;
@@ -102,13 +126,14 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   const uint32_t qbuf = ring + kSlots * Sh::kSlotBytes, pbuf = qbuf + Sh::kQBytes;
   auto full = [&](uint32_t s) { return bars + s * 8; };
   auto empty = [&](uint32_t s) { return bars + (kSlots + s) * 8; };
-  const uint32_t q_full = bars + 2 * kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 8, meet = pv_done + 8,
-                 drain = meet + 8;
+  // q_full: Q is there; s_full, p_full, pv_done, meet: per group; summed, read: the second group's sums, and O, at an
+  // item's end
+  const uint32_t q_full = bars + 2 * kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, meet = pv_done + 16,
+                 summed = meet + 16, read = summed + 8, job_full = read + 8, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
 
   int64_t at;
   Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<N>(c, b); },
-                             [&](const SplitSpan& s) { return blockIdx.x < s.n ? s.begin(blockIdx.x) : (int64_t)-1; }, &at, &spot);
+  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<N>(c, b); }, &at, &spot);
   if (at < 0) {
     if (tid == 0) P.a.cuts[blockIdx.x] = Cut{};
     return;
@@ -119,12 +144,19 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(q_full, 128);
-    mbar_init(s_full, 1);
-    mbar_init(s_full + 8, 1);
-    mbar_init(p_full, 128);
-    mbar_init(pv_done, 1);
-    mbar_init(meet, 4);
+    mbar_init(q_full, 256);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full + 8 * g, 1);
+      mbar_init(p_full + 8 * g, 128);
+      mbar_init(pv_done + 8 * g, 1);
+      mbar_init(meet + 8 * g, 4);
+    }
+    mbar_init(summed, 4);
+    mbar_init(read, 4);
+    for (int e = 0; e < kJobs; ++e) {
+      mbar_init(job_full + 8 * e, 1);
+      mbar_init(job_empty + 8 * e, 9);
+    }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -136,22 +168,24 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-
-  Walk<N> walk;
-  walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+  cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up meanwhile; it waits for this one's end
 
   if (warp == kTmaWarp) {
     // ---- TMA: a tile's slots in turn through the ring; lane p fetches page p of the tile ------------
-    const int per_tile = kKeys / P.box.rows;
+    const int per_tile = kTileKeys / P.box.rows;
     uint32_t pos = 0;
-    bool ok = true;
-    while (ok && walk.next(c)) {
-      const Item<N>& it = walk.it;
-      for (int t = it.ta; ok && t < it.tb; ++t) {
-        const int j = t * kKeys + lane * P.box.rows;
+    Publisher<N, kTileKeys> pub;
+    pub.walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+    pub.cut = Cut{};
+    pub.n = 0;
+    Job job, then;
+    bool ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job);
+    while (ok && job.ta < job.tb) {
+      for (int t = job.ta; ok && t < job.tb; ++t) {
+        const int j = t * kTileKeys + lane * P.box.rows;
         int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
-        if (lane < per_tile && j < it.s.kv_len) {
-          const int64_t r = pool_row(c, it.b, j);
+        if (lane < per_tile && j < job.kv_len) {
+          const int64_t r = pool_row(c, job.b, j);
           if (r >= 0) row = (int32_t)r;
         }
 #pragma unroll
@@ -169,70 +203,82 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
           __syncwarp();
           if (lane < per_tile)
             for (int g = 0; g < n; ++g)
-              tma_load(ring + slot * Sh::kSlotBytes + g * kGroupBytes + lane * P.box.rows * 128, isv ? &vmap : &kmap, (g0 + g) * 64, it.h, row,
+              tma_load(ring + slot * Sh::kSlotBytes + g * kGroupBytes + lane * P.box.rows * 128, isv ? &vmap : &kmap, (g0 + g) * 64, job.head, row,
                        full(slot));
         }
+        // the item behind this one, looked up once this one's first loads are out
+        if (ok && t == job.ta) ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &then);
       }
+      job = then;
     }
-    if (lane == 0) write_cut<N>(P.a, S, c, spot, at, 0);
+    if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
     if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
       int none = 0;
       for (uint32_t p = pos > kSlots ? pos - kSlots : 0; p < pos; ++p) mbar_wait(full(p % kSlots), (p / kSlots) & 1, &none);
     }
   } else if (warp == kMmaWarp) {
-    // ---- products ----------------------------------------------------------------------------------
-    if (lane == 0) {
-      const uint32_t qk = inst_desc(BF16, N, false, false), pv = inst_desc(BF16, N, true, true);
-      const int ksteps = c.head_dim / 16;
+    // ---- products: one thread ------------------------------------------------------------------------
+    if (elect_one()) {
+      // P^T: 32-byte swizzle, rows of the product contiguous per key, 8-key groups 256 bytes apart, the next 16 rows
+      // one block on.  V: the next 64 columns one group on (KG = 1: the block's upper half repeats rows nobody reads).
+      constexpr uint32_t kHi = desc_hi(1024, kSwizzle128), kPHi = desc_hi(256, kSwizzle32);
+      constexpr uint32_t kVLbo = KG == 1 ? 1024 : kGroupBytes;
+      const uint32_t qk = inst_desc(BF16, kTileKeys, N, false, false), pv = inst_desc(BF16, 128, N, true, true);
+      const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kVLbo), q_lo = desc_lo(qbuf, 16), p_lo = desc_lo(pbuf, Sh::kPBlock);
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t n) {  // the n-th completion (from 0)
         ok = ok && mbar_wait(bar, n & 1, dead);
         return ok;
       };
       auto scores = [&](uint32_t step) {  // S^T of the CTA's tile `step`
+#pragma unroll
         for (int s = 0; s < kKS; ++s) {
           const uint32_t pos = step * kTS + s, slot = pos % kSlots;
           if (!wait(full(slot), pos / kSlots)) return;
           tc_fence_after();
-          const uint32_t kb = ring + slot * Sh::kSlotBytes;
-          const int g0 = Sh::group(s), n = Sh::groups(s);
-          for (int g = 0; g < n; ++g) {
-            const uint32_t qb = qbuf + (g0 + g) * N * 128;
-            for (int k = 0; k < 4 && (g0 + g) * 4 + k < ksteps; ++k)
-              mma_ss(tmem + (step & 1) * N, smem_desc(kb + g * kGroupBytes + k * 32, 16, 1024), smem_desc(qb + k * 32, 16, 1024), qk,
-                     g0 + g > 0 || k > 0);
-          }
-          if (!SHARED || s == 0) tc_commit(empty(slot));
+          const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (step & 1) * N, done = empty(slot),
+                         sbar = s_full + 8 * (step & 1);
+#pragma unroll
+          for (int g = 0; g < Sh::groups(s); ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ss(d, a + ((g * kGroupBytes + k * 32) >> 4), kHi, q_lo + (((Sh::group(s) + g) * N * 128 + k * 32) >> 4), kHi, qk,
+                     Sh::group(s) + g > 0 || k > 0);
+          if (!SHARED || s == 0) tc_commit(done);
+          if (s == kKS - 1) tc_commit(sbar);
         }
-        tc_commit(s_full + 8 * (step & 1));
       };
       auto values = [&](uint32_t step, bool acc) {  // O^T += V^T P^T
+#pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           const uint32_t pos = step * kTS + (SHARED ? 1 : kKS) + mb, slot = pos % kSlots;
           if (!wait(full(slot), pos / kSlots)) return;
           tc_fence_after();
-          const uint32_t vb = ring + slot * Sh::kSlotBytes;
-          // one group of columns only (KG = 1): the block's upper half repeats rows nobody reads
-          for (int k = 0; k < kKeys / 16; ++k)
-            mma_ss(tmem + (2 + mb) * N, smem_desc(vb + k * 2048, KG == 1 ? 1024 : kGroupBytes, 1024), p_desc(pbuf + k * 512), pv, acc || k > 0);
-          tc_commit(empty(slot));
+          const uint32_t a = v_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (2 + (step & 1) * MB + mb) * N, done = empty(slot),
+                         p = p_lo + (step & 1) * (Sh::kPBytes >> 4), pbar = pv_done + 8 * (step & 1);
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            mma_ss(d, a + (k * 2048 >> 4), kHi, p + (k * 512 >> 4), kPHi, pv, acc || k > 0);
+          tc_commit(done);
+          if (mb == MB - 1) tc_commit(pbar);
         }
-        tc_commit(pv_done);
       };
       uint32_t step = 0, items = 0;
-      while (ok && walk.next(c)) {
-        const int n = walk.it.tb - walk.it.ta;
-        if (!wait(q_full, items)) break;
-        ++items;
+      Job job;
+      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, items, dead, &job)) && job.ta < job.tb) {
+        const int n = job.tb - job.ta;
+        if (!wait(q_full, items - 1)) break;
         tc_fence_after();
-        scores(step);
-        for (int t = 0; ok && t < n; ++t, ++step) {
-          if (!SHARED && t + 1 < n) scores(step + 1);  // under the softmax of this tile
-          if (!wait(p_full, step)) break;
-          tc_fence_after();
-          values(step, t > 0);
-          if (SHARED && t + 1 < n && ok) scores(step + 1);
+        for (int t = 0; ok && t <= n; ++t) {  // a tile's scores run under the softmax of the one before
+          if (t < n) scores(step + t);
+          if (t > 0) {
+            const uint32_t s = step + t - 1;
+            if (!wait(p_full + 8 * (s & 1), s >> 1)) break;
+            tc_fence_after();
+            values(s, t > 2);
+          }
         }
+        step += n;
       }
       if (*dead) {  // no product may be in flight when TMEM is freed
         int none = 0;
@@ -242,177 +288,213 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     }
     __syncwarp();
   } else {
-    // ---- softmax: a thread per key -------------------------------------------------------------------
-    const uint32_t lanes = (uint32_t)warp << 21;
+    // ---- softmax: a thread per key, the CTA's tiles by turns to two groups of four warps -------------
+    const int wg = warp >> 2, wt = tid & 127, ww = warp & 3;
+    const uint32_t lanes = (uint32_t)ww << 21;
+    const uint32_t ts = tmem + lanes + wg * N, to = tmem + lanes + (2 + wg * MB) * N;  // this group's S^T and O^T
+    const int key = kTileKeys == 128 ? wt : ww * 16 + (lane & 15);  // the thread's key of a tile
+    const bool holds = kTileKeys == 128 || lane < 16;
+    const uint32_t pdst = pbuf + wg * Sh::kPBytes + key * 32;
     const int chunks = c.head_dim / 8;
-    uint32_t step = 0, meets = 0;
-    // The four warps meet.  Not a bar.sync, which no bound could end if a warp had left after a timeout.
+    uint32_t step = 0, mine = 0, meets = 0, nitem = 0;  // tiles of the CTA, of this group, meetings, items
+    // The group's four warps meet.  Not a bar.sync, which no bound could end if a warp had left after a timeout.
     auto meet_warps = [&] {
       __syncwarp();
-      if (lane == 0) mbar_arrive(meet);
-      return warp_wait(meet, meets++ & 1, dead);
+      if (lane == 0) mbar_arrive(meet + 8 * wg);
+      return warp_wait(meet + 8 * wg, meets++ & 1, dead);
     };
-    auto load_q = [&](const Item<N>& it) {
-      for (int i = tid; i < it.rows * KG * 8; i += 128) {
-        const int r = i / (KG * 8), x = i - r * (KG * 8);
-        const int tok = (it.row + r) / c.group, gh = (it.row + r) - tok * c.group;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (x < chunks)
-          v = __ldg(reinterpret_cast<const uint4*>(c.q + (it.s.row0 + tok) * c.q_token_stride + (int64_t)(it.h * c.group + gh) * c.q_head_stride) + x);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qbuf + (x >> 3) * N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4)), "r"(v.x),
-                     "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    // The next item: its rows' places and limits (tables of kTurns items, by turns: a warp may be two items ahead of
+    // another), and Q into shared memory.
+    Job job;
+    uint32_t jobs = 0;
+    auto open = [&] {
+      if (!take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) return false;
+      if (job.ta == job.tb) return true;
+      if (wt < job.rows) {
+        const int tok = (job.row + wt) / c.group, gh = job.row + wt - tok * c.group;
+        if (wg == 0) s_row[jobs % kTurns][wt] = (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + gh;
+        s_lim[wg][jobs % kTurns][wt] = visible_keys(c, Seq{job.kv_len, job.q_len, job.row0}, tok);
+      }
+      constexpr int kAhead = KG > 2 ? 4 : 1;  // chunks of 16 bytes in flight per thread
+#pragma unroll 1
+      for (int i0 = tid; i0 < job.rows * KG * 8; i0 += 256 * kAhead) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = i0 + u * 256, r = i / (KG * 8), x = i - r * (KG * 8);
+          v[u] = make_uint4(0, 0, 0, 0);
+          if (r < job.rows && x < chunks) {
+            const int tok = (job.row + r) / c.group, gh = (job.row + r) - tok * c.group;
+            v[u] = __ldg(reinterpret_cast<const uint4*>(c.q + (job.row0 + tok) * c.q_token_stride + (int64_t)(job.head * c.group + gh) * c.q_head_stride) + x);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = i0 + u * 256, r = i / (KG * 8), x = i - r * (KG * 8);
+          if (r < job.rows)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qbuf + (x >> 3) * N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4)), "r"(v[u].x),
+                         "r"(v[u].y), "r"(v[u].z), "r"(v[u].w) : "memory");
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(q_full);
+      return true;
     };
-    bool have = walk.next(c), ok = true;
-    if (have) load_q(walk.it);
-    while (ok && have) {
-      const Item<N> it = walk.it;
+    bool ok = open();
+    while (ok && job.ta < job.tb) {
+      const Job it = job;
+      const uint32_t turn = jobs % kTurns;
       const int rows = it.rows;
-      float m[N], l[N];
+      bool fresh = true;  // no tile of this item yet
+      float top = -INFINITY;  // the maximum in use of row `lane`
+      float l[N];             // this thread's share of each row's sum
 #pragma unroll
-      for (int n = 0; n < N; ++n) m[n] = -INFINITY, l[n] = 0.f;
-      const int vis0 = visible_keys(c, it.s, it.row / c.group);  // what every row sees
-      for (int t = it.ta; t < it.tb; ++t, ++step) {
-        const int j0 = t * kKeys, j = j0 + tid;
-        const bool there = j < it.s.kv_len && pool_row(c, it.b, j) >= 0;
-        if (!(ok = warp_wait(s_full + 8 * (step & 1), (step >> 1) & 1, dead))) break;
+      for (int n = 0; n < N; ++n) l[n] = 0.f;
+      const uint32_t last = step + it.tb - it.ta - 1;
+      for (int t = it.ta + ((int)(step & 1) ^ wg); t < it.tb; t += 2, ++mine) {
+        const int j0 = t * kTileKeys, j = j0 + key;
+        const bool there = holds && j < it.kv_len && pool_row(c, it.b, j) >= 0;
+        if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
         tc_fence_after();
         uint32_t x[N];
-        tmem_ld_cols<N>(tmem + lanes + (step & 1) * N, x);
-        if (j0 + kKeys > vis0 || !__all_sync(0xffffffffu, there)) {
+        tmem_ld_cols<N>(ts, x);
+        if (fresh && !(ok = meet_warps())) break;  // the item's tables are written
+        // the first row sees the least
+        if (j0 + kTileKeys > s_lim[wg][turn][0] || !__all_sync(0xffffffffu, there)) {
 #pragma unroll
           for (int n = 0; n < N; ++n)
-            if (n < rows && !(there && j < visible_keys(c, it.s, (it.row + n) / c.group))) x[n] = 0xff800000u;
+            if (n < rows && !(there && j < s_lim[wg][turn][n])) x[n] = 0xff800000u;
         }
-        float* const mine = reinterpret_cast<float*>(s_max[step & 1]) + warp;
+        float4* const peak = s_max[wg][mine & 1];
 #pragma unroll
         for (int n = 0; n < N; n += 4)
           if (n < rows) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float w = warp_max(__uint_as_float(x[n + e]));
-              if (lane == n + e) mine[4 * (n + e)] = w;
+              if (lane == n + e) reinterpret_cast<float*>(peak)[4 * (n + e) + ww] = w;
             }
           }
         if (!(ok = meet_warps())) break;
-        float f[N];
-        bool grow = false;
+        const float4 w = peak[lane & (N - 1)];
+        const float mx = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * c.scale_log2;
+        const bool grows = lane < rows && (mx > top + 8.f || (top == -INFINITY && mx > -INFINITY));
+        const float f = grows ? fast_exp2(top - mx) : 1.f;  // 0 for the first maximum
+        if (grows) top = mx;
+        const float zero = top == -INFINITY ? 0.f : top;
+        const bool grow = __any_sync(0xffffffffu, grows);
+        // the group's product before has read P and written O; at an item's start, O has been read as well
+        if (mine > 0 && !(ok = warp_wait(pv_done + 8 * wg, (mine - 1) & 1, dead))) break;
+        if (wg == 1 && fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+        if (!fresh && grow) {  // the same in every thread of the group
+          tc_fence_after();
+#pragma unroll
+          for (int n = 0; n < N; ++n) l[n] *= __shfl_sync(0xffffffffu, f, n);
+#pragma unroll 1
+          for (int mb = 0; mb < MB; ++mb) {
+            uint32_t o[N];
+            tmem_ld_cols<N>(to + mb * N, o);
+#pragma unroll
+            for (int n = 0; n < N; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * __shfl_sync(0xffffffffu, f, n));
+            tmem_st_cols<N>(to + mb * N, o);
+          }
+          tc_wait_st();
+        }
+        fresh = false;
 #pragma unroll
         for (int n = 0; n < N; n += 4)
           if (n < rows) {
+            float p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float4 w = s_max[step & 1][n + e];
-              const float mx = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * c.scale_log2;
-              f[n + e] = 1.f;
-              if (mx > m[n + e] + 8.f || (m[n + e] == -INFINITY && mx > -INFINITY)) {
-                f[n + e] = fast_exp2(m[n + e] - mx);  // 0 for the first maximum
-                m[n + e] = mx;
-                l[n + e] *= f[n + e];
-                grow = grow || n + e < rows;
-              }
-            }
-          }
-        if (t > it.ta) {  // the product before has read P and written O
-          if (!(ok = warp_wait(pv_done, (step - 1) & 1, dead))) break;
-          if (grow) {  // the same in every thread
-            tc_fence_after();
-#pragma unroll 1
-            for (int mb = 0; mb < MB; ++mb) {
-              uint32_t o[N];
-              tmem_ld_cols<N>(tmem + lanes + (2 + mb) * N, o);
-#pragma unroll
-              for (int n = 0; n < N; n += 4)
-                if (n < rows) {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) o[n + e] = __float_as_uint(__uint_as_float(o[n + e]) * f[n + e]);
-                }
-              tmem_st_cols<N>(tmem + lanes + (2 + mb) * N, o);
-            }
-            tc_wait_st();
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < N; n += 8)
-          if (n < rows) {
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float z = m[n + e] == -INFINITY ? 0.f : m[n + e];
-              p[e] = n + e < rows ? fast_exp2(fmaf(__uint_as_float(x[n + e]), c.scale_log2, -z)) : 0.f;
+              p[e] = fast_exp2(fmaf(__uint_as_float(x[n + e]), c.scale_log2, -__shfl_sync(0xffffffffu, zero, n + e)));
               l[n + e] += p[e];
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(pbuf + (n >> 4) * (kKeys * 32) + tid * 32 +
-                                                                        ((((n >> 3) & 1) ^ ((tid >> 2) & 1)) << 4)),
-                         "r"(pack2<BF16>(p[0], p[1])), "r"(pack2<BF16>(p[2], p[3])), "r"(pack2<BF16>(p[4], p[5])), "r"(pack2<BF16>(p[6], p[7]))
-                         : "memory");
+            if (holds)
+              asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(pdst + (n >> 4) * Sh::kPBlock + ((((n >> 3) & 1) ^ ((key >> 2) & 1)) << 4) + (n & 4) * 2),
+                           "r"(pack2<BF16>(p[0], p[1])), "r"(pack2<BF16>(p[2], p[3])) : "memory");
           }
         // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V
-        if (j0 + kKeys > it.s.kv_len && it.s.kv_len % c.page_tokens != 0) {
+        if (j0 + kTileKeys > it.kv_len && it.kv_len % c.page_tokens != 0) {
           for (int s = SHARED ? 1 : kKS; s < kTS; ++s) {
-            const uint32_t pos = step * kTS + s, slot = pos % kSlots;
+            const uint32_t pos = (step + t - it.ta) * kTS + s, slot = pos % kSlots;
             if (!(ok = warp_wait(full(slot), (pos / kSlots) & 1, dead))) break;
-            if (j >= it.s.kv_len)
-              for (int i = 0; i < Sh::kGroups * 8; ++i)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + slot * Sh::kSlotBytes + (i >> 3) * kGroupBytes + tid * 128 + (i & 7) * 16),
+            if (j >= it.kv_len && holds)
+              for (int i = 0; i < kKGroups * 8; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + slot * Sh::kSlotBytes + (i >> 3) * kGroupBytes + key * 128 + (i & 7) * 16),
                              "r"(0) : "memory");
           }
           if (!ok) break;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_fence_before();
-        mbar_arrive(p_full);
+        mbar_arrive(p_full + 8 * wg);
       }
       if (!ok) break;
-      have = walk.next(c);
-      if (have) load_q(walk.it);  // the item's last QK^T has been seen
+      // the item's last QK^T is done: the next one's Q may come
+      if (!(ok = warp_wait(s_full + 8 * (last & 1), (last >> 1) & 1, dead)) || !(ok = open())) break;
 
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (n < rows) {
-          float w = l[n];
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
-          if (lane == 0) reinterpret_cast<float*>(s_sum)[4 * n + warp] = w;
-        }
-      if (!(ok = meet_warps())) break;
-      if (!(ok = warp_wait(pv_done, (step - 1) & 1, dead))) break;
-      tc_fence_after();
-      const bool whole = it.ta == 0 && it.tb == it.nt;
-      float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
-      const int tok0 = it.row / c.group, gh0 = it.row - tok0 * c.group;
-#pragma unroll 1
-      for (int mb = 0; mb < MB; ++mb) {
-        uint32_t o[N];
-        tmem_ld_cols<N>(tmem + lanes + (2 + mb) * N, o);
-        const int col = mb * 128 + tid;
-        int tok = tok0, gh = gh0;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (n < rows) {
-            const float4 w = s_sum[n];
-            const float sum = (w.x + w.y) + (w.z + w.w);
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-            const int64_t r = (it.s.row0 + tok) * (int64_t)(c.kv_heads * c.group) + it.h * c.group + gh;
-            const float v = __uint_as_float(o[n]);
-            if (col < c.v_dim) {
-              if (whole) P.a.out[r * c.v_dim + col] = (uint16_t)(pack2<BF16>(v * inv, 0.f) & 0xffff);
-              else part[n * c.v_dim + col] = v;
-            }
-            if (mb == 0 && tid == n) {
-              if (!whole) {
-                part[P.a.part_rows * c.v_dim + n] = m[n];
-                part[P.a.part_rows * (c.v_dim + 1) + n] = sum;
-              } else if (P.a.lse) {
-                P.a.lse[r] = sum == 0.f ? -INFINITY : fmaf(m[n], 0.693147180559945f, logf(sum));
-              }
-            }
-            if (++gh == c.group) gh = 0, ++tok;
-          }
+      // the groups' maxima and sums meet in shared memory; the first group joins them and writes the item
+      if (wg == 1 && fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+      {
+        // N values over 32 lanes: each step halves the values a lane holds and the lanes that share one
+        const float sum = lane_sums<N>(l, lane);
+        if (lane < N) reinterpret_cast<float*>(s_sum[wg])[4 * lane + ww] = sum;
+        if (wt < N) s_top[wg][lane] = top;
       }
-      tc_fence_before();
+      if (wg == 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(summed);
+      } else {
+        if (!(ok = meet_warps()) || !(ok = warp_wait(summed, nitem & 1, dead))) break;
+        float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
+        if (wt < rows) {
+          const float4 u = s_sum[0][wt], v = s_sum[1][wt];
+          const float m0 = s_top[0][wt], m1 = s_top[1][wt];
+          const float mm = fmaxf(m0, m1), z = mm == -INFINITY ? 0.f : mm;
+          const float f0 = fast_exp2(m0 - z), f1 = fast_exp2(m1 - z);
+          const float sum = ((u.x + u.y) + (u.z + u.w)) * f0 + ((v.x + v.y) + (v.z + v.w)) * f1;
+          const float inv = it.whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+          s_mix[wt] = make_float2(f0 * inv, f1 * inv);
+          if (!it.whole) {
+            part[P.a.part_rows * c.v_dim + wt] = mm;
+            part[P.a.part_rows * (c.v_dim + 1) + wt] = sum;
+          } else if (P.a.lse) {
+            P.a.lse[s_row[turn][wt]] = sum == 0.f ? -INFINITY : fmaf(mm, 0.693147180559945f, logf(sum));
+          }
+        }
+        if (!(ok = meet_warps())) break;
+        if (!(ok = warp_wait(pv_done + 8 * (last & 1), (last >> 1) & 1, dead))) break;
+        if (last != step && !(ok = warp_wait(pv_done + 8 * (~last & 1), ((last - 1) >> 1) & 1, dead))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int mb = 0; mb < MB; ++mb) {
+          uint32_t o[N], o1[N];
+          tmem_ld_cols<N>(tmem + lanes + (2 + mb) * N, o);
+          tmem_ld_cols<N>(tmem + lanes + (2 + MB + mb) * N, o1);
+          const int col = mb * 128 + wt;
+          if (col < c.v_dim) {
+#pragma unroll
+            for (int n = 0; n < N; n += 4)
+              if (n < rows) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 w = s_mix[n + e];  // a group without tiles has weight 0 and an O that holds anything
+                  const float v = (w.x != 0.f ? __uint_as_float(o[n + e]) * w.x : 0.f) + (w.y != 0.f ? __uint_as_float(o1[n + e]) * w.y : 0.f);
+                  if (n + e < rows) {
+                    if (it.whole) P.a.out[s_row[turn][n + e] * c.v_dim + col] = (uint16_t)(pack2<BF16>(v, 0.f) & 0xffff);
+                    else part[(n + e) * c.v_dim + col] = v;
+                  }
+                }
+              }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(read);
+      }
+      step = last + 1;
+      ++nitem;
     }
   }
   __syncthreads();
@@ -444,7 +526,7 @@ void launch_any(const DecodeParams& P, const CUtensorMap& k, const CUtensorMap& 
 }  // namespace
 
 // Single-buffer pools need V to begin at the second column group.
-bool attend_decode_fits(const CacheParams& c) { return (c.v ? c.head_dim <= 256 : c.v_col == 64) && pages_fit(c); }
+bool attend_decode_fits(const CacheParams& c) { return (c.v ? c.head_dim <= 256 : c.v_col == 64) && pages_fit(c, c.v ? kKeys : 64); }
 
 // Single-buffer pools often have more than 16 heads per KV head: 32 rows an item then, so that K and V are read
 // half as often.
@@ -456,7 +538,7 @@ AttendShape attend_decode_shape(const CacheParams& c, int sms, int64_t rows) {
 bool launch_attend_decode(const AttendParams& A, bool bf16, cudaStream_t s) {
   DecodeParams P;
   P.a = A;
-  P.box = pool_boxes(A.c);
+  P.box = pool_boxes(A.c, A.c.v ? kKeys : 64);
   CUtensorMap k, v;
   if (!pool_map(&k, A.c.k, A.c, bf16, P.box)) return false;
   v = k;

@@ -22,7 +22,7 @@
 // Work.  As in ztcp_attend.cu the items form one line that the CTAs (one per SM) share evenly, in units of
 // keys x group (Line); attend_merge_kernel joins items that several CTAs share.
 //
-// Waits are bounded: a wait that does not end within about two seconds sets the CTA's error word, every role leaves
+// Waits are bounded: a wait that runs out (ztcp_tc.cuh) sets the CTA's error word, every role leaves
 // its loop, copies and products in flight are waited for (bounded again), TMEM is freed, and the merge kernel
 // reports ZTCP_SEQ_TIMEOUT for every sequence.
 #include "ztcp_tc.cuh"
@@ -59,7 +59,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-constexpr int kBars = 32;  // barrier slots at the start of shared memory
+constexpr int kBars = 40;  // barrier slots at the start of shared memory
 
 template <bool BF16, int HALVES, int SLOTS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -70,6 +70,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   extern __shared__ uint8_t smem_raw[];
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
+  __shared__ Job s_jobs[kJobs];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   volatile int* const dead = &dead_s;
@@ -81,13 +82,13 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   const uint32_t qtile = tiles, ring = tiles + 2 * kTile;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + (SLOTS + s) * 8; };
-  const uint32_t q_full = bars + 2 * SLOTS * 8, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16, drain = o_full + 16;
-  static_assert(2 * SLOTS + 9 <= kBars, "barrier slots");
+  const uint32_t q_full = bars + 2 * SLOTS * 8, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
+                 job_full = o_full + 16, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
+  static_assert(2 * SLOTS + 9 + 2 * kJobs <= kBars, "barrier slots");
 
   int64_t at;
   Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<kItemRows>(c, b); },
-                             [&](const SplitSpan& s) { return blockIdx.x < s.n ? s.begin(blockIdx.x) : (int64_t)-1; }, &at, &spot);
+  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<kItemRows>(c, b); }, &at, &spot);
   if (at < 0) {
     if (tid == 0) P.a.cuts[blockIdx.x] = Cut{};
     return;
@@ -104,6 +105,10 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       mbar_init(p_full + 8 * q, 128);
       mbar_init(o_full + 8 * q, 1);
     }
+    for (int e = 0; e < kJobs; ++e) {
+      mbar_init(job_full + 8 * e, 1);
+      mbar_init(job_empty + 8 * e, 9);
+    }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -115,22 +120,24 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-
-  Walk<kItemRows> walk;
-  walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+  cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up meanwhile; it waits for this one's end
 
   if (warp == kTmaWarp) {
     // ---- TMA: K and V tiles in turn through the ring; lane p fetches page p of the tile ------------
     const int per_tile = kKeys / P.box.rows;
     uint32_t pos = 0;  // tiles so far: K of step t is 2 t, V is 2 t + 1
-    bool ok = true;
-    while (ok && walk.next(c)) {
-      const Item<kItemRows>& it = walk.it;
-      for (int t = it.ta; ok && t < it.tb; ++t) {
+    Publisher<kItemRows, kKeys> pub;
+    pub.walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+    pub.cut = Cut{};
+    pub.n = 0;
+    Job job, then;
+    bool ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job);
+    while (ok && job.ta < job.tb) {
+      for (int t = job.ta; ok && t < job.tb; ++t) {
         const int j = t * kKeys + lane * P.box.rows;
         int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
-        if (lane < per_tile && j < it.s.kv_len) {
-          const int64_t r = pool_row(c, it.b, j);
+        if (lane < per_tile && j < job.kv_len) {
+          const int64_t r = pool_row(c, job.b, j);
           if (r >= 0) row = (int32_t)r;
         }
 #pragma unroll
@@ -146,92 +153,98 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           if (lane < per_tile)
 #pragma unroll
             for (int x = 0; x < HALVES; ++x)
-              tma_load(ring + slot * kTile + x * kHalf + lane * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, it.h, row, full(slot));
+              tma_load(ring + slot * kTile + x * kHalf + lane * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, job.head, row, full(slot));
         }
+        // the item behind this one, looked up once this one's first loads are out
+        if (ok && t == job.ta) ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &then);
       }
+      job = then;
     }
-    if (lane == 0) write_cut<kItemRows>(P.a, S, c, spot, at, 0);
+    if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
     if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
       int none = 0;
       for (uint32_t p = pos > SLOTS ? pos - SLOTS : 0; p < pos; ++p) mbar_wait(full(p % SLOTS), (p / SLOTS) & 1, &none);
     }
   } else if (warp == kMmaWarp) {
-    // ---- products ----------------------------------------------------------------------------------
-    if (lane == 0) {
-      const uint32_t qk = inst_desc(BF16, kKeys, false, false), pv = inst_desc(BF16, kCols, false, true);
-      const int ksteps = (c.head_dim + 15) / 16;
-      uint32_t step = 0;                      // tiles so far
-      uint32_t items0 = 0, items1 = 0;        // items so far, per row tile
-      uint32_t softs0 = 0, softs1 = 0;        // tiles so far, per row tile
-      bool ok = true, have = walk.next(c);
-      int nq = 0;
-      auto scores = [&](int q, uint32_t st) {  // S_q = Q_q K^T of step st
-        const uint32_t kb = ring + (2 * st % SLOTS) * kTile, qb = qtile + q * kTile;
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-          mma_ss(tmem + q * 128, smem_desc(qb + off, 16, 1024), smem_desc(kb + off, 16, 1024), qk, k > 0);
-        }
-        tc_commit(s_full + 8 * q);
-      };
-      auto wait = [&](uint32_t bar, uint32_t n) {  // the n-th completion (from 0)
-        ok = ok && mbar_wait(bar, n & 1, dead);
+    // ---- products: one thread ------------------------------------------------------------------------
+    if (elect_one()) {
+      constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
+      const uint32_t qk = inst_desc(BF16, 128, kKeys, false, false), pv = inst_desc(BF16, 128, kCols, false, true);
+      const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kHalf), q_lo = desc_lo(qtile, 16);
+      uint32_t kslot = 0, kphase = 0;    // of the next K tile; V's follows it
+      uint32_t vslot = 1, vphase = 0;
+      uint32_t items[2] = {0, 0};        // items so far, per row tile
+      uint32_t softs[2] = {0, 0};        // tiles so far, per row tile
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = ok && mbar_wait(bar, parity & 1, dead);
         return ok;
       };
-      if (have) {  // the first step's scores
-        nq = walk.it.rows > kRowTile ? 2 : 1;
-        if (wait(full(0), 0)) {
-          for (int q = 0; q < nq; ++q)
-            if (wait(q_full + 8 * q, 0)) {
-              tc_fence_after();
-              scores(q, 0);
-            }
-          tc_commit(empty(0));
+      auto advance = [&](uint32_t& slot, uint32_t& phase) {  // two slots on
+        slot += 2;
+        if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+      };
+      const uint32_t tm = tmem;
+      // Step t multiplies P of tile t - 1 by V and computes the scores of tile t; per row tile in turn, so that each
+      // has the other's products to hide its softmax under.
+      Job job, then;
+      uint32_t njobs = 0;
+      int cur = 0, n = 0;  // row tiles of the step before, and tiles of its item
+      int t = 0;           // of the item's tiles, those whose scores are out
+      ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &then);
+      while (ok) {
+        const bool fresh = t == n;  // the step's scores are those of the next item
+        if (fresh) {
+          job = then;
+          if (cur == 0 && job.ta == job.tb) break;
         }
-      }
-      while (ok && have) {
-        const int n = walk.it.tb - walk.it.ta;
-        const int cur = nq;
-        bool more = false;
-        for (int t = 0; ok && t < n; ++t, ++step) {
-          const bool last = t + 1 == n;
-          if (last) {
-            more = walk.next(c);
-            nq = more ? (walk.it.rows > kRowTile ? 2 : 1) : 0;
+        const int nxt = fresh ? (job.ta < job.tb ? (job.rows > kRowTile ? 2 : 1) : 0) : cur;
+        if (cur && !wait(full(vslot), vphase)) break;
+        bool k_there = false;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (q < cur) {
+            if (!wait(p_full + 8 * q, softs[q])) break;
+            ++softs[q];
+            tc_fence_after();
+            const uint32_t b = v_lo + vslot * (kTile >> 4);
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_ts(tm + 256 + q * 128, tm + q * 128 + k * 8, b + (k * 2048 >> 4), kHi, pv, t > 1 || k > 0);
+            if (fresh) tc_commit(o_full + 8 * q);
+            if (fresh) ++items[q];
           }
-          const bool nxt = !last || more;
-          const uint32_t vp = 2 * step + 1, kp = vp + 1;
-          if (!wait(full(vp % SLOTS), vp / SLOTS)) break;
-          bool k_there = false;
-          for (int q = 0; ok && q < 2; ++q) {
-            if (q < cur) {
-              if (!wait(p_full + 8 * q, q ? softs1 : softs0)) break;
-              if (q) ++softs1;
-              else ++softs0;
-              tc_fence_after();
-              const uint32_t vb = ring + (vp % SLOTS) * kTile;
-              for (int k = 0; k < kKeys / 16; ++k)
-                mma_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, smem_desc(vb + k * 2048, kHalf, 1024), pv, t > 0 || k > 0);
-              if (last) {
-                tc_commit(o_full + 8 * q);
-                if (q) ++items1;
-                else ++items0;
-              }
+          if (q < nxt) {
+            if (!k_there && !wait(full(kslot), kphase)) break;
+            k_there = true;
+            if (fresh && !wait(q_full + 8 * q, items[q])) break;
+            tc_fence_after();
+            const uint32_t a = q_lo + q * (kTile >> 4), b = k_lo + kslot * (kTile >> 4);
+#pragma unroll
+            for (int k = 0; k < HALVES * 4; ++k) {
+              const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+              mma_ss(tm + q * 128, a + off, kHi, b + off, kHi, qk, k > 0);
             }
-            if (nxt && q < nq) {
-              if (!k_there) {
-                if (!wait(full(kp % SLOTS), kp / SLOTS)) break;
-                k_there = true;
-              }
-              if (last && !wait(q_full + 8 * q, q ? items1 : items0)) break;
-              tc_fence_after();
-              scores(q, step + 1);
-            }
+            tc_commit(s_full + 8 * q);
           }
-          if (!ok) break;
-          tc_commit(empty(vp % SLOTS));
-          if (nxt) tc_commit(empty(kp % SLOTS));
         }
-        have = more;
+        if (!ok) break;
+        if (cur) {
+          tc_commit(empty(vslot));
+          advance(vslot, vphase);
+        }
+        if (nxt) {
+          tc_commit(empty(kslot));
+          advance(kslot, kphase);
+        }
+        if (fresh) {
+          if (nxt == 0) break;
+          n = job.tb - job.ta;
+          t = 0;
+          ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &then);
+        }
+        cur = nxt;
+        ++t;
       }
       if (*dead) {  // no product may be in flight when TMEM is freed
         int none = 0;
@@ -248,33 +261,37 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     const uint32_t qdst = qtile + q * kTile + wg * 128;
     const int chunks = c.head_dim / 8;
     uint32_t step = 0, mine = 0, done = 0;  // tiles of the CTA, tiles and items of this row tile
-    // Item's row of this thread -> shared memory (rows past the item's end: the last one, results unused)
-    auto load_q = [&](const Item<kItemRows>& it) {
-      const int r = it.row + min(q * kRowTile + wg, it.rows - 1);
+    // The next item, and this thread's row of it into shared memory (rows past the item's end: the last one, whose
+    // results are not used)
+    Job job;
+    uint32_t njobs = 0;
+    auto open = [&] {
+      if (!take_job(s_jobs, job_full, job_empty, njobs, lane, dead, &job)) return false;
+      if (job.ta == job.tb || (q == 1 && job.rows <= kRowTile)) return true;
+      const int r = job.row + min(q * kRowTile + wg, job.rows - 1);
       const int tok = r / c.group, gh = r - tok * c.group;
-      const uint16_t* const src = c.q + (it.s.row0 + tok) * c.q_token_stride + (int64_t)(it.h * c.group + gh) * c.q_head_stride;
-      for (int x = 0; x < kCols / 8; ++x) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (x < chunks) v = __ldg(reinterpret_cast<const uint4*>(src) + x);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qdst + (x >> 3) * kHalf + (((x & 7) ^ (wg & 7)) << 4)), "r"(v.x), "r"(v.y),
-                     "r"(v.z), "r"(v.w) : "memory");
-      }
+      const uint16_t* const src = c.q + (job.row0 + tok) * c.q_token_stride + (int64_t)(job.head * c.group + gh) * c.q_head_stride;
+      uint4 v[kCols / 8];
+#pragma unroll
+      for (int x = 0; x < kCols / 8; ++x) v[x] = x < chunks ? __ldg(reinterpret_cast<const uint4*>(src) + x) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < kCols / 8; ++x)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qdst + (x >> 3) * kHalf + (((x & 7) ^ (wg & 7)) << 4)), "r"(v[x].x), "r"(v[x].y),
+                     "r"(v[x].z), "r"(v[x].w) : "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(q_full + 8 * q);
+      return true;
     };
-    bool have = walk.next(c), ok = true;
-    if (have && (q == 0 || walk.it.rows > kRowTile)) load_q(walk.it);
-    while (ok && have) {
-      const Item<kItemRows> it = walk.it;
-      const int n = it.tb - it.ta;
+    bool ok = open();
+    while (ok && job.ta < job.tb) {
+      const Job it = job;
       if (q == 1 && it.rows <= kRowTile) {  // nothing in this row tile
-        step += n;
-        have = walk.next(c);
-        if (have && walk.it.rows > kRowTile) load_q(walk.it);
+        step += it.tb - it.ta;
+        ok = open();
         continue;
       }
       const int r = q * kRowTile + wg;
-      const int lim = r < it.rows ? visible_keys(c, it.s, (it.row + r) / c.group) : 0;
+      const int lim = r < it.rows ? visible_keys(c, Seq{it.kv_len, it.q_len, it.row0}, (it.row + r) / c.group) : 0;
       float m = -INFINITY, l = 0.f;
       for (int t = it.ta; t < it.tb; ++t, ++step, ++mine) {
         const int j0 = t * kKeys;
@@ -282,7 +299,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         unsigned bad = 0;
         {
           const int j = j0 + lane * P.box.rows;
-          const bool b = lane < kKeys / P.box.rows && j < it.s.kv_len && pool_row(c, it.b, j) < 0;
+          const bool b = lane < kKeys / P.box.rows && j < it.kv_len && pool_row(c, it.b, j) < 0;
           bad = __ballot_sync(0xffffffffu, b);
         }
         if (!(ok = warp_wait(s_full + 8 * q, mine & 1, dead))) break;
@@ -343,8 +360,8 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         unpair(sum1, s2, s3);
         l += (s0 + s1) + (s2 + s3);
         // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V
-        const int end = it.s.kv_len - j0;
-        if (q == 0 && end < kKeys && it.s.kv_len % c.page_tokens != 0) {
+        const int end = it.kv_len - j0;
+        if (q == 0 && end < kKeys && it.kv_len % c.page_tokens != 0) {
           const uint32_t vp = 2 * step + 1;
           if (!(ok = warp_wait(full(vp % SLOTS), (vp / SLOTS) & 1, dead))) break;
           if (wg >= end)
@@ -359,15 +376,14 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         mbar_arrive(p_full + 8 * q);
       }
       if (!ok) break;
-      have = walk.next(c);
-      if (have && (q == 0 || walk.it.rows > kRowTile)) load_q(walk.it);  // the item's last QK^T has been seen
+      if (!(ok = open())) break;  // the item's last QK^T has been seen: the next one's Q may come
 
       if (!(ok = warp_wait(o_full + 8 * q, done & 1, dead))) break;
       ++done;
       tc_fence_after();
-      const bool whole = it.ta == 0 && it.tb == it.nt;
+      const bool whole = it.whole;
       const int tok = (it.row + r) / c.group, gh = (it.row + r) - tok * c.group;
-      const int64_t o = (it.s.row0 + tok) * (int64_t)(c.kv_heads * c.group) + it.h * c.group + gh;
+      const int64_t o = (it.row0 + tok) * (int64_t)(c.kv_heads * c.group) + it.head * c.group + gh;
       float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll 1
@@ -424,14 +440,14 @@ void launch_kernel(const TcParams& P, const CUtensorMap& k, const CUtensorMap& v
 
 }  // namespace
 
-bool attend_tc_fits(const CacheParams& c) { return c.v && c.head_dim <= 128 && pages_fit(c); }
+bool attend_tc_fits(const CacheParams& c) { return c.v && c.head_dim <= 128 && pages_fit(c, kKeys); }
 
 AttendShape attend_tc_shape(const CacheParams& c, int sms) { return {sms, kItemRows, kItemRows * (c.v_dim + 2)}; }
 
 bool launch_attend_tc(const AttendParams& A, bool bf16, cudaStream_t s) {
   TcParams P;
   P.a = A;
-  P.box = pool_boxes(A.c);
+  P.box = pool_boxes(A.c, kKeys);
   CUtensorMap k, v;
   if (!pool_map(&k, A.c.k, A.c, bf16, P.box) || !pool_map(&v, A.c.v, A.c, bf16, P.box)) return false;
   if (A.c.head_dim <= 64) bf16 ? launch_kernel<true, 1, 8>(P, k, v, s) : launch_kernel<false, 1, 8>(P, k, v, s);

@@ -185,13 +185,20 @@ __device__ __forceinline__ int64_t pool_row(const CacheParams& c, int b, int j) 
   return (e < 0 || e >= c.pool_pages) ? -1 : (int64_t)e * c.page_tokens + (j - p * c.page_tokens);
 }
 
+// a / b for non-negative a; most values fit 32 bits, whose division is several times shorter.
+__device__ __forceinline__ int64_t div_pos(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+  return a / b;
+}
+
 // Work laid out on one line -- sequence by sequence, `count(b)` units each -- that a grid's CTAs share evenly.
 struct SplitSpan {
   int64_t total;  // units in all
-  int32_t n;      // CTAs that take part: min(grid, total), so that each has at least one unit
-  __device__ __forceinline__ int64_t begin(int cta) const { return total * cta / n; }
+  int64_t share;  // units of a CTA (the last ones may have fewer or none)
+  __device__ __forceinline__ int64_t begin(int cta) const { return total < share * cta ? total : share * cta; }
+  __device__ __forceinline__ int64_t own_begin() const { return begin(blockIdx.x) < total ? begin(blockIdx.x) : (int64_t)-1; }
   // The CTA whose share holds unit w.
-  __device__ __forceinline__ int owner(int64_t w) const { return (int)(((w + 1) * n - 1) / total); }
+  __device__ __forceinline__ int owner(int64_t w) const { return (int)div_pos(w, share); }
 };
 
 struct Spot {
@@ -199,10 +206,10 @@ struct Spot {
   int64_t first;  // the sequence's first unit on the line
 };
 
-// Sums every sequence's units (block-wide, up to 32 warps) and finds the sequence that holds unit `pick(span)`
-// (-1: none wanted).  All threads get the span, the wanted unit and its spot.
-template <class Count, class Pick>
-__device__ __forceinline__ SplitSpan locate(int n_seqs, int grid, Count count, Pick pick, int64_t* want, Spot* spot) {
+// Sums every sequence's units (block-wide, up to 32 warps) and finds the sequence that holds the first unit of this
+// CTA's share (-1: it has none).  All threads get the span, that unit and its spot.
+template <class Count>
+__device__ __forceinline__ SplitSpan locate(int n_seqs, int grid, Count count, int64_t* want, Spot* spot) {
   __shared__ int64_t sm[34];
   const int t = threadIdx.x, nt = blockDim.x;
   const int per = (n_seqs + nt - 1) / nt;
@@ -225,8 +232,9 @@ __device__ __forceinline__ SplitSpan locate(int n_seqs, int grid, Count count, P
   }
   SplitSpan S;
   S.total = total;
-  S.n = (int32_t)(total < grid ? total : grid);
-  const int64_t target = S.n > 0 ? pick(S) : -1;
+  S.share = div_pos(total + grid - 1, grid);
+  if (S.share == 0) S.share = 1;
+  const int64_t target = S.own_begin();
   int64_t at = base + inc - sum;
   if (target >= at && target < at + sum)
     for (int b = b0; b < b1; ++b) {

@@ -75,8 +75,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
   }
   int64_t at;
   Spot spot;
-  const SplitSpan S = locate(c.n_seqs, gridDim.x, [&](int b) { return (int64_t)seq_units(P, b); },
-                             [&](const SplitSpan& s) { return blockIdx.x < s.n ? s.begin(blockIdx.x) : (int64_t)-1; }, &at, &spot);
+  const SplitSpan S = locate(c.n_seqs, gridDim.x, [&](int b) { return (int64_t)seq_units(P, b); }, &at, &spot);
   if (at < 0) return;
   Cursor cons;
   cons.load(P, spot.seq);

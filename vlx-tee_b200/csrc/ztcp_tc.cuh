@@ -9,11 +9,11 @@ namespace ztcp {
 
 constexpr int kKeys = 128;                           // keys per tile
 constexpr int kGroupBytes = kKeys * 128;             // a tile's 64-column group: 128 rows of 128 bytes
-constexpr long long kWaitCycles = 4000000000ll;      // bound of a wait, about two seconds
+constexpr uint32_t kWaitTries = 2000000;             // bound of a wait: 0.05 to 2 seconds
 
 // Boxes of the pool's TMA loads.
 struct PoolBoxes {
-  int32_t rows;       // rows of one box: a page, or 128 of a larger one (8 to 128, a power of two)
+  int32_t rows;       // rows of one box: a page, or a tile's keys of a larger one (8 to 128, a power of two)
   int32_t shift;      // its logarithm
   int32_t pool_rows;  // rows of the tensor maps; a load at this row is filled with zeros
 };
@@ -30,25 +30,24 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+// Waits for the phase of this parity; false when the wait ran out (kWaitTries attempts, each of which the hardware may
+// suspend for about a microsecond), and the CTA's dead flag is set.  The loop is written out because its length is on
+// the product warp's critical path (measured: 7 cycles when the phase is there, against 65 for a loop in C).
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+      "{\n\t.reg .pred P, Q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n\tTRY%=:\n\tmbarrier.try_wait.parity.shared.b64 P, [%1], %2;\n\t@P bra DONE%=;\n\t"
+      "add.u32 n, n, 1;\n\tsetp.lt.u32 Q, n, %3;\n\t@Q bra TRY%=;\n\tDONE%=:\n\tselp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity), "n"(kWaitTries) : "memory");
+  if (!ok) *dead = 1;
   return ok;
 }
-// False when the wait ran out, here or (dead set) elsewhere in the CTA.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try(bar, parity)) return true;
-  const long long start = clock64();
-  while (!mbar_try(bar, parity)) {
-    if (*dead) return false;
-    if (clock64() - start > kWaitCycles) {
-      *dead = 1;
-      return false;
-    }
-  }
-  return true;
+// One lane of a converged warp, always the same.  The compiler keeps the operands of what it guards in uniform
+// registers, which tcgen05 instructions read (measured: 39 cycles per small product, against 44 to 53 under lane == 0).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p;
 }
 // The same for a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
@@ -65,13 +64,19 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-               "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+// Matrix descriptors as their two words: the low one holds the address (in 16 bytes) and lbo and takes offsets by
+// plain addition, the high one is a constant of the layout.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-               "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
   asm volatile(
@@ -101,20 +106,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 // Shared-memory matrix descriptor, 128-byte swizzle, descriptor version 1.  K-major operands (Q, K: 64 columns per
 // 128-byte row): 8-row groups 1,024 bytes apart.  MN-major operand (V: 64 output columns per row of a key): 8-key
 // groups 1,024 bytes apart, the next 64 columns `lbo` bytes on.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-// Instruction descriptor: fp32 accumulators, both operands of the pool's type, M = 128.
-__device__ __forceinline__ uint32_t inst_desc(bool bf16, int n, bool a_mn_major, bool b_mn_major) {
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr & 0x3ffff) >> 4) | (lbo >> 4) << 16; }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle) { return (sbo >> 4) | 1u << 14 | swizzle << 29; }
+constexpr uint32_t kSwizzle128 = 2, kSwizzle32 = 6;
+// Instruction descriptor: fp32 accumulators, both operands of the pool's type.
+__device__ __forceinline__ uint32_t inst_desc(bool bf16, int m, int n, bool a_mn_major, bool b_mn_major) {
   const uint32_t t = bf16 ? 1 : 0;
-  return 1u << 4 | t << 7 | t << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+  return 1u << 4 | t << 7 | t << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
 // ---- the line of items ----------------------------------------------------------------------------
 // Items of up to ROWS (token, head-of-the-group) rows of one sequence and KV head form one line, sequence by
 // sequence, row tile by row tile, head by head, that the CTAs share evenly, in units of keys x group: an item's
 // length is what its last row sees plus its own rows, which sums over row tiles in closed form.  Shares are rounded
-// to tiles of 128 keys.
+// to tiles of KEYS keys.
 template <int ROWS>
 struct Line {
   int64_t head;  // units of row tile 0's items, without the rows' share
@@ -142,7 +147,7 @@ __device__ __forceinline__ int64_t seq_work(const CacheParams& c, int b) {
 }
 
 // An item and the tiles [ta, tb) of its `nt` that a share [pos, end) of the line covers.
-template <int ROWS>
+template <int ROWS, int KEYS>
 struct Item {
   Seq s;
   Line<ROWS> line;
@@ -157,7 +162,7 @@ struct Item {
   }
   __device__ __forceinline__ void find(const CacheParams& c, int64_t pos) {  // pos lies in sequence b
     const int64_t x = pos - seq_start;
-    int lo = 0, hi = line.row_tiles - 1;
+    int lo = 0, hi = line.row_tiles - 1;  // one token per sequence: no search
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if (line.before(mid) * line.heads <= x) lo = mid;
@@ -165,25 +170,29 @@ struct Item {
     }
     rt = lo;
     cost = line.cost(rt);
-    h = (int)((x - line.before(rt) * line.heads) / cost);
+    h = (int)div_pos(x - line.before(rt) * line.heads, cost);
     start = seq_start + line.before(rt) * line.heads + h * cost;
     row = rt * ROWS;
     rows = min(s.q_len * c.group - row, ROWS);
     const int vis = visible_keys(c, s, (row + rows - 1) / c.group);
-    nt = vis > 0 ? (vis + kKeys - 1) / kKeys : 1;
+    nt = vis > 0 ? (vis + KEYS - 1) / KEYS : 1;
   }
-  __device__ __forceinline__ int tile_at(int64_t pos) const { return (int)((pos - start) * nt / cost); }
-  __device__ __forceinline__ void clip(int64_t pos, int64_t end) {
+  // The first tile of a share that begins at pos: whole tiles of keys x group before it, rounded down.
+  __device__ __forceinline__ int tile_at(const CacheParams& c, int64_t pos) const {
+    const int64_t t = div_pos(pos - start, (int64_t)c.group * KEYS);
+    return t < nt ? (int)t : nt;
+  }
+  __device__ __forceinline__ void clip(const CacheParams& c, int64_t pos, int64_t end) {
     inside = pos > start;
-    ta = tile_at(pos);
-    tb = end >= start + cost ? nt : tile_at(end);
+    ta = inside ? tile_at(c, pos) : 0;
+    tb = end >= start + cost ? nt : tile_at(c, end);
   }
 };
 
 // Walks the items of a share; every role of the CTA walks the same ones.
-template <int ROWS>
+template <int ROWS, int KEYS>
 struct Walk {
-  Item<ROWS> it;
+  Item<ROWS, KEYS> it;
   int64_t pos, end;
   __device__ __forceinline__ void begin(const CacheParams& c, const Spot& spot, int64_t p, int64_t e) {
     pos = p;
@@ -194,7 +203,7 @@ struct Walk {
     while (pos < end) {
       while (pos >= it.seq_start + it.line.total()) it.load_seq_at(c, it.b + 1, it.seq_start + it.line.total());
       it.find(c, pos);
-      it.clip(pos, end);
+      it.clip(c, pos, end);
       pos = min(end, it.start + it.cost);
       if (it.ta < it.tb) return true;
     }
@@ -203,33 +212,77 @@ struct Walk {
 };
 
 
-// The CTA's record of what it left to join (see Cut): the item that its share's end cuts, if that item began in the
-// share, and the tiles of its two partials.
-template <int ROWS>
-__device__ __forceinline__ void write_cut(const AttendParams& P, const SplitSpan& S, const CacheParams& c, const Spot& spot, int64_t begin,
-                                          int32_t error) {
-  Cut cut = {};
-  cut.error = error;
-  const int64_t end = S.begin(blockIdx.x + 1);
-  Item<ROWS> it;
-  it.load_seq_at(c, spot.seq, spot.first);
-  it.find(c, begin);
-  it.clip(begin, end);
-  if (it.inside) cut.tiles[0] = it.tb - it.ta;
-  if (end < S.total) {  // the item that holds the share's last unit
-    while (end - 1 >= it.seq_start + it.line.total()) it.load_seq_at(c, it.b + 1, it.seq_start + it.line.total());
-    it.find(c, end - 1);
-    if (it.start >= begin && it.start + it.cost > end) {
-      it.clip(it.start, end);
-      cut.tiles[1] = it.tb;
+// What the roles of a CTA need to know of an item.  The TMA warp walks the share and publishes its items through a
+// small ring in shared memory, one ahead of the one that it loads, so that the walk's divisions run once and off the
+// other roles' path.
+struct Job {
+  int64_t row0;                          // the sequence's first row
+  int32_t b, kv_len, q_len, row, rows, head;
+  int32_t ta, tb;                        // tiles; ta == tb: no more items
+  int32_t whole, inside;                 // all of the item's tiles; the item began before this share
+};
+constexpr int kJobs = 4;
+
+template <int ROWS, int KEYS>
+struct Publisher {
+  Walk<ROWS, KEYS> walk;
+  Cut cut;
+  uint32_t n;  // published so far
+  // Publishes the next item (lane 0 of the warp writes) and keeps it in `job`; false after a timeout.
+  __device__ __forceinline__ bool next(const CacheParams& c, const SplitSpan& S, Job* jobs, uint32_t full, uint32_t empty, int lane, volatile int* dead,
+                                       Job* job) {
+    Item<ROWS, KEYS>& it = walk.it;
+    const int64_t begin = S.begin(blockIdx.x);
+    const bool have = walk.next(c);
+    job->row0 = it.s.row0;
+    job->b = it.b;
+    job->kv_len = it.s.kv_len;
+    job->q_len = it.s.q_len;
+    job->row = it.row;
+    job->rows = it.rows;
+    job->head = it.h;
+    job->ta = have ? it.ta : 0;
+    job->tb = have ? it.tb : 0;
+    job->whole = it.ta == 0 && it.tb == it.nt;
+    job->inside = it.inside;
+    if (have && it.inside) cut.tiles[0] = it.tb - it.ta;
+    if (walk.pos >= walk.end && it.start >= begin && it.start + it.cost > walk.end) {  // the share ends inside the item
       cut.row0 = it.s.row0;
       cut.row = it.row;
       cut.rows = it.rows;
       cut.head = it.h;
       cut.last = S.owner(it.start + it.cost - 1);
+      cut.tiles[1] = it.tb;
     }
+    const uint32_t e = n % kJobs;
+    if (n >= kJobs && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * e, (n / kJobs - 1) & 1, dead))) return false;
+    if (lane == 0) {
+      jobs[e] = *job;
+      mbar_arrive(full + 8 * e);
+    }
+    ++n;
+    return true;
   }
-  P.cuts[blockIdx.x] = cut;
+};
+
+// The other side, for one thread that stands for its warp.
+__device__ __forceinline__ bool take_job_alone(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, volatile int* dead, Job* job) {
+  const uint32_t e = n % kJobs;
+  if (!mbar_wait(full + 8 * e, (n / kJobs) & 1, dead)) return false;
+  *job = jobs[e];
+  mbar_arrive(empty + 8 * e);
+  ++n;
+  return true;
+}
+// The other side: a warp takes the next item (false after a timeout) and frees its place at once.
+__device__ __forceinline__ bool take_job(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, int lane, volatile int* dead, Job* job) {
+  const uint32_t e = n % kJobs;
+  if (!warp_wait(full + 8 * e, (n / kJobs) & 1, dead)) return false;
+  *job = jobs[e];
+  __syncwarp();
+  if (lane == 0) mbar_arrive(empty + 8 * e);
+  ++n;
+  return true;
 }
 
 #endif  // __CUDACC__
@@ -260,14 +313,14 @@ inline bool pool_map(CUtensorMap* map, const void* pool, const CacheParams& c, b
 }
 
 
-// Pages must fill TMA boxes of whole swizzle groups (8 rows) that fit a tile of 128 keys evenly.
-inline bool pages_fit(const CacheParams& c) {
+// Pages must fill TMA boxes of whole swizzle groups (8 rows) that fit a tile of `keys` evenly.
+inline bool pages_fit(const CacheParams& c, int keys) {
   const int T = c.page_tokens;
-  return T % 8 == 0 && (T <= kKeys ? kKeys % T == 0 : T % kKeys == 0) && c.pool_pages * T < ((int64_t)1 << 31) && encode_tiled() != nullptr;
+  return T % 8 == 0 && (T <= keys ? keys % T == 0 : T % keys == 0) && c.pool_pages * T < ((int64_t)1 << 31) && encode_tiled() != nullptr;
 }
-inline PoolBoxes pool_boxes(const CacheParams& c) {
+inline PoolBoxes pool_boxes(const CacheParams& c, int keys) {
   PoolBoxes b;
-  b.rows = c.page_tokens < kKeys ? c.page_tokens : kKeys;
+  b.rows = c.page_tokens < keys ? c.page_tokens : keys;
   b.shift = 0;
   while (1 << b.shift < b.rows) ++b.shift;
   b.pool_rows = (int32_t)(c.pool_pages * c.page_tokens);
