@@ -189,3 +189,83 @@ def ragged(seed, batch, kv_max, q_max):
     r = random.Random(seed)
     kv = [r.randint(0, kv_max) for _ in range(batch)]
     return kv, [r.randint(0, min(q_max, max(n, 1))) for n in kv]
+
+
+def dense_sequence(pool, table, n):
+    """Tokens [0, n) of one sequence, on the pool's device: [n, H, D]."""
+    T = pool.shape[1]
+    at = torch.arange(n, device=pool.device)
+    return pool[table[at // T].long(), at % T]
+
+
+def attend_large(q, k_pool, v_pool, tables, kv_lens, q_lens, scale, rope_dim=0):
+    """``attend`` (causal) for long sequences: the same numbers and bounds, on the inputs' device, a head at a time."""
+    u, D = half_step(q.dtype), k_pool.shape[3]
+    H = k_pool.shape[2]
+    G = q.shape[1] // H
+    dv = D - (rope_dim if v_pool is None else 0)
+    out = torch.zeros((q.shape[0], q.shape[1], dv), dtype=torch.float64, device=q.device)
+    tol, lse = torch.zeros_like(out), torch.full(q.shape[:2], float("-inf"), dtype=torch.float64, device=q.device)
+    ltol = torch.zeros_like(lse)
+    row = 0
+    for b, (n, m) in enumerate(zip(kv_lens, q_lens)):
+        if n and m:
+            keys = dense_sequence(k_pool, tables[b], n).double()
+            vals = keys[..., D - dv:] if v_pool is None else dense_sequence(v_pool, tables[b], n).double()
+            hidden = torch.arange(n, device=q.device)[None] > (torch.arange(m, device=q.device) + n - m)[:, None]
+            for h in range(q.shape[1]):
+                qv, kv, vv = q[row:row + m, h].double(), keys[:, h // G], vals[:, h // G]
+                s = (qv @ kv.T * scale).masked_fill(hidden, float("-inf"))
+                size = (qv.abs() @ kv.abs().T * scale).masked_fill(hidden, 0).amax(1)
+                l = torch.logsumexp(s, 1)
+                w = torch.exp(s - l[:, None])
+                e = (D + 3) * U32 * size + s.masked_fill(hidden, 0).abs().amax(1) * 4 * U32 + (n + 8) * U32
+                o = w @ vv
+                out[row:row + m, h] = o
+                tol[row:row + m, h] = u * o.abs() + (u + 2 * e)[:, None] * (w @ vv.abs()) + torch.finfo(q.dtype).tiny
+                lse[row:row + m, h] = l
+                ltol[row:row + m, h] = e + 4 * U32 * l.abs()
+        row += m
+    return out.cpu(), lse.cpu(), tol.cpu(), ltol.cpu()
+
+
+def mass_large(q, k_pool, tables, kv_lens, q_lens, lse, before, decay, scale):
+    """``mass`` (causal) for long sequences, on the inputs' device."""
+    T, H, D = k_pool.shape[1:]
+    G = q.shape[1] // H
+    out = torch.zeros(tables.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    row = 0
+    for b, (n, m) in enumerate(zip(kv_lens, q_lens)):
+        page = torch.arange(n, device=q.device) // T
+        if n and m:
+            keys = dense_sequence(k_pool, tables[b], n).double()
+            hidden = torch.arange(n, device=q.device)[None] > (torch.arange(m, device=q.device) + n - m)[:, None]
+            for h in range(q.shape[1]):
+                qv, kv, l = q[row:row + m, h].double(), keys[:, h // G], lse[row:row + m, h, None].double()
+                s = (qv @ kv.T * scale).masked_fill(hidden, float("-inf"))
+                w = torch.exp(s - l).nan_to_num(nan=0.0)
+                e = ((D + 3) * U32 * (qv.abs() @ kv.abs().T) * scale + 4 * U32 * (s.masked_fill(hidden, 0).abs() + l.abs().nan_to_num(posinf=0.0))
+                     + (T + m * q.shape[1] + 8) * U32)
+                out[b].index_add_(0, page, w.sum(0))
+                tol[b].index_add_(0, page, (w * e).sum(0))
+        if before is not None:
+            out[b, :-(-n // T)] += decay * before[b, :-(-n // T)].double()
+        tol[b] += 4 * U32 * out[b].abs()
+        row += m
+    return out.cpu(), tol.cpu()
+
+
+def make_large_cache(kv_lens, T, H, D, dtype, seed, mla=False):
+    """``make_cache`` without NaN in the unused rows, made on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = [-(-n // T) for n in kv_lens]
+    pool = sum(pages) + 2
+    order = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+    tables = torch.full((len(kv_lens), max(pages)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(pages):
+        tables[b, :n] = order[at:at + n]
+        at += n
+    k, v = (torch.randn((pool, T, H, D), generator=g, device="cuda").to(dtype) for _ in range(2))
+    return k, None if mla else v, tables, torch.tensor(kv_lens, dtype=torch.int32, device="cuda")

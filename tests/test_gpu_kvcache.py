@@ -104,6 +104,27 @@ def test_long_context_splits():
     check_attend([5000], [1], 64, 1, 16, 576, BF16, mla_rope=64, decode=True)
 
 
+@pytest.mark.parametrize("H,G,D,T,mla_rope,q_max", [
+    (8, 4, 128, 64, None, 1), (8, 1, 64, 16, None, 1), (4, 8, 256, 64, None, 1), (1, 16, 576, 64, 64, 1),
+    (1, 40, 576, 16, 64, 2), (8, 4, 128, 64, None, 90), (4, 8, 64, 16, None, 33), (2, 2, 128, 48, None, 9)])
+def test_many_tiles_per_cta(H, G, D, T, mla_rope, q_max):
+    """Batches whose every CTA passes many tiles of several items through its rings, run three times over."""
+    batch = 40 if q_max == 1 else 8
+    kv, q_lens = ref.ragged(D + T, batch, 5000, q_max)
+    kv = [n + 1500 for n in kv]
+    q_lens = [max(1, m) for m in q_lens]
+    k, v, tables, lens = ref.make_large_cache(kv, T, H, D, BF16, 7, mla_rope is not None)
+    q = queries(sum(q_lens), H * G, D, BF16, 8)
+    out, lse, status = run_attend(q, k, v, tables, lens, q_lens, rope_dim=mla_rope or 0)
+    assert not status.any()
+    for _ in range(2):
+        again = run_attend(q, k, v, tables, lens, q_lens, rope_dim=mla_rope or 0)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    want, wl, tol, ltol = ref.attend_large(q, k, v, tables, kv, q_lens, D ** -0.5, mla_rope or 0)
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+
+
 def test_large_scores():
     # a scale of 1 on 128 columns: scores of tens, one weight near 1
     check_attend([500, 260], [3, 100], 64, 2, 4, 128, BF16, scale=1.0)
@@ -256,6 +277,30 @@ def test_mass_decode(dtype, T, H, G, D):
 @pytest.mark.parametrize("causal", [True, False])
 def test_mass_window(dtype, T, D, causal):
     check_mass([200, 0, 70, 33, 513], [32, 3, 70, 0, 64], T, 2, 4, D, dtype, causal=causal, empty=False)
+
+
+@pytest.mark.parametrize("H,G,D,T,q_max,batch", [(8, 4, 128, 64, 1, 40), (8, 4, 128, 64, 64, 6), (2, 8, 64, 16, 1, 40),
+                                                  (4, 4, 64, 16, 100, 6), (1, 16, 576, 64, 2, 20)])
+def test_mass_long_sequences(H, G, D, T, q_max, batch):
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = ref.ragged(D + T, batch, 5000, q_max)
+    kv = [n + 1500 for n in kv]
+    q_lens = [max(1, m) for m in q_lens]
+    k, _, tables, lens = ref.make_large_cache(kv, T, H, D, BF16, 9, True)
+    q = queries(sum(q_lens), H * G, D, BF16, 8)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    out = torch.empty((q.shape[0], H * G, D - 64 if D > 512 else D), dtype=BF16, device=DEV)
+    starts = ref.starts_of(q_lens)
+    kvcache.attend_pages(q, k, None if D > 512 else k.clone(), tables, lens, out, lse=lse, q_starts=starts,
+                         max_q_len=q_max, rope_dim=64 if D > 512 else 0)
+    before = torch.rand(tables.shape, device=DEV)
+    mass = torch.empty_like(before)
+    for _ in range(3):
+        kvcache.page_mass(q, k, tables, lens, lse, before, mass, decay=0.5, q_starts=starts, max_q_len=q_max)
+        torch.cuda.synchronize()
+    want, tol = ref.mass_large(q, k, tables, kv, q_lens, lse, before, 0.5, D ** -0.5)
+    ref.assert_close(mass, want, tol, "mass")
 
 
 def test_mass_more_rows_than_tokens():

@@ -27,7 +27,7 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kTurns = 4;
-constexpr int kBars = 48;  // barrier slots at the start of shared memory
+constexpr int kBars = 40;  // barrier slots at the start of shared memory
 
 struct DecodeParams {
   AttendParams a;
@@ -49,11 +49,12 @@ struct Shape {
   static constexpr int kPBlock = kTileKeys * 32;                        // P^T of 16 rows
   static constexpr int kPBytes = N / 16 * kPBlock;
   static constexpr int kTail = 2 * kPBytes + kQBytes;
-  static constexpr int kSlots = (232448 - 8192 - kTail) / kSlotBytes;
+  static constexpr int kRoom = (232448 - 8192 - kTail) / kSlotBytes;
+  static constexpr int kSlots = kRoom < 3 * kTileSlots ? kRoom : 3 * kTileSlots;  // fewer than four tiles: see s_full
   static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kTail;
   static constexpr int kCols = (2 + 2 * MB) * N <= 64 ? 64 : ((2 + 2 * MB) * N <= 128 ? 128 : ((2 + 2 * MB) * N <= 256 ? 256 : 512));
   // the next tile's K and this tile's V share the ring
-  static_assert(kSlots >= (SHARED ? 2 * kTileSlots : kTileSlots + kKSlots) && 2 * kSlots + 12 + 2 * kJobs <= kBars && (2 + 2 * MB) * N <= kCols, "shape");
+  static_assert(kSlots >= (SHARED ? 2 * kTileSlots : kTileSlots + kKSlots) && kSlots + 16 + 2 * kJobs <= kBars && (2 + 2 * MB) * N <= kCols, "shape");
   // first column group, and number of groups, of slot s of a tile's K
   static __device__ __forceinline__ constexpr int group(int s) { return SHARED ? (s == 0 ? 0 : 2 * s - 1) : s * kGroups; }
   static __device__ __forceinline__ constexpr int groups(int s) { return SHARED && s == 0 ? 1 : kGroups; }
@@ -113,9 +114,9 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   __shared__ uint32_t tmem_s;
   __shared__ float4 s_max[2][2][N], s_sum[2][N];  // per group (and tile, by turns) and row: one value of each warp
   __shared__ float s_top[2][N];                   // per group and row: the maximum in use
-  __shared__ float2 s_mix[N];                     // per row: what the groups' O count
-  __shared__ int64_t s_row[kTurns][N];            // per item, by turns, and row: the row of the output,
-  __shared__ int32_t s_lim[2][kTurns][N];         // and (per group) the keys that it sees
+  __shared__ float2 s_mix[2][N];                     // per row: what the groups' O count
+  __shared__ int64_t s_row[2][kTurns][N];         // per group, item (by turns) and row: the row of the output,
+  __shared__ int32_t s_lim[2][kTurns][N];         // and the keys that it sees
   __shared__ Job s_jobs[kJobs];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -125,34 +126,27 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   const uint32_t ring = (bars + kBars * 8 + 1023) & ~1023u;
   const uint32_t qbuf = ring + kSlots * Sh::kSlotBytes, pbuf = qbuf + Sh::kQBytes;
   auto full = [&](uint32_t s) { return bars + s * 8; };
-  auto empty = [&](uint32_t s) { return bars + (kSlots + s) * 8; };
-  // q_full: Q is there; s_full, p_full, pv_done, meet: per group; summed, read: the second group's sums, and O, at an
-  // item's end
-  const uint32_t q_full = bars + 2 * kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, meet = pv_done + 16,
+  // s_full, pv_done: a tile's scores and products are done, four barriers by turns -- the TMA warp, which waits for the
+  // tiles whose slots it refills, may find up to three later ones done as well, and a barrier tells a phase only from
+  // the next one.  q_full: Q is there; p_full, meet: per group; summed, read: at an item's end, both groups' sums are
+  // there and both have read O
+  const uint32_t q_full = bars + kSlots * 8, s_full = q_full + 8, p_full = s_full + 32, pv_done = p_full + 16, meet = pv_done + 32,
                  summed = meet + 16, read = summed + 8, job_full = read + 8, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
 
-  int64_t at;
-  Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<N>(c, b); }, &at, &spot);
-  if (at < 0) {
-    if (tid == 0) P.a.cuts[blockIdx.x] = Cut{};
-    return;
-  }
   if (tid == 0) {
     dead_s = 0;
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
-    }
+    for (int s = 0; s < kSlots; ++s) mbar_init(full(s), 1);
     mbar_init(q_full, 256);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(pv_done + 8 * i, 1);
+    }
     for (int g = 0; g < 2; ++g) {
-      mbar_init(s_full + 8 * g, 1);
       mbar_init(p_full + 8 * g, 128);
-      mbar_init(pv_done + 8 * g, 1);
       mbar_init(meet + 8 * g, 4);
     }
-    mbar_init(summed, 4);
-    mbar_init(read, 4);
+    mbar_init(summed, 8);
+    mbar_init(read, 8);
     for (int e = 0; e < kJobs; ++e) {
       mbar_init(job_full + 8 * e, 1);
       mbar_init(job_empty + 8 * e, 9);
@@ -174,13 +168,16 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     // ---- TMA: a tile's slots in turn through the ring; lane p fetches page p of the tile ------------
     const int per_tile = kTileKeys / P.box.rows;
     uint32_t pos = 0;
+    int64_t at;
+    Spot spot;
+    const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work<N>(c, b); }, &at, &spot);
     Publisher<N, kTileKeys> pub;
-    pub.walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+    pub.walk.begin(c, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
     pub.cut = Cut{};
     pub.n = 0;
-    Job job, then;
-    bool ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job);
-    while (ok && job.ta < job.tb) {
+    Job job;
+    bool ok = true;
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
       for (int t = job.ta; ok && t < job.tb; ++t) {
         const int j = t * kTileKeys + lane * P.box.rows;
         int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
@@ -191,7 +188,10 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
 #pragma unroll
         for (int s = 0; s < kTS; ++s, ++pos) {
           const uint32_t slot = pos % kSlots;
-          ok = ok && (pos < kSlots || mbar_wait(empty(slot), (pos / kSlots - 1) & 1, dead));
+          if (pos >= kSlots) {  // the slot's last tile: its K is done with its scores, its V (or shared K) with its products
+            const uint32_t was = pos - kSlots, tile = was / kTS;
+            ok = ok && mbar_wait((SHARED || was % kTS >= kKS ? pv_done : s_full) + 8 * (tile & 3), (tile >> 2) & 1, dead);
+          }
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -206,10 +206,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
               tma_load(ring + slot * Sh::kSlotBytes + g * kGroupBytes + lane * P.box.rows * 128, isv ? &vmap : &kmap, (g0 + g) * 64, job.head, row,
                        full(slot));
         }
-        // the item behind this one, looked up once this one's first loads are out
-        if (ok && t == job.ta) ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &then);
       }
-      job = then;
     }
     if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
     if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
@@ -236,32 +233,31 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
           const uint32_t pos = step * kTS + s, slot = pos % kSlots;
           if (!wait(full(slot), pos / kSlots)) return;
           tc_fence_after();
-          const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (step & 1) * N, done = empty(slot),
-                         sbar = s_full + 8 * (step & 1);
+          const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (step & 1) * N;
 #pragma unroll
           for (int g = 0; g < Sh::groups(s); ++g)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mma_ss(d, a + ((g * kGroupBytes + k * 32) >> 4), kHi, q_lo + (((Sh::group(s) + g) * N * 128 + k * 32) >> 4), kHi, qk,
                      Sh::group(s) + g > 0 || k > 0);
-          if (!SHARED || s == 0) tc_commit(done);
-          if (s == kKS - 1) tc_commit(sbar);
         }
+        tc_commit(s_full + 8 * (step & 3));
       };
       auto values = [&](uint32_t step, bool acc) {  // O^T += V^T P^T
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           const uint32_t pos = step * kTS + (SHARED ? 1 : kKS) + mb, slot = pos % kSlots;
-          if (!wait(full(slot), pos / kSlots)) return;
-          tc_fence_after();
-          const uint32_t a = v_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (2 + (step & 1) * MB + mb) * N, done = empty(slot),
-                         p = p_lo + (step & 1) * (Sh::kPBytes >> 4), pbar = pv_done + 8 * (step & 1);
+          if (!SHARED) {  // a shared tile has been waited for by its scores
+            if (!wait(full(slot), pos / kSlots)) return;
+            tc_fence_after();
+          }
+          const uint32_t a = v_lo + slot * (Sh::kSlotBytes >> 4), d = tmem + (2 + (step & 1) * MB + mb) * N,
+                         p = p_lo + (step & 1) * (Sh::kPBytes >> 4);
 #pragma unroll
           for (int k = 0; k < kTileKeys / 16; ++k)
             mma_ss(d, a + (k * 2048 >> 4), kHi, p + (k * 512 >> 4), kPHi, pv, acc || k > 0);
-          tc_commit(done);
-          if (mb == MB - 1) tc_commit(pbar);
         }
+        tc_commit(pv_done + 8 * (step & 3));
       };
       uint32_t step = 0, items = 0;
       Job job;
@@ -297,6 +293,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     const uint32_t pdst = pbuf + wg * Sh::kPBytes + key * 32;
     const int chunks = c.head_dim / 8;
     uint32_t step = 0, mine = 0, meets = 0, nitem = 0;  // tiles of the CTA, of this group, meetings, items
+    auto tile_wait = [&](uint32_t bars, uint32_t tile) { return warp_wait(bars + 8 * (tile & 3), (tile >> 2) & 1, dead); };
     // The group's four warps meet.  Not a bar.sync, which no bound could end if a warp had left after a timeout.
     auto meet_warps = [&] {
       __syncwarp();
@@ -312,7 +309,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       if (job.ta == job.tb) return true;
       if (wt < job.rows) {
         const int tok = (job.row + wt) / c.group, gh = job.row + wt - tok * c.group;
-        if (wg == 0) s_row[jobs % kTurns][wt] = (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + gh;
+        s_row[wg][jobs % kTurns][wt] = (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + gh;
         s_lim[wg][jobs % kTurns][wt] = visible_keys(c, Seq{job.kv_len, job.q_len, job.row0}, tok);
       }
       constexpr int kAhead = KG > 2 ? 4 : 1;  // chunks of 16 bytes in flight per thread
@@ -354,13 +351,18 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       for (int t = it.ta + ((int)(step & 1) ^ wg); t < it.tb; t += 2, ++mine) {
         const int j0 = t * kTileKeys, j = j0 + key;
         const bool there = holds && j < it.kv_len && pool_row(c, it.b, j) >= 0;
-        if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
+        const uint32_t g = 2 * mine + wg;  // the CTA's tile
+        if (!(ok = tile_wait(s_full, g))) break;
         tc_fence_after();
         uint32_t x[N];
         tmem_ld_cols<N>(ts, x);
         if (fresh && !(ok = meet_warps())) break;  // the item's tables are written
+        if (!holds) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) x[n] = 0xff800000u;
+        }
         // the first row sees the least
-        if (j0 + kTileKeys > s_lim[wg][turn][0] || !__all_sync(0xffffffffu, there)) {
+        if (j0 + kTileKeys > s_lim[wg][turn][0] || !__all_sync(0xffffffffu, there || !holds)) {
 #pragma unroll
           for (int n = 0; n < N; ++n)
             if (n < rows && !(there && j < s_lim[wg][turn][n])) x[n] = 0xff800000u;
@@ -384,8 +386,8 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
         const float zero = top == -INFINITY ? 0.f : top;
         const bool grow = __any_sync(0xffffffffu, grows);
         // the group's product before has read P and written O; at an item's start, O has been read as well
-        if (mine > 0 && !(ok = warp_wait(pv_done + 8 * wg, (mine - 1) & 1, dead))) break;
-        if (wg == 1 && fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+        if (mine > 0 && !(ok = tile_wait(pv_done, g - 2))) break;
+        if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
         if (!fresh && grow) {  // the same in every thread of the group
           tc_fence_after();
 #pragma unroll
@@ -417,7 +419,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
         // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V
         if (j0 + kTileKeys > it.kv_len && it.kv_len % c.page_tokens != 0) {
           for (int s = SHARED ? 1 : kKS; s < kTS; ++s) {
-            const uint32_t pos = (step + t - it.ta) * kTS + s, slot = pos % kSlots;
+            const uint32_t pos = g * kTS + s, slot = pos % kSlots;
             if (!(ok = warp_wait(full(slot), (pos / kSlots) & 1, dead))) break;
             if (j >= it.kv_len && holds)
               for (int i = 0; i < kKGroups * 8; ++i)
@@ -432,67 +434,71 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       }
       if (!ok) break;
       // the item's last QK^T is done: the next one's Q may come
-      if (!(ok = warp_wait(s_full + 8 * (last & 1), (last >> 1) & 1, dead)) || !(ok = open())) break;
+      if (!(ok = tile_wait(s_full, last)) || !(ok = open())) break;
 
-      // the groups' maxima and sums meet in shared memory; the first group joins them and writes the item
-      if (wg == 1 && fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+      // The groups' maxima and sums meet in shared memory; each group then joins and writes its share of the columns
+      // (one block of columns: its share of the rows).
+      if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
       {
-        // N values over 32 lanes: each step halves the values a lane holds and the lanes that share one
         const float sum = lane_sums<N>(l, lane);
         if (lane < N) reinterpret_cast<float*>(s_sum[wg])[4 * lane + ww] = sum;
         if (wt < N) s_top[wg][lane] = top;
       }
-      if (wg == 1) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(summed);
-      } else {
-        if (!(ok = meet_warps()) || !(ok = warp_wait(summed, nitem & 1, dead))) break;
-        float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
-        if (wt < rows) {
-          const float4 u = s_sum[0][wt], v = s_sum[1][wt];
-          const float m0 = s_top[0][wt], m1 = s_top[1][wt];
-          const float mm = fmaxf(m0, m1), z = mm == -INFINITY ? 0.f : mm;
-          const float f0 = fast_exp2(m0 - z), f1 = fast_exp2(m1 - z);
-          const float sum = ((u.x + u.y) + (u.z + u.w)) * f0 + ((v.x + v.y) + (v.z + v.w)) * f1;
-          const float inv = it.whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
-          s_mix[wt] = make_float2(f0 * inv, f1 * inv);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(summed);
+      if (!(ok = warp_wait(summed, nitem & 1, dead))) break;
+      float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
+      if (wt < rows) {
+        const float4 u = s_sum[0][wt], v = s_sum[1][wt];
+        const float m0 = s_top[0][wt], m1 = s_top[1][wt];
+        const float mm = fmaxf(m0, m1), z = mm == -INFINITY ? 0.f : mm;
+        const float f0 = fast_exp2(m0 - z), f1 = fast_exp2(m1 - z);
+        const float sum = ((u.x + u.y) + (u.z + u.w)) * f0 + ((v.x + v.y) + (v.z + v.w)) * f1;
+        const float inv = it.whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+        s_mix[wg][wt] = make_float2(f0 * inv, f1 * inv);
+        if (wg == 0) {
           if (!it.whole) {
             part[P.a.part_rows * c.v_dim + wt] = mm;
             part[P.a.part_rows * (c.v_dim + 1) + wt] = sum;
           } else if (P.a.lse) {
-            P.a.lse[s_row[turn][wt]] = sum == 0.f ? -INFINITY : fmaf(mm, 0.693147180559945f, logf(sum));
+            P.a.lse[s_row[wg][turn][wt]] = sum == 0.f ? -INFINITY : fmaf(mm, 0.693147180559945f, logf(sum));
           }
         }
-        if (!(ok = meet_warps())) break;
-        if (!(ok = warp_wait(pv_done + 8 * (last & 1), (last >> 1) & 1, dead))) break;
-        if (last != step && !(ok = warp_wait(pv_done + 8 * (~last & 1), ((last - 1) >> 1) & 1, dead))) break;
-        tc_fence_after();
-#pragma unroll 1
-        for (int mb = 0; mb < MB; ++mb) {
-          uint32_t o[N], o1[N];
-          tmem_ld_cols<N>(tmem + lanes + (2 + mb) * N, o);
-          tmem_ld_cols<N>(tmem + lanes + (2 + MB + mb) * N, o1);
-          const int col = mb * 128 + wt;
-          if (col < c.v_dim) {
-#pragma unroll
-            for (int n = 0; n < N; n += 4)
-              if (n < rows) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 w = s_mix[n + e];  // a group without tiles has weight 0 and an O that holds anything
-                  const float v = (w.x != 0.f ? __uint_as_float(o[n + e]) * w.x : 0.f) + (w.y != 0.f ? __uint_as_float(o1[n + e]) * w.y : 0.f);
-                  if (n + e < rows) {
-                    if (it.whole) P.a.out[s_row[turn][n + e] * c.v_dim + col] = (uint16_t)(pack2<BF16>(v, 0.f) & 0xffff);
-                    else part[(n + e) * c.v_dim + col] = v;
-                  }
-                }
-              }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(read);
       }
+      if (!(ok = meet_warps())) break;
+      if (!(ok = tile_wait(pv_done, last))) break;
+      if (last != step && !(ok = tile_wait(pv_done, last - 1))) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int mb = MB > 1 ? wg : 0; mb < MB; mb += 2) {
+        uint32_t o[N], o1[N];
+        tmem_ld_cols<N>(tmem + lanes + (2 + mb) * N, o);
+        tmem_ld_cols<N>(tmem + lanes + (2 + MB + mb) * N, o1);
+        const int col = mb * 128 + wt;
+        if (col < c.v_dim) {
+#pragma unroll
+          for (int n = 0; n < N; n += 4)
+            if (n < rows && (MB > 1 || (n / 4 & 1) == wg)) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 w = s_mix[wg][n + e];  // a group without tiles has weight 0 and an O that holds anything
+                v[e] = (w.x != 0.f ? __uint_as_float(o[n + e]) * w.x : 0.f) + (w.y != 0.f ? __uint_as_float(o1[n + e]) * w.y : 0.f);
+              }
+              if (it.whole) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n + e < rows) P.a.out[s_row[wg][turn][n + e] * c.v_dim + col] = (uint16_t)(pack2<BF16>(v[e], 0.f) & 0xffff);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[(n + e) * c.v_dim + col] = v[e];  // rows up to N have room
+              }
+            }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(read);
       step = last + 1;
       ++nitem;
     }

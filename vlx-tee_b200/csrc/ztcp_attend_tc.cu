@@ -86,13 +86,6 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
                  job_full = o_full + 16, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
   static_assert(2 * SLOTS + 9 + 2 * kJobs <= kBars, "barrier slots");
 
-  int64_t at;
-  Spot spot;
-  const SplitSpan S = locate(c.n_seqs, P.a.grid, [&](int b) { return seq_work<kItemRows>(c, b); }, &at, &spot);
-  if (at < 0) {
-    if (tid == 0) P.a.cuts[blockIdx.x] = Cut{};
-    return;
-  }
   if (tid == 0) {
     dead_s = 0;
     for (int s = 0; s < SLOTS; ++s) {
@@ -126,13 +119,16 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     // ---- TMA: K and V tiles in turn through the ring; lane p fetches page p of the tile ------------
     const int per_tile = kKeys / P.box.rows;
     uint32_t pos = 0;  // tiles so far: K of step t is 2 t, V is 2 t + 1
+    int64_t at;
+    Spot spot;
+    const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work<kItemRows>(c, b); }, &at, &spot);
     Publisher<kItemRows, kKeys> pub;
-    pub.walk.begin(c, spot, at, S.begin(blockIdx.x + 1));
+    pub.walk.begin(c, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
     pub.cut = Cut{};
     pub.n = 0;
-    Job job, then;
-    bool ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job);
-    while (ok && job.ta < job.tb) {
+    Job job;
+    bool ok = true;
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
       for (int t = job.ta; ok && t < job.tb; ++t) {
         const int j = t * kKeys + lane * P.box.rows;
         int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
@@ -155,10 +151,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
             for (int x = 0; x < HALVES; ++x)
               tma_load(ring + slot * kTile + x * kHalf + lane * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, job.head, row, full(slot));
         }
-        // the item behind this one, looked up once this one's first loads are out
-        if (ok && t == job.ta) ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &then);
       }
-      job = then;
     }
     if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
     if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
@@ -187,15 +180,14 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       const uint32_t tm = tmem;
       // Step t multiplies P of tile t - 1 by V and computes the scores of tile t; per row tile in turn, so that each
       // has the other's products to hide its softmax under.
-      Job job, then;
+      Job job;
       uint32_t njobs = 0;
       int cur = 0, n = 0;  // row tiles of the step before, and tiles of its item
       int t = 0;           // of the item's tiles, those whose scores are out
-      ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &then);
       while (ok) {
         const bool fresh = t == n;  // the step's scores are those of the next item
-        if (fresh) {
-          job = then;
+        if (fresh) {  // published once the loads of the item before are out
+          if (!(ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job))) break;
           if (cur == 0 && job.ta == job.tb) break;
         }
         const int nxt = fresh ? (job.ta < job.tb ? (job.rows > kRowTile ? 2 : 1) : 0) : cur;
@@ -241,7 +233,6 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           if (nxt == 0) break;
           n = job.tb - job.ta;
           t = 0;
-          ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &then);
         }
         cur = nxt;
         ++t;

@@ -9,7 +9,7 @@ namespace ztcp {
 
 constexpr int kKeys = 128;                           // keys per tile
 constexpr int kGroupBytes = kKeys * 128;             // a tile's 64-column group: 128 rows of 128 bytes
-constexpr uint32_t kWaitTries = 2000000;             // bound of a wait: 0.05 to 2 seconds
+constexpr long long kWaitCycles = 2000000000ll;      // bound of a wait: a second or so
 
 // Boxes of the pool's TMA loads.
 struct PoolBoxes {
@@ -30,17 +30,25 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for the phase of this parity; false when the wait ran out (kWaitTries attempts, each of which the hardware may
-// suspend for about a microsecond), and the CTA's dead flag is set.  The loop is written out because its length is on
-// the product warp's critical path (measured: 7 cycles when the phase is there, against 65 for a loop in C).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred P, Q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n\tTRY%=:\n\tmbarrier.try_wait.parity.shared.b64 P, [%1], %2;\n\t@P bra DONE%=;\n\t"
-      "add.u32 n, n, 1;\n\tsetp.lt.u32 Q, n, %3;\n\t@Q bra TRY%=;\n\tDONE%=:\n\tselp.u32 %0, 1, 0, P;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity), "n"(kWaitTries) : "memory");
-  if (!ok) *dead = 1;
+      "{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared.b64 P, [%1], %2;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
+}
+// Waits for the phase of this parity.  False when the wait ran out: here, which sets the CTA's dead flag, or in another
+// role.  (A single attempt may be suspended by the hardware for tens of microseconds, so the bound is one of time.)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try(bar, parity)) return true;
+  const long long start = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*dead) return false;
+    if (clock64() - start > kWaitCycles) {
+      *dead = 1;
+      return false;
+    }
+  }
+  return true;
 }
 // One lane of a converged warp, always the same.  The compiler keeps the operands of what it guards in uniform
 // registers, which tcgen05 instructions read (measured: 39 cycles per small product, against 44 to 53 under lane == 0).
@@ -198,6 +206,9 @@ struct Walk {
     pos = p;
     end = e;
     it.load_seq_at(c, spot.seq, spot.first);
+    it.start = it.cost = 0;  // no item yet
+    it.rt = it.h = it.nt = it.ta = it.tb = it.rows = it.row = 0;
+    it.inside = false;
   }
   __device__ __forceinline__ bool next(const CacheParams& c) {  // the next item with tiles, in `it`
     while (pos < end) {
@@ -212,9 +223,50 @@ struct Walk {
 };
 
 
+// The share of a CTA, found by one warp: sums every sequence's units, 32 sequences at a time, and finds the sequence
+// that holds the share's first unit (-1: the share is empty).
+template <class Count>
+__device__ __forceinline__ SplitSpan locate_warp(int n_seqs, int grid, int lane, Count count, int64_t* want, Spot* spot) {
+  auto sums = [&](int base) {  // inclusive, over the 32 sequences from `base`
+    int64_t x = base + lane < n_seqs ? count(base + lane) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += o;
+    }
+    return x;
+  };
+  SplitSpan S;
+  S.total = 0;
+  int64_t x = 0;
+  for (int base = 0; base < n_seqs; base += 32) {
+    x = sums(base);
+    S.total += __shfl_sync(0xffffffffu, x, 31);
+  }
+  S.share = div_pos(S.total + grid - 1, grid);
+  if (S.share == 0) S.share = 1;
+  *want = S.own_begin();
+  spot->seq = 0;
+  spot->first = 0;
+  if (*want >= 0)
+    for (int base = 0; base < n_seqs; base += 32) {
+      if (n_seqs > 32) x = sums(base);
+      const unsigned m = __ballot_sync(0xffffffffu, *want < spot->first + x);
+      if (m) {
+        const int l = __ffs(m) - 1;
+        const int64_t before = __shfl_sync(0xffffffffu, x, l > 0 ? l - 1 : 0);
+        spot->seq = base + l;
+        spot->first += l > 0 ? before : 0;
+        break;
+      }
+      spot->first += __shfl_sync(0xffffffffu, x, 31);
+    }
+  return S;
+}
+
 // What the roles of a CTA need to know of an item.  The TMA warp walks the share and publishes its items through a
-// small ring in shared memory, one ahead of the one that it loads, so that the walk's divisions run once and off the
-// other roles' path.
+// small ring in shared memory, so that the walk's divisions run once and, as that warp is a ring of tiles ahead, off
+// the other roles' path.
 struct Job {
   int64_t row0;                          // the sequence's first row
   int32_t b, kv_len, q_len, row, rows, head;
