@@ -81,12 +81,16 @@ int64_t ztcp_attend_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queri
 int32_t ztcp_attend_pages(const ztcp_kv_cache* cache, const ztcp_queries* queries, void* out, float* lse,
                           int32_t* status, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Workspace bytes of ztcp_page_mass on the current device; -1 when the arguments are invalid. */
+int64_t ztcp_page_mass_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queries* queries);
+
 /* out_mass[b, p] = decay * mass[b, p] + sum over the sequence's rows, their heads and the tokens j of page p that
  * the row sees, of exp(scale * score - lse[row, head]); 0 past the sequence's last page.  mass and out_mass are
  * [n_seqs, max_pages] fp32, dense, and may be the same memory; mass may be NULL (no earlier weight).  lse as
- * ztcp_attend_pages writes it; a row whose lse is -inf adds nothing. */
+ * ztcp_attend_pages writes it; a row whose lse is -inf adds nothing.  `workspace`: as for ztcp_attend_pages. */
 int32_t ztcp_page_mass(const ztcp_kv_cache* cache, const ztcp_queries* queries, const float* lse, const float* mass,
-                       float decay, float* out_mass, int32_t* status, void* stream);
+                       float decay, float* out_mass, int32_t* status, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 /* Norm, rotation and append of new tokens.  Row r of q (num_q_heads vectors) goes to q_out (dense), of k and v
  * (geom.num_heads vectors each) to pool slot slots[r] (page slots[r] / num_tokens, row slots[r] % num_tokens); a

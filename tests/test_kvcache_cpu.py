@@ -74,7 +74,7 @@ def test_attend_and_mass_refusals(lib, ckw, qkw, msg):
     assert lib.ztcp_attend_workspace_bytes(c, q) == -1 and lib.ztcp_last_error().decode() == msg
     assert lib.ztcp_attend_pages(c, q, FAKE, None, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
     assert lib.ztcp_last_error().decode() == msg
-    assert lib.ztcp_page_mass(c, q, FAKE, None, 1.0, FAKE, FAKE, None) == capi.ZTCP_EINVAL
+    assert lib.ztcp_page_mass(c, q, FAKE, None, 1.0, FAKE, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
     assert lib.ztcp_last_error().decode() == msg
 
 
@@ -95,12 +95,14 @@ def test_attend_refusals(lib):
 
 
 def test_mass_refusals(lib):
-    def refuse(msg, lse=FAKE, decay=1.0, out=FAKE, status=FAKE):
-        rc = lib.ztcp_page_mass(cache(), rows(), lse, None, decay, out, status, None)
+    def refuse(msg, lse=FAKE, decay=1.0, out=FAKE, status=FAKE, ws=FAKE):
+        rc = lib.ztcp_page_mass(cache(), rows(), lse, None, decay, out, status, ws, 1 << 40, None)
         assert rc == capi.ZTCP_EINVAL and lib.ztcp_last_error().decode() == msg
 
-    refuse("lse, out_mass and status must not be NULL", lse=None)
-    refuse("lse, out_mass and status must not be NULL", out=None)
+    refuse("lse, out_mass, status and workspace must not be NULL", lse=None)
+    refuse("lse, out_mass, status and workspace must not be NULL", out=None)
+    refuse("lse, out_mass, status and workspace must not be NULL", ws=None)
+    refuse("workspace must be 16-byte aligned", ws=FAKE + 8)
     refuse("decay must be finite", decay=float("inf"))
 
 

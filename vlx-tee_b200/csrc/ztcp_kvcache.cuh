@@ -30,6 +30,7 @@ struct CacheParams {
   int32_t kv_heads, group;          // group = query heads per KV head
   int32_t head_dim, v_dim, v_col;
   int32_t causal;
+  float scale;
   float scale_log2;  // scale * log2(e): scores enter exp2
   int32_t* status;
 };
@@ -64,7 +65,10 @@ struct MassParams {
   const float* mass;  // or null
   float decay;
   float* out;
-  int32_t unit_pages;  // whole pages per unit of work
+  int32_t unit_pages;  // general kernel: whole pages per unit of work
+  int32_t grid;        // tensor-core kernel: CTAs,
+  int32_t* errors;     // one word each,
+  float* part;         // and segment sums
 };
 
 // The attention kernels: whether they can take a call, their shape, and the launch (false: no tensor map could be
@@ -80,6 +84,10 @@ bool launch_attend_decode(const AttendParams& P, bool bf16, cudaStream_t s);
 // Joins what the kernel before it left to join, and writes the sequences' status; `rows`: of an item, at most.
 void launch_attend_merge(const AttendParams& P, bool bf16, int64_t rows, cudaStream_t s);
 void launch_page_mass(const MassParams& P, bool bf16, cudaStream_t s);
+// Tensor-core kernel (ztcp_mass_tc.cu): whether it can take a call, workspace bytes, launch (false: no tensor map).
+bool page_mass_tc_fits(const CacheParams& c);
+int64_t page_mass_tc_workspace(const CacheParams& c, int sms);
+bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s);
 
 // ------------------------------------------------------------------------------------------------
 // Device helpers

@@ -81,6 +81,7 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   c->v_col = k->v_pool ? 0 : (int32_t)g.rope_dim;
   c->v_dim = c->head_dim - c->v_col;
   c->causal = q->causal != 0;
+  c->scale = q->scale;
   c->scale_log2 = (float)((double)q->scale * 1.4426950408889634);
   return ZTCP_OK;
 }
@@ -99,10 +100,15 @@ int32_t launched(const char* what) {
   return ZTCP_OK;
 }
 
-// The kernel of a call.  Items of at most 64 rows (of one token or a few, and a group) leave the tensor cores idle
-// whatever is done, so the decode kernel turns the products over and reads K and V at memory speed; more rows take
-// the chunk kernel's 256-row items.  What their loads cannot take (odd page sizes, other head dims) goes to the
-// general kernel.
+int sm_count() {  // of the current device; 0 without one
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return sms;
+}
+
+// The kernel of a call.  Items of few rows (one token or a few, times a group) leave the tensor cores idle whatever is
+// done, so the decode kernel turns the products over and reads K and V at memory speed; more rows take the chunk
+// kernel's 256-row items.  What their loads cannot take (odd page sizes, other head dims) goes to the general kernel.
 enum class Kernel { general, chunk, decode };
 
 Kernel pick_kernel(const ztcp::CacheParams& c, const ztcp_queries* q) {
@@ -113,8 +119,8 @@ Kernel pick_kernel(const ztcp::CacheParams& c, const ztcp_queries* q) {
 
 // Fills the workspace-dependent part of P for a workspace at `base`; returns the bytes it takes, 0 without a device.
 int64_t plan(Kernel k, const ztcp::CacheParams& c, const ztcp_queries* q, void* base, ztcp::AttendParams* P) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  const int sms = sm_count();
+  if (sms <= 0) return 0;
   const ztcp::AttendShape s = k == Kernel::chunk    ? ztcp::attend_tc_shape(c, sms)
                               : k == Kernel::decode ? ztcp::attend_decode_shape(c, sms, c.group * q->max_q_len)
                                                     : ztcp::attend_shape(c, sms);
@@ -169,20 +175,43 @@ int32_t ztcp_attend_pages(const ztcp_kv_cache* cache, const ztcp_queries* querie
   return launched("attend_merge_kernel");
 }
 
+int64_t ztcp_page_mass_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queries* queries) {
+  ztcp::CacheParams c;
+  if (to_params(cache, queries, &c) != ZTCP_OK) return -1;
+  const int sms = sm_count();
+  if (sms <= 0) {
+    launched("ztcp_page_mass_workspace_bytes");
+    return -1;
+  }
+  return ztcp::page_mass_tc_fits(c) ? ztcp::page_mass_tc_workspace(c, sms) : 16;
+}
+
 int32_t ztcp_page_mass(const ztcp_kv_cache* cache, const ztcp_queries* queries, const float* lse, const float* mass,
-                       float decay, float* out_mass, int32_t* status, void* stream) {
-  ztcp::MassParams P;
+                       float decay, float* out_mass, int32_t* status, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+  ztcp::MassParams P = {};
   const int32_t rc = to_params(cache, queries, &P.c);
   if (rc != ZTCP_OK) return rc;
-  if (!lse || !out_mass || !status) return invalid("lse, out_mass and status must not be NULL");
+  if (!lse || !out_mass || !status || !workspace) return invalid("lse, out_mass, status and workspace must not be NULL");
+  if (!aligned(workspace, 16)) return invalid("workspace must be 16-byte aligned");
   if (!isfinite(decay)) return invalid("decay must be finite");
+  const int sms = sm_count();
+  if (sms <= 0) return launched("ztcp_page_mass") != ZTCP_OK ? ZTCP_ECUDA : set_last_error(ZTCP_ECUDA, "no CUDA device");
+  const bool tc = ztcp::page_mass_tc_fits(P.c);
+  if (workspace_bytes < (tc ? ztcp::page_mass_tc_workspace(P.c, sms) : 16)) return invalid("workspace smaller than ztcp_page_mass_workspace_bytes");
   P.c.status = status;
   P.lse = lse;
   P.mass = mass;
   P.decay = decay;
   P.out = out_mass;
-  P.unit_pages = P.c.page_tokens >= 64 ? 1 : 64 / P.c.page_tokens;
-  ztcp::launch_page_mass(P, cache->dtype == ZTCP_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+  const bool bf16 = cache->dtype == ZTCP_DTYPE_BF16;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!tc) {
+    P.unit_pages = P.c.page_tokens >= 64 ? 1 : 64 / P.c.page_tokens;
+    ztcp::launch_page_mass(P, bf16, s);
+  } else if (!ztcp::launch_page_mass_tc(P, P.c.group * queries->max_q_len, sms, workspace, bf16, s)) {
+    return set_last_error(ZTCP_ECUDA, "cuTensorMapEncodeTiled failed");
+  }
   return launched("page_mass_kernel");
 }
 

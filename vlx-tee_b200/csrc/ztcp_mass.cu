@@ -1,7 +1,8 @@
 // ztcp_mass.cu -- attention weight per page (ztcp_page_mass), general kernel.
 //
 // Mathematics.  out[b, p] = decay * mass[b, p] + sum over rows r, heads and tokens j of page p of
-// 2^(s_rj log2 e - lse_r log2 e): with the log-sum-exp known, weights need one product and no second pass.
+// exp(s_rj - lse_r): with the log-sum-exp known, weights need one product and no second pass.  (s - lse is formed by
+// one fma and then multiplied by log2 e, so that it is rounded once, as a small number.)
 //
 // Work.  A unit is as many whole pages as fit 64 keys (one, where a page is larger), of one sequence, all KV heads:
 // its sums never cross CTAs, so there are no atomics and results repeat bit for bit.  Units of all sequences form
@@ -60,7 +61,7 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t base, int row, int chunk, 
 template <bool BF16, int STAGES, int PER_SM>
 __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __grid_constant__ MassParams P) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_neg[STAGES][kQRows];      // -lse * log2(e) of the stage's rows, -inf where a row adds nothing
+  __shared__ float s_neg[STAGES][kQRows];      // -lse of the stage's rows, -inf where a row adds nothing
   __shared__ int32_t s_lim[STAGES][kQRows];    // keys that the row sees
   __shared__ uint8_t s_there[STAGES][kKeys];   // the key lies in a pool page
   __shared__ float s_key[2][kKeys];
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
         float neg = -INFINITY;
         if (r < rows) {
           const float x = __ldg(P.lse + (prod.s.row0 + tok) * (int64_t)(c.kv_heads * c.group) + head);
-          if (x != -INFINITY) neg = -x * 1.44269504088896f;
+          if (x != -INFINITY) neg = -x;
         }
         s_neg[stage][r] = neg;
         s_lim[stage][r] = r < rows ? visible_keys(c, prod.s, tok) : 0;
@@ -156,8 +157,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
           const int r = rg * 16 + n * 8 + 2 * t4 + e;
           const float neg = s_neg[stage][r];
           const int lim = s_lim[stage][r];
-          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale_log2, neg));
-          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale_log2, neg));
+          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale, neg) * 1.44269504088896f);
+          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale, neg) * 1.44269504088896f);
         }
     }
 

@@ -1,0 +1,470 @@
+// ztcp_mass_tc.cu -- attention weight per page (ztcp_page_mass) on the 5th-generation tensor cores.
+//
+// The mathematics is that of ztcp_mass.cu: weights exp(scale * q.k - lse) summed over rows, heads and a page's keys.
+//   S^T[128 keys, N rows] = K Q^T   (tcgen05.mma, keys on the 128 lanes)
+// puts a key's weights into one thread, which adds them up over the columns; a warp's 32 keys (or a smaller page's)
+// are then one segment, whose sum goes to the workspace per KV head.  page_mass_join_kernel adds a page's segments
+// and heads in a fixed order, so there are no atomics and results repeat bit for bit.
+//
+// Accuracy.  The exponent is formed as fma(s, scale, -lse) -- one rounding of a value that is small wherever the
+// weight is not -- and only then multiplied by log2 e: folding log2 e into the scale would round s * scale * log2 e
+// and lse * log2 e, both of tens, apart from each other.
+//
+// Work.  An item is one KV head of one sequence, a tile 128 of its keys times as many chunks of N rows as its queries
+// need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
+// Bound: for few rows the reading of K; for an observation window the exponentials, N x 128 a tile.
+//
+// Warps.  0-3 and 4-7: sums of every other step, a thread per key, no warp waiting for another; 8: products; 9: TMA
+// (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
+// ztcp_attend_tc.cu.
+#include "../../include/ztcp_kvcache.h"
+#include "ztcp_tc.cuh"
+
+namespace ztcp {
+
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kBars = 40;
+
+struct MassTcParams {
+  MassParams m;
+  PoolBoxes box;
+  // A chunk's rows, at most N: whole tokens of a group each, or (groups wider than N) a part of one token's group.
+  int32_t chunk_tokens;  // tokens of a chunk
+  int32_t parts;         // chunks that share a token: 1, or ceil(group / N)
+  int32_t part_heads;    // heads of the group in a chunk
+  int32_t seg_shift;     // log2 of the keys of a segment: 32, or a smaller page's
+  int32_t segs;          // segments of a sequence in the workspace
+};
+
+template <int KG, int N>
+struct Shape {
+  static constexpr int kGroups = KG == 1 ? 1 : 2;           // column groups of a slot
+  static constexpr int kSlotBytes = kGroups * kGroupBytes;
+  static constexpr int kTileSlots = (KG + kGroups - 1) / kGroups;
+  static constexpr int kQBytes = KG * N * 128;
+  static constexpr int kQSlots = kQBytes > 32 * 1024 ? 1 : 2;
+  static constexpr int kNegBytes = 8 * N * 4;               // every warp its copy of a chunk's -lse
+  static constexpr int kRoom = (232448 - 4096 - kQSlots * kQBytes - kNegBytes) / kSlotBytes;
+  static constexpr int kSlots = kRoom < 8 ? kRoom : 8;
+  static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kQSlots * kQBytes + kNegBytes;
+  static constexpr int kCols = 2 * N < 32 ? 32 : 2 * N;     // TMEM: S^T of two steps
+  static_assert(kSlots >= kTileSlots && 2 * kSlots + 9 + 2 * kJobs <= kBars, "shape");
+};
+
+// Tiles and chunks of a sequence.
+struct MassSeq {
+  Seq s;
+  int32_t tiles, chunks;
+  __device__ __forceinline__ int64_t cost() const { return (int64_t)tiles * chunks; }
+};
+__device__ __forceinline__ MassSeq mass_seq(const MassTcParams& P, int b) {
+  const CacheParams& c = P.m.c;
+  MassSeq m;
+  m.s = load_seq(c, b);
+  m.tiles = m.s.q_len > 0 ? (m.s.kv_len + kKeys - 1) / kKeys : 0;
+  m.chunks = (m.s.q_len + P.chunk_tokens - 1) / P.chunk_tokens * P.parts;
+  return m;
+}
+
+template <bool BF16, int KG, int N>
+__global__ void __launch_bounds__(kThreads, 1)
+page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
+  using Sh = Shape<KG, N>;
+  constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kQS = Sh::kQSlots;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int dead_s;
+  __shared__ uint32_t tmem_s;
+  __shared__ Job s_jobs[kJobs];  // row: chunks of the item; whole, inside: not used
+  const CacheParams& c = P.m.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  volatile int* const dead = &dead_s;
+  const uint32_t bars = smem_u32(smem_raw);
+  const uint32_t ring = (bars + kBars * 8 + 1023) & ~1023u;
+  const uint32_t qbuf = ring + kSlots * Sh::kSlotBytes;
+  float* const negs = reinterpret_cast<float*>(smem_raw + (qbuf - bars) + kQS * Sh::kQBytes);
+  auto full = [&](uint32_t s) { return bars + s * 8; };
+  auto empty = [&](uint32_t s) { return bars + (kSlots + s) * 8; };
+  const uint32_t q_full = bars + 2 * kSlots * 8, q_empty = q_full + 16, s_full = q_empty + 16, s_read = s_full + 16, job_full = s_read + 16,
+                 job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
+  if (tid == 0) {
+    dead_s = 0;
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + 8 * i, 1);
+      mbar_init(q_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(s_read + 8 * i, 4);
+    }
+    for (int e = 0; e < kJobs; ++e) {
+      mbar_init(job_full + 8 * e, 1);
+      mbar_init(job_empty + 8 * e, 9);
+    }
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "n"(Sh::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  cudaTriggerProgrammaticLaunchCompletion();
+
+  if (warp == kTmaWarp) {
+    // ---- TMA -------------------------------------------------------------------------------------------
+    int64_t at;
+    Spot spot;
+    const SplitSpan S = locate_warp(c.n_seqs, P.m.grid, lane, [&](int b) { return mass_seq(P, b).cost() * c.kv_heads; }, &at, &spot);
+    int64_t pos = at < 0 ? 0 : at;
+    const int64_t end = at < 0 ? 0 : S.begin(blockIdx.x + 1);
+    int64_t first = spot.first;
+    int b = spot.seq;
+    const int per_tile = kKeys / P.box.rows;
+    uint32_t kpos = 0, qpos = 0, n = 0;
+    bool ok = true;
+    auto next = [&](Job* job) {  // publishes the share's next item (none: ta == tb)
+      *job = Job{};
+      while (pos < end && job->ta == job->tb) {
+        MassSeq m = mass_seq(P, b);
+        while (pos >= first + m.cost() * c.kv_heads) {
+          first += m.cost() * c.kv_heads;
+          m = mass_seq(P, ++b);
+        }
+        const int64_t x = pos - first, h = div_pos(x, m.cost()), start = first + h * m.cost();
+        job->row0 = m.s.row0;
+        job->b = b;
+        job->kv_len = m.s.kv_len;
+        job->q_len = m.s.q_len;
+        job->row = m.chunks;
+        job->head = (int32_t)h;
+        job->ta = (int32_t)div_pos(pos - start, m.chunks);
+        pos = min(end, start + m.cost());
+        job->tb = (int32_t)div_pos(pos - start, m.chunks);
+      }
+      const uint32_t e = n % kJobs;
+      if (n >= kJobs && !warp_wait(job_empty + 8 * e, (n / kJobs - 1) & 1, dead)) return false;
+      if (lane == 0) {
+        s_jobs[e] = *job;
+        mbar_arrive(job_full + 8 * e);
+      }
+      ++n;
+      return true;
+    };
+    Job job;
+    while (ok && (ok = next(&job)) && job.ta < job.tb) {
+      auto load_q = [&](int ch) {
+        const uint32_t slot = qpos % kQS;
+        if (qpos >= kQS && !warp_wait(q_empty + 8 * slot, (qpos / kQS - 1) & 1, dead)) return false;
+        if (lane == 0) mbar_expect(q_full + 8 * slot, KG * P.chunk_tokens * P.part_heads * 128);
+        const int first_tok = ch / P.parts * P.chunk_tokens;
+        __syncwarp();
+        if (lane < KG)
+          tma_load4(qbuf + slot * Sh::kQBytes + lane * N * 128, &qmap, lane * 64, ch % P.parts * N, job.head, (int)job.row0 + first_tok,
+                    q_full + 8 * slot);
+        ++qpos;
+        return true;
+      };
+      if (job.row == 1) ok = load_q(0);
+      for (int t = job.ta; ok && t < job.tb; ++t) {
+        const int j = t * kKeys + lane * P.box.rows;
+        int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
+        if (lane < per_tile && j < job.kv_len) {
+          const int64_t r = pool_row(c, job.b, j);
+          if (r >= 0) row = (int32_t)r;
+        }
+#pragma unroll
+        for (int s = 0; s < kTS; ++s, ++kpos) {
+          const uint32_t slot = kpos % kSlots;
+          if (kpos >= kSlots && !(ok = warp_wait(empty(slot), (kpos / kSlots - 1) & 1, dead))) break;
+          const int groups = KG - s * Sh::kGroups < Sh::kGroups ? KG - s * Sh::kGroups : Sh::kGroups;
+          if (lane == 0) mbar_expect(full(slot), groups * kGroupBytes);
+          __syncwarp();
+          if (lane < per_tile)
+            for (int g = 0; g < groups; ++g)
+              tma_load(ring + slot * Sh::kSlotBytes + g * kGroupBytes + lane * P.box.rows * 128, &kmap, (s * Sh::kGroups + g) * 64, job.head, row, full(slot));
+        }
+        if (job.row > 1)
+          for (int ch = 0; ok && ch < job.row; ++ch) ok = load_q(ch);
+      }
+    }
+    if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
+      int none = 0;
+      for (uint32_t p = kpos > kSlots ? kpos - kSlots : 0; p < kpos; ++p) mbar_wait(full(p % kSlots), (p / kSlots) & 1, &none);
+      for (uint32_t p = qpos > kQS ? qpos - kQS : 0; p < qpos; ++p) mbar_wait(q_full + 8 * (p % kQS), (p / kQS) & 1, &none);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- products: one thread ---------------------------------------------------------------------------
+    if (elect_one()) {
+      constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
+      const uint32_t qk = inst_desc(BF16, 128, N, false, false);
+      const uint32_t k_lo = desc_lo(ring, 16), q_lo = desc_lo(qbuf, 16);
+      uint32_t kpos = 0, qpos = 0, step = 0, jobs = 0;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t n) {  // the n-th completion (from 0)
+        ok = ok && mbar_wait(bar, n & 1, dead);
+        return ok;
+      };
+      Job job;
+      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, jobs, dead, &job)) && job.ta < job.tb) {
+        const int chunks = job.row;
+        const int tiles = job.tb - job.ta;
+        for (int t = 0; ok && t < tiles; ++t) {
+          for (int ch = 0; ok && ch < chunks; ++ch, ++step) {
+            const bool fresh = chunks > 1 || t == 0;             // this step's Q is a new one,
+            const bool spent = chunks > 1 || t + 1 == tiles;     // and not used again
+            const uint32_t qslot = qpos % kQS, buf = step & 1;
+            if (fresh && !wait(q_full + 8 * qslot, qpos / kQS)) break;
+            if (step > 1 && !wait(s_read + 8 * buf, (step >> 1) - 1)) break;
+#pragma unroll
+            for (int s = 0; s < kTS; ++s) {
+              const uint32_t pos = kpos + s, slot = pos % kSlots;
+              if (ch == 0 && !wait(full(slot), pos / kSlots)) break;
+              tc_fence_after();
+              const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), q = q_lo + qslot * (Sh::kQBytes >> 4), d = tmem + buf * N;
+#pragma unroll
+              for (int g = 0; g < Sh::kGroups; ++g)
+                if (s * Sh::kGroups + g < KG)
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    mma_ss(d, a + ((g * kGroupBytes + k * 32) >> 4), kHi, q + (((s * Sh::kGroups + g) * N * 128 + k * 32) >> 4), kHi, qk,
+                           s * Sh::kGroups + g > 0 || k > 0);
+              if (ch + 1 == chunks) tc_commit(empty(slot));
+            }
+            if (!ok) break;
+            tc_commit(s_full + 8 * buf);
+            if (spent) {
+              tc_commit(q_empty + 8 * qslot);
+              ++qpos;
+            }
+          }
+          kpos += kTS;
+        }
+      }
+      if (*dead) {  // no product may be in flight when TMEM is freed
+        int none = 0;
+        tc_commit(drain);
+        mbar_wait(drain, 0, &none);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- sums: a thread per key -------------------------------------------------------------------------
+    const int wg = warp >> 2, key = tid & 127;
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N;
+    float* const neg = negs + warp * N;
+    const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
+    uint32_t step = 0, mine = 0, jobs = 0;
+    Job job;
+    bool ok = true;
+    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
+      const int chunks = job.row;
+      // -lse of a chunk's rows, -inf where a row adds nothing
+      auto load_neg = [&](int ch) {
+        __syncwarp();
+#pragma unroll 1
+        for (int r = lane; r < N; r += 32) {
+          const int t = r / P.part_heads, tok = ch / P.parts * P.chunk_tokens + t, g = ch % P.parts * N + r - t * P.part_heads;
+          float x = -INFINITY;
+          if (t < P.chunk_tokens && tok < job.q_len && g < c.group) {
+            x = -__ldg(P.m.lse + (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + g);
+            if (x == INFINITY) x = -INFINITY;
+          }
+          neg[r] = x;
+        }
+        __syncwarp();
+      };
+      if (chunks == 1) load_neg(0);
+      for (int t = job.ta; ok && t < job.tb; ++t) {
+        const int j = t * kKeys + key;
+        const bool there = j < job.kv_len && pool_row(c, job.b, j) >= 0;
+        float sum = 0.f;
+        bool some = false;
+        for (int ch = 0; ch < chunks; ++ch, ++step) {
+          if ((step & 1) != wg) continue;
+          some = true;
+          if (chunks > 1) load_neg(ch);
+          const int tok0 = ch / P.parts * P.chunk_tokens;
+          const int valid = P.parts == 1 ? min(P.chunk_tokens, job.q_len - tok0) * c.group : min(N, c.group - ch % P.parts * N);  // the chunk's rows
+          // token i of the chunk sees key j when j < kv_len - q_len + tok0 + i + 1: rows from `from` on
+          const int from = c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0;
+          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
+          ++mine;
+          tc_fence_after();
+          uint64_t acc0 = pair(0.f, 0.f), acc1 = acc0;
+          constexpr int kBlock = N < 32 ? N : 32;
+#pragma unroll 1
+          for (int n0 = 0; n0 < N && n0 < valid; n0 += kBlock) {
+            uint32_t x[kBlock];
+            if constexpr (N < 32) tmem_ld16(ts, x);
+            else {
+              tmem_ld32(ts + n0, x);
+              tmem_ready32(x);
+            }
+            const bool whole = __all_sync(0xffffffffu, from <= n0) && n0 + kBlock <= valid;
+#pragma unroll
+            for (int i = 0; i < kBlock; i += 4) {
+              if (N < 32 && i >= valid) break;
+              const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
+              float a, b2, d, e;
+              unpair(mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, pair(w.x, w.y)), log2e), a, b2);
+              unpair(mul2(fma2(pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, pair(w.z, w.w)), log2e), d, e);
+              a = fast_exp2(a);
+              b2 = fast_exp2(b2);
+              d = fast_exp2(d);
+              e = fast_exp2(e);
+              if (!whole) {
+                const int r = n0 + i;
+                a = r >= from && r < valid ? a : 0.f;
+                b2 = r + 1 >= from && r + 1 < valid ? b2 : 0.f;
+                d = r + 2 >= from && r + 2 < valid ? d : 0.f;
+                e = r + 3 >= from && r + 3 < valid ? e : 0.f;
+              }
+              acc0 = add2(acc0, pair(a, b2));
+              acc1 = add2(acc1, pair(d, e));
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_read + 8 * wg);
+          float s0, s1, s2, s3;
+          unpair(acc0, s0, s1);
+          unpair(acc1, s2, s3);
+          sum += (s0 + s1) + (s2 + s3);
+        }
+        if (!ok) break;
+        if (some) {  // one chunk: slot 0; more: each group's own
+          if (!there) sum = 0.f;
+          const int seg = 1 << P.seg_shift;
+          for (int d = seg >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if ((lane & (seg - 1)) == 0 && j < job.kv_len)
+            P.m.part[(((int64_t)(chunks > 1 ? wg : 0) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + (j >> P.seg_shift)] = sum;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0) P.m.errors[blockIdx.x] = *dead;
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Sh::kCols) : "memory");
+  }
+}
+
+// A page's weight: its segments' sums, head by head, in a fixed order.  A thread per page; also the status.
+__global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_constant__ MassTcParams P) {
+  const CacheParams& c = P.m.c;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int b = (int)(i / c.max_pages), p = (int)(i - (int64_t)b * c.max_pages);
+  float before = 0.f;
+  MassSeq m = {};
+  if (b < c.n_seqs) {
+    m = mass_seq(P, b);
+    if (P.m.mass && (int64_t)p * c.page_tokens < m.s.kv_len) before = P.m.mass[i];
+  }
+  cudaGridDependencySynchronize();
+  for (int s = blockIdx.x * 8 + (threadIdx.x >> 5); s < c.n_seqs; s += gridDim.x * 8) {
+    int late = 0;
+    for (int e = threadIdx.x & 31; e < P.m.grid; e += 32) late |= __ldcg(P.m.errors + e);
+    if (!__any_sync(0xffffffffu, late)) write_seq_status(c, s, threadIdx.x & 31);
+    else if (threadIdx.x % 32 == 0) c.status[s] = ZTCP_SEQ_TIMEOUT;
+  }
+  if (b >= c.n_seqs) return;
+  float sum = 0.f;
+  if ((int64_t)p * c.page_tokens < m.s.kv_len && m.chunks > 0) {
+    const int s0 = (p * c.page_tokens) >> P.seg_shift;
+    const int n = (min(c.page_tokens, m.s.kv_len - p * c.page_tokens) + (1 << P.seg_shift) - 1) >> P.seg_shift;
+    for (int slot = 0; slot < (m.chunks > 1 ? 2 : 1); ++slot)
+      for (int h = 0; h < c.kv_heads; ++h) {
+        const float* const q = P.m.part + (((int64_t)slot * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
+        for (int k = 0; k < n; ++k) sum += __ldcg(q + k);
+      }
+  }
+  P.m.out[i] = P.m.mass ? fmaf(P.m.decay, before, sum) : sum;
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+// Q as [token][KV head][head of the group][head_dim], boxes of `tokens` tokens x `heads` of a group x 64 columns.
+bool query_map(CUtensorMap* map, const CacheParams& c, bool bf16, int tokens, int heads) {
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.group, (cuuint64_t)c.kv_heads, (cuuint64_t)c.total_rows};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.q_head_stride * 2, (cuuint64_t)c.q_head_stride * 2 * c.group, (cuuint64_t)c.q_token_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)heads, 1, (cuuint32_t)tokens}, elem[4] = {1, 1, 1, 1};
+  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t*>(c.q), dims, strides,
+                        box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int KG, int N>
+void launch_kernel(const MassTcParams& P, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t s) {
+  auto* const f = page_mass_tc_kernel<BF16, KG, N>;
+  constexpr int smem = Shape<KG, N>::kSmem;
+  cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  f<<<P.m.grid, kThreads, smem, s>>>(P, k, q);
+}
+
+template <bool BF16>
+void launch_any(const MassTcParams& P, int n, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t s) {
+  const int d = P.m.c.head_dim;
+  if (d <= 64) n == 16 ? launch_kernel<BF16, 1, 16>(P, k, q, s) : n == 64 ? launch_kernel<BF16, 1, 64>(P, k, q, s) : launch_kernel<BF16, 1, 256>(P, k, q, s);
+  else if (d <= 128) n == 16 ? launch_kernel<BF16, 2, 16>(P, k, q, s) : n == 64 ? launch_kernel<BF16, 2, 64>(P, k, q, s) : launch_kernel<BF16, 2, 256>(P, k, q, s);
+  else if (d <= 256) n == 16 ? launch_kernel<BF16, 4, 16>(P, k, q, s) : launch_kernel<BF16, 4, 64>(P, k, q, s);
+  else n == 16 ? launch_kernel<BF16, 9, 16>(P, k, q, s) : launch_kernel<BF16, 9, 32>(P, k, q, s);
+}
+
+// Rows of a chunk: the smallest of 16, 64 and 256 that holds a sequence's rows; wide heads leave less room for Q.
+int chunk_rows(const CacheParams& c, int64_t rows) {
+  if (rows <= 16) return 16;
+  if (c.head_dim > 256) return 32;
+  return rows <= 64 || c.head_dim > 128 ? 64 : 256;
+}
+int seg_shift(const CacheParams& c) { return c.page_tokens >= 32 ? 5 : c.page_tokens == 16 ? 4 : 3; }
+int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_tokens >> seg_shift(c); }
+
+}  // namespace
+
+bool page_mass_tc_fits(const CacheParams& c) { return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31); }
+
+int64_t page_mass_tc_workspace(const CacheParams& c, int sms) {
+  return (sms + 3) / 4 * 16 + 2 * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+}
+
+bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s) {
+  MassTcParams P;
+  P.m = m;
+  P.m.grid = sms;
+  P.m.errors = static_cast<int32_t*>(workspace);
+  P.m.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (sms + 3) / 4 * 16);
+  P.box = pool_boxes(m.c, kKeys);
+  const int n = chunk_rows(m.c, rows);
+  P.chunk_tokens = m.c.group < n ? n / m.c.group : 1;
+  P.parts = (m.c.group + n - 1) / n;
+  P.part_heads = m.c.group < n ? m.c.group : n;
+  P.seg_shift = seg_shift(m.c);
+  P.segs = (int32_t)seg_count(m.c);
+  CUtensorMap k, q;
+  if (!pool_map(&k, m.c.k, m.c, bf16, P.box) || !query_map(&q, m.c, bf16, P.chunk_tokens, P.part_heads)) return false;
+  if (bf16) launch_any<true>(P, n, k, q, s);
+  else launch_any<false>(P, n, k, q, s);
+  if (cudaPeekAtLastError() != cudaSuccess) return true;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t pages = (int64_t)m.c.n_seqs * m.c.max_pages;
+  cfg.gridDim = dim3((unsigned)((pages + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, page_mass_join_kernel, P);
+  return true;
+}
+
+}  // namespace ztcp

@@ -31,8 +31,8 @@ SEQ_BAD_BLOCK = 6   # ZTCP_SEQ_BAD_BLOCK
 SEQ_TIMEOUT = 7     # ZTCP_SEQ_TIMEOUT: a wait inside the attention kernel did not end; the outputs are not valid
 
 # every symbol include/ztcp_kvcache.h declares
-KVCACHE_SYMBOLS = ("ztcp_attend_workspace_bytes", "ztcp_attend_pages", "ztcp_page_mass", "ztcp_append_tokens",
-                   "ztcp_select_cold_pages")
+KVCACHE_SYMBOLS = ("ztcp_attend_workspace_bytes", "ztcp_attend_pages", "ztcp_page_mass_workspace_bytes",
+                   "ztcp_page_mass", "ztcp_append_tokens", "ztcp_select_cold_pages")
 
 _FLOATS = (torch.float16, torch.bfloat16)
 
@@ -80,7 +80,9 @@ def _load() -> C.CDLL:
         lib.ztcp_attend_pages.restype = C.c_int32
         lib.ztcp_attend_pages.argtypes = [C.POINTER(_Cache), C.POINTER(_Queries), vp, vp, vp, vp, i64, vp]
         lib.ztcp_page_mass.restype = C.c_int32
-        lib.ztcp_page_mass.argtypes = [C.POINTER(_Cache), C.POINTER(_Queries), vp, vp, C.c_float, vp, vp, vp]
+        lib.ztcp_page_mass_workspace_bytes.restype = i64
+        lib.ztcp_page_mass_workspace_bytes.argtypes = [C.POINTER(_Cache), C.POINTER(_Queries)]
+        lib.ztcp_page_mass.argtypes = [C.POINTER(_Cache), C.POINTER(_Queries), vp, vp, C.c_float, vp, vp, vp, i64, vp]
         lib.ztcp_append_tokens.restype = C.c_int32
         lib.ztcp_append_tokens.argtypes = [C.POINTER(_Append), vp, vp]
         lib.ztcp_select_cold_pages.restype = C.c_int32
@@ -192,6 +194,14 @@ def _status(status, n, dev):
     return status
 
 
+def _workspace(size_of, cache, queries, dev) -> torch.Tensor:
+    with torch.cuda.device(dev):
+        size = size_of(cache, queries)
+    if size < 0:
+        capi.check(capi.ZTCP_EINVAL)
+    return torch.empty(size, dtype=torch.uint8, device=dev)
+
+
 def _run_once(call: PreparedCall, stream):
     """Enqueues a call whose own buffers die with it: memory that a stream other than the current one still uses is
     handed back only when that stream is done with it."""
@@ -238,12 +248,8 @@ def prepare_attend(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor |
                     [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables),
                      ("kv_lens", kv_lens), ("q_starts", q_starts)])
     lib = _load()
-    with torch.cuda.device(dev):
-        size = lib.ztcp_attend_workspace_bytes(cache, queries)
-    if size < 0:
-        capi.check(capi.ZTCP_EINVAL)
-    workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-    args = (cache, queries, out.data_ptr(), _ptr(lse), status.data_ptr(), workspace.data_ptr(), size)
+    workspace = _workspace(lib.ztcp_attend_workspace_bytes, cache, queries, dev)
+    args = (cache, queries, out.data_ptr(), _ptr(lse), status.data_ptr(), workspace.data_ptr(), workspace.numel())
     return PreparedCall(lib.ztcp_attend_pages, args, dev, (*keep, out, lse, workspace, status), status)
 
 
@@ -265,7 +271,8 @@ def prepare_page_mass(q: torch.Tensor, k_pool: torch.Tensor, block_tables: torch
     sees, of exp(scale * q.k - lse); 0 past the last page.  mass and out_mass are [sequences, pages] fp32 like
     block_tables and may be one tensor; ``mass=None`` starts from nothing.  q, lse and the other arguments as
     ``prepare_attend`` takes and writes them; q may be the last rows of a chunk (an observation window) with their
-    lse.  Calling the result enqueues the kernel and returns status[n] int32."""
+    lse.  Calling the result enqueues the kernels and returns status[n] int32.  The prepared call owns its workspace, as
+    ``prepare_attend``'s does."""
     dev, cache, queries, keep = _pack_cache(q, k_pool, None, block_tables, kv_lens, q_starts, max_q_len, 0, scale,
                                             causal, check_block_table)
     _require_cuda("lse", lse, (torch.float32,), dev)
@@ -282,8 +289,10 @@ def prepare_page_mass(q: torch.Tensor, k_pool: torch.Tensor, block_tables: torch
                     [("q", q), ("k_pool", k_pool), ("block_tables", block_tables), ("kv_lens", kv_lens),
                      ("q_starts", q_starts), ("lse", lse), ("mass", None if same else mass)])
     lib = _load()
-    args = (cache, queries, lse.data_ptr(), _ptr(mass), float(decay), out_mass.data_ptr(), status.data_ptr())
-    return PreparedCall(lib.ztcp_page_mass, args, dev, (*keep, lse, mass, out_mass, status), status)
+    workspace = _workspace(lib.ztcp_page_mass_workspace_bytes, cache, queries, dev)
+    args = (cache, queries, lse.data_ptr(), _ptr(mass), float(decay), out_mass.data_ptr(), status.data_ptr(),
+            workspace.data_ptr(), workspace.numel())
+    return PreparedCall(lib.ztcp_page_mass, args, dev, (*keep, lse, mass, out_mass, workspace, status), status)
 
 
 def page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, *, stream=None, **kw) -> torch.Tensor:
