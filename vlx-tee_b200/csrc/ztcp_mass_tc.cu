@@ -14,8 +14,8 @@
 // need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
 // Bound: for few rows the reading of K; for an observation window the exponentials, N x 128 a tile.
 //
-// Warps.  0-3 and 4-7: sums of every other step, a thread per key, no warp waiting for another; 8: products; 9: TMA
-// (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
+// Warps.  Groups of four: sums of every other step, a thread per key, no warp waiting for another; then one for the
+// products and one for TMA (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
 // ztcp_attend_tc.cu.
 #include "../../include/ztcp_kvcache.h"
 #include "ztcp_tc.cuh"
@@ -24,9 +24,8 @@ namespace ztcp {
 
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kBars = 40;
+constexpr int kSlotSums = 4;  // sums of a segment in the workspace: by step parity and half of the columns
 
 struct MassTcParams {
   MassParams m;
@@ -37,16 +36,22 @@ struct MassTcParams {
   int32_t part_heads;    // heads of the group in a chunk
   int32_t seg_shift;     // log2 of the keys of a segment: 32, or a smaller page's
   int32_t segs;          // segments of a sequence in the workspace
+  int32_t halves;        // groups that share a step's columns
 };
 
 template <int KG, int N>
 struct Shape {
+  // Warps of the sums: two groups of four by turns; for 256 rows, where their arithmetic is the limit, as many again,
+  // each with half of the columns (measured: see the top).
+  static constexpr int kHalves = N == 256 ? 2 : 1;
+  static constexpr int kSumWarps = 8 * kHalves;
+  static constexpr int kThreads = (kSumWarps + 2) * 32;
   static constexpr int kGroups = KG == 1 ? 1 : 2;           // column groups of a slot
   static constexpr int kSlotBytes = kGroups * kGroupBytes;
   static constexpr int kTileSlots = (KG + kGroups - 1) / kGroups;
   static constexpr int kQBytes = KG * N * 128;
   static constexpr int kQSlots = kQBytes > 32 * 1024 ? 1 : 2;
-  static constexpr int kNegBytes = 8 * N * 4;               // every warp its copy of a chunk's -lse
+  static constexpr int kNegBytes = 8 * N * 4;               // every warp its copy of its columns' -lse
   static constexpr int kRoom = (232448 - 4096 - kQSlots * kQBytes - kNegBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 8 ? kRoom : 8;
   static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kQSlots * kQBytes + kNegBytes;
@@ -70,10 +75,10 @@ __device__ __forceinline__ MassSeq mass_seq(const MassTcParams& P, int b) {
 }
 
 template <bool BF16, int KG, int N>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__((Shape<KG, N>::kThreads), 1)
 page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
   using Sh = Shape<KG, N>;
-  constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kQS = Sh::kQSlots;
+  constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kQS = Sh::kQSlots, kMmaWarp = Sh::kSumWarps, kTmaWarp = kMmaWarp + 1;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
@@ -99,11 +104,11 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
       mbar_init(q_full + 8 * i, 1);
       mbar_init(q_empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(s_read + 8 * i, 4);
+      mbar_init(s_read + 8 * i, Sh::kSumWarps / 2);
     }
     for (int e = 0; e < kJobs; ++e) {
       mbar_init(job_full + 8 * e, 1);
-      mbar_init(job_empty + 8 * e, 9);
+      mbar_init(job_empty + 8 * e, Sh::kSumWarps + 1);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -257,29 +262,34 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     __syncwarp();
   } else {
     // ---- sums: a thread per key -------------------------------------------------------------------------
-    const int wg = warp >> 2, key = tid & 127;
-    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N;
-    float* const neg = negs + warp * N;
+    constexpr int kOwn = N / Sh::kHalves;  // columns of a group
+    const int wg = (warp >> 2) & 1, half = warp >> 3, key = tid & 127;
+    const int col0 = half * kOwn;
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N + col0;
+    float* const neg = negs + warp * kOwn;
     const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
     uint32_t step = 0, mine = 0, jobs = 0;
     Job job;
     bool ok = true;
     while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
       const int chunks = job.row;
+      bool none = false;  // a row of the chunk adds nothing
       // -lse of a chunk's rows, -inf where a row adds nothing
       auto load_neg = [&](int ch) {
         __syncwarp();
+        bool inf = false;
 #pragma unroll 1
-        for (int r = lane; r < N; r += 32) {
-          const int t = r / P.part_heads, tok = ch / P.parts * P.chunk_tokens + t, g = ch % P.parts * N + r - t * P.part_heads;
+        for (int i = lane; i < kOwn; i += 32) {
+          const int r = col0 + i, t = r / P.part_heads, tok = ch / P.parts * P.chunk_tokens + t, g = ch % P.parts * N + r - t * P.part_heads;
           float x = -INFINITY;
           if (t < P.chunk_tokens && tok < job.q_len && g < c.group) {
             x = -__ldg(P.m.lse + (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + g);
             if (x == INFINITY) x = -INFINITY;
+            inf = inf || x == -INFINITY;
           }
-          neg[r] = x;
+          neg[i] = x;
         }
-        __syncwarp();
+        none = __any_sync(0xffffffffu, inf);
       };
       if (chunks == 1) load_neg(0);
       for (int t = job.ta; ok && t < job.tb; ++t) {
@@ -293,25 +303,37 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           if (chunks > 1) load_neg(ch);
           const int tok0 = ch / P.parts * P.chunk_tokens;
           const int valid = P.parts == 1 ? min(P.chunk_tokens, job.q_len - tok0) * c.group : min(N, c.group - ch % P.parts * N);  // the chunk's rows
+          const int mine_valid = valid - col0;  // of them, in this group's columns: those below this
           // token i of the chunk sees key j when j < kv_len - q_len + tok0 + i + 1: rows from `from` on
-          const int from = c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0;
+          const int from = (c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0) - col0;
           if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
           ++mine;
           tc_fence_after();
           uint64_t acc0 = pair(0.f, 0.f), acc1 = acc0;
           constexpr int kBlock = N < 32 ? N : 32;
-#pragma unroll 1
-          for (int n0 = 0; n0 < N && n0 < valid; n0 += kBlock) {
-            uint32_t x[kBlock];
-            if constexpr (N < 32) tmem_ld16(ts, x);
-            else {
-              tmem_ld32(ts + n0, x);
-              tmem_ready32(x);
+          // columns [n0, n0 + kBlock); of eight pairs, three exponentials go to the FMA pipes (measured: see the top)
+          auto add_block = [&](const uint32_t* x, int n0) {
+            if (n0 >= mine_valid) return;
+            const bool whole = !none && n0 + kBlock <= mine_valid && __all_sync(0xffffffffu, from <= n0);
+            if (whole && N >= 64) {
+#pragma unroll
+              for (int i = 0; i < kBlock; i += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
+                uint64_t u = mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, pair(w.x, w.y)), log2e);
+                uint64_t v = mul2(fma2(pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, pair(w.z, w.w)), log2e);
+                float a, b2;
+                if (i % 16 == 4) u = exp2_poly(u);
+                else unpair(u, a, b2), u = pair(fast_exp2(a), fast_exp2(b2));
+                if (i % 8 == 0) v = exp2_poly(v);
+                else unpair(v, a, b2), v = pair(fast_exp2(a), fast_exp2(b2));
+                acc0 = add2(acc0, u);
+                acc1 = add2(acc1, v);
+              }
+              return;
             }
-            const bool whole = __all_sync(0xffffffffu, from <= n0) && n0 + kBlock <= valid;
 #pragma unroll
             for (int i = 0; i < kBlock; i += 4) {
-              if (N < 32 && i >= valid) break;
+              if (N < 32 && i >= mine_valid) break;
               const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
               float a, b2, d, e;
               unpair(mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, pair(w.x, w.y)), log2e), a, b2);
@@ -322,30 +344,68 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
               e = fast_exp2(e);
               if (!whole) {
                 const int r = n0 + i;
-                a = r >= from && r < valid ? a : 0.f;
-                b2 = r + 1 >= from && r + 1 < valid ? b2 : 0.f;
-                d = r + 2 >= from && r + 2 < valid ? d : 0.f;
-                e = r + 3 >= from && r + 3 < valid ? e : 0.f;
+                a = r >= from && r < mine_valid ? a : 0.f;
+                b2 = r + 1 >= from && r + 1 < mine_valid ? b2 : 0.f;
+                d = r + 2 >= from && r + 2 < mine_valid ? d : 0.f;
+                e = r + 3 >= from && r + 3 < mine_valid ? e : 0.f;
               }
               acc0 = add2(acc0, pair(a, b2));
               acc1 = add2(acc1, pair(d, e));
             }
+          };
+          auto release = [&] {  // S^T has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read + 8 * wg);
+          };
+          if constexpr (N < 64) {
+            uint32_t x[kBlock];
+            if constexpr (N == 16) tmem_ld16(ts, x);
+            else {
+              tmem_ld32(ts, x);
+              tmem_ready32(x);
+            }
+            release();
+            add_block(x, 0);
+          } else if constexpr (Sh::kHalves == 2) {
+#pragma unroll 1
+            for (int n0 = 0; n0 < kOwn; n0 += 32) {
+              uint32_t x[32];
+              tmem_ld32(ts + n0, x);
+              tmem_ready32(x);
+              const bool more = n0 + 32 < kOwn && n0 + 32 < mine_valid;
+              if (!more) release();
+              add_block(x, n0);
+              if (!more) break;
+            }
+          } else {  // one block's loads under the other's arithmetic
+            uint32_t x[32], y[32];
+            tmem_ld32(ts, x);
+#pragma unroll 1
+            for (int n0 = 0; n0 < kOwn; n0 += 64) {
+              tmem_ready32(x);
+              tmem_ld32(ts + n0 + 32, y);
+              add_block(x, n0);
+              tmem_ready32(y);
+              const bool more = n0 + 64 < kOwn && n0 + 64 < mine_valid;
+              if (more) tmem_ld32(ts + n0 + 64, x);
+              else release();
+              add_block(y, n0 + 32);
+              if (!more) break;
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_read + 8 * wg);
           float s0, s1, s2, s3;
           unpair(acc0, s0, s1);
           unpair(acc1, s2, s3);
           sum += (s0 + s1) + (s2 + s3);
         }
         if (!ok) break;
-        if (some) {  // one chunk: slot 0; more: each group's own
+        if (some) {
           if (!there) sum = 0.f;
           const int seg = 1 << P.seg_shift;
           for (int d = seg >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
           if ((lane & (seg - 1)) == 0 && j < job.kv_len)
-            P.m.part[(((int64_t)(chunks > 1 ? wg : 0) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + (j >> P.seg_shift)] = sum;
+            P.m.part[(((int64_t)(chunks > 1 ? 2 * wg + half : half) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + (j >> P.seg_shift)] = sum;
         }
       }
     }
@@ -358,16 +418,25 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   }
 }
 
-// A page's weight: its segments' sums, head by head, in a fixed order.  A thread per page; also the status.
+// A page's weight: its segments' sums, head by head, in a fixed order.  Eight threads per page, each with every eighth
+// head, then a tree; also the status.
 __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_constant__ MassTcParams P) {
   const CacheParams& c = P.m.c;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int sub = threadIdx.x & 7;
   const int b = (int)(i / c.max_pages), p = (int)(i - (int64_t)b * c.max_pages);
   float before = 0.f;
-  MassSeq m = {};
+  int n = 0, slots = 0;
   if (b < c.n_seqs) {
-    m = mass_seq(P, b);
-    if (P.m.mass && (int64_t)p * c.page_tokens < m.s.kv_len) before = P.m.mass[i];
+    const MassSeq m = mass_seq(P, b);
+    const int64_t left = m.s.kv_len - (int64_t)p * c.page_tokens;
+    if (left > 0) {
+      if (P.m.mass) before = P.m.mass[i];
+      if (m.chunks > 0) {
+        n = (int)((min((int64_t)c.page_tokens, left) + (1 << P.seg_shift) - 1) >> P.seg_shift);
+        slots = m.chunks > 1 ? 2 : 1;
+      }
+    }
   }
   cudaGridDependencySynchronize();
   for (int s = blockIdx.x * 8 + (threadIdx.x >> 5); s < c.n_seqs; s += gridDim.x * 8) {
@@ -376,18 +445,18 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
     if (!__any_sync(0xffffffffu, late)) write_seq_status(c, s, threadIdx.x & 31);
     else if (threadIdx.x % 32 == 0) c.status[s] = ZTCP_SEQ_TIMEOUT;
   }
-  if (b >= c.n_seqs) return;
   float sum = 0.f;
-  if ((int64_t)p * c.page_tokens < m.s.kv_len && m.chunks > 0) {
-    const int s0 = (p * c.page_tokens) >> P.seg_shift;
-    const int n = (min(c.page_tokens, m.s.kv_len - p * c.page_tokens) + (1 << P.seg_shift) - 1) >> P.seg_shift;
-    for (int slot = 0; slot < (m.chunks > 1 ? 2 : 1); ++slot)
-      for (int h = 0; h < c.kv_heads; ++h) {
-        const float* const q = P.m.part + (((int64_t)slot * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
+  const int64_t s0 = (int64_t)p * c.page_tokens >> P.seg_shift;
+  for (int slot = 0; slot < slots; ++slot)
+    for (int half = 0; half < P.halves; ++half)
+      for (int h = sub; h < c.kv_heads; h += 8) {
+        const float* const q = P.m.part + (((int64_t)(2 * slot + half) * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
+#pragma unroll 2
         for (int k = 0; k < n; ++k) sum += __ldcg(q + k);
       }
-  }
-  P.m.out[i] = P.m.mass ? fmaf(P.m.decay, before, sum) : sum;
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (b < c.n_seqs && sub == 0) P.m.out[i] = P.m.mass ? fmaf(P.m.decay, before, sum) : sum;
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -406,7 +475,7 @@ void launch_kernel(const MassTcParams& P, const CUtensorMap& k, const CUtensorMa
   auto* const f = page_mass_tc_kernel<BF16, KG, N>;
   constexpr int smem = Shape<KG, N>::kSmem;
   cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  f<<<P.m.grid, kThreads, smem, s>>>(P, k, q);
+  f<<<P.m.grid, Shape<KG, N>::kThreads, smem, s>>>(P, k, q);
 }
 
 template <bool BF16>
@@ -432,7 +501,7 @@ int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_t
 bool page_mass_tc_fits(const CacheParams& c) { return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31); }
 
 int64_t page_mass_tc_workspace(const CacheParams& c, int sms) {
-  return (sms + 3) / 4 * 16 + 2 * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+  return (sms + 3) / 4 * 16 + kSlotSums * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
 }
 
 bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s) {
@@ -448,6 +517,7 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   P.part_heads = m.c.group < n ? m.c.group : n;
   P.seg_shift = seg_shift(m.c);
   P.segs = (int32_t)seg_count(m.c);
+  P.halves = n == 256 ? 2 : 1;
   CUtensorMap k, q;
   if (!pool_map(&k, m.c.k, m.c, bf16, P.box) || !query_map(&q, m.c, bf16, P.chunk_tokens, P.part_heads)) return false;
   if (bf16) launch_any<true>(P, n, k, q, s);
@@ -455,7 +525,7 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   if (cudaPeekAtLastError() != cudaSuccess) return true;
   cudaLaunchConfig_t cfg = {};
   const int64_t pages = (int64_t)m.c.n_seqs * m.c.max_pages;
-  cfg.gridDim = dim3((unsigned)((pages + 255) / 256));
+  cfg.gridDim = dim3((unsigned)((pages + 31) / 32));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
