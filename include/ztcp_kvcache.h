@@ -107,8 +107,8 @@ typedef struct ztcp_append {
   void *k_pool, *v_pool;
   const int64_t* slots;       /* [n_tokens] */
   const int32_t* positions;   /* [n_tokens] */
-  const float* rope_table;    /* [max_pos, rope_dim]; NULL when rope_dim is 0 */
-  const float *q_weight, *k_weight; /* [head_dim - norm_from] fp32, or NULL: no norm */
+  const float* rope_table;    /* [max_pos, rope_dim], 16-byte aligned; NULL when rope_dim is 0 */
+  const float *q_weight, *k_weight; /* [head_dim - norm_from] fp32, 16-byte aligned, or NULL: no norm */
   int64_t n_tokens, num_q_heads, pool_pages, max_pos;
   ztcp_geometry geom;
   int32_t dtype, norm_from, interleaved;

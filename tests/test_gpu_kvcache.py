@@ -340,6 +340,13 @@ def test_mass_sums_to_the_rows():
     (4, 2, 1, 1024, 256, True, 0, True, False),
     (3, 5, 1, 80, 0, False, 16, True, False),
     (2, 1, 1, 16, 16, False, 0, True, True),
+    (1001, 32, 8, 128, 128, False, 0, True, False),
+    (1200, 32, 7, 128, 64, True, 0, True, False),
+    (7001, 8, 2, 64, 32, False, 0, True, False),
+    (701, 16, 1, 576, 64, True, 64, True, True),
+    (2100, 7, 2, 256, 128, False, 0, True, False),
+    (9001, 3, 1, 48, 0, False, 16, True, False),
+    (600, 20, 2, 1024, 256, False, 0, True, False),
 ])
 def test_append(dtype, n, Hq, H, D, R, interleaved, norm_from, weights, mla):
     from ztcp_b200 import kvcache

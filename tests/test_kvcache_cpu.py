@@ -114,6 +114,8 @@ def test_mass_refusals(lib):
     (dict(slots=None), "slots must not be NULL"),
     (dict(rope_table=None), "a rotation needs positions and a rope table"),
     (dict(positions=None), "a rotation needs positions and a rope table"),
+    (dict(q_weight=FAKE + 4), "rope_table, q_weight and k_weight must be 16-byte aligned"),
+    (dict(rope_table=FAKE + 8), "rope_table, q_weight and k_weight must be 16-byte aligned"),
     (dict(norm_from=8), "norm_from must be a multiple of 16 below head_dim"),
     (dict(norm_from=128), "norm_from must be a multiple of 16 below head_dim"),
     (dict(eps=-1.0), "eps must be non-negative and finite"),

@@ -229,9 +229,13 @@ int32_t ztcp_append_tokens(const ztcp_append* a, int32_t* status, void* stream) 
   if ((a->q && bad_rows(a->q, a->q_token_stride, a->q_head_stride)) || bad_rows(a->k, a->k_token_stride, a->k_head_stride) ||
       (a->v && bad_rows(a->v, a->v_token_stride, a->v_head_stride)) || (a->q && !aligned(a->q_out, 16)))
     return invalid("q, k, v and q_out must be 16-byte aligned with strides of multiples of 8 elements");
+  for (int64_t st : {a->q_head_stride, a->k_head_stride, a->v_head_stride})
+    if (st > kInt32Max || st < 0) return invalid("head strides must be non-negative and below 2^31 elements");
   if (!a->slots) return invalid("slots must not be NULL");
   if (g.rope_dim > 0 && (!a->positions || !a->rope_table || a->max_pos <= 0))
     return invalid("a rotation needs positions and a rope table");
+  if (!aligned(a->rope_table, 16) || !aligned(a->q_weight, 16) || !aligned(a->k_weight, 16))
+    return invalid("rope_table, q_weight and k_weight must be 16-byte aligned");
   if (a->norm_from < 0 || a->norm_from >= g.head_dim || a->norm_from % 16 != 0)
     return invalid("norm_from must be a multiple of 16 below head_dim");
   if (!(a->eps >= 0.f) || isinf(a->eps)) return invalid("eps must be non-negative and finite");

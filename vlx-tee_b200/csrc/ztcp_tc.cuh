@@ -136,28 +136,7 @@ __device__ __forceinline__ uint32_t inst_desc(bool bf16, int m, int n, bool a_mn
   return 1u << 4 | t << 7 | t << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
-// ---- arithmetic on pairs of fp32 -------------------------------------------------------------------
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+// ---- 2^t -----------------------------------------------------------------------------------------------
 // 2^t of a pair on the FMA pipes, for finite t: 2^n by the exponent bits, n = round(t), and 2^f for |f| <= 1/2 by the
 // polynomial of degree 5 with the least relative error there (fitted for this; 7.5e-8, and 2.2e-7 with its fp32
 // evaluation, against 2.4e-7 of ex2.approx).  Below 2^-126 it stays there.  The special-function unit gives 16
