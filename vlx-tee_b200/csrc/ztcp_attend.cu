@@ -353,10 +353,21 @@ __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __gri
   const int64_t mo = (int64_t)P.part_rows * c.v_dim, lo = mo + P.part_rows;
   auto part = [&](int i) { return P.part + (int64_t)(2 * (x + i) + (i == 0 ? 1 : 0)) * P.part_floats; };
   const int quads = c.v_dim / 4;
-  for (int base = blockIdx.y * kMergeQuads; base < rows * quads; base += gridDim.y * kMergeQuads) {
+  const int count = (P.tiled ? (rows + 7) / 8 * 8 : rows) * quads;
+  for (int base = blockIdx.y * kMergeQuads; base < count; base += gridDim.y * kMergeQuads) {
+    // rows by quads; tiled partials are read as 8 rows by 4 quads a warp, whole sectors on both sides
     const int i = base + quad;
-    const bool live = i < rows * quads;
-    const int r = live ? i / quads : 0, col = live ? (i - r * quads) * 4 : 0;
+    int r, col;
+    if (P.tiled) {
+      const int blk = i >> 5, across = quads >> 2;
+      r = blk / across * 8 + (i & 7);
+      col = (blk % across * 4 + (i >> 3 & 3)) * 4;
+    } else {
+      r = i / quads;
+      col = (i - r * quads) * 4;
+    }
+    const bool live = r < rows;
+    if (!live) r = 0;
     float m = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = grp; k0 < n; k0 += 16) {  // four partials in flight
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __gri
           const float* const p = part(k);
           pm[u] = __ldcg(p + mo + r);
           pl[u] = __ldcg(p + lo + r);
-          po[u] = __ldcg(reinterpret_cast<const float4*>(p + (int64_t)r * c.v_dim + col));
+          po[u] = __ldcg(reinterpret_cast<const float4*>(p + (P.tiled ? (int64_t)(col / 4 * P.part_rows + r) * 4 : (int64_t)r * c.v_dim + col)));
         }
       }
 #pragma unroll
@@ -448,7 +459,7 @@ void launch_kernel(const AttendParams& P, const Variant& v, cudaStream_t s) {
 
 }  // namespace
 
-AttendShape attend_shape(const CacheParams& c, int sms) { return {sms * pick(c).per_sm, kRows, kRows * (c.v_dim + 2)}; }
+AttendShape attend_shape(const CacheParams& c, int sms) { return {sms * pick(c).per_sm, kRows, kRows * (c.v_dim + 2), 0}; }
 
 void launch_attend(const AttendParams& P, bool bf16, cudaStream_t s) {
   const Variant v = pick(P.c);

@@ -165,9 +165,9 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     uint32_t pos = 0;
     int64_t at;
     Spot spot;
-    const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work<N>(c, b); }, &at, &spot);
-    Publisher<N, kTileKeys> pub;
-    pub.walk.begin(c, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
+    const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work(c, N, b); }, &at, &spot);
+    Publisher<kTileKeys> pub;
+    pub.walk.begin(c, N, 0, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
     pub.cut = Cut{};
     pub.n = 0;
     Job job;
@@ -533,7 +533,7 @@ bool attend_decode_fits(const CacheParams& c) { return (c.v ? c.head_dim <= 256 
 // half as often.
 AttendShape attend_decode_shape(const CacheParams& c, int sms, int64_t rows) {
   const int n = !c.v && rows > 16 ? 32 : 16;
-  return {sms, n, n * (c.v_dim + 2)};
+  return {sms, n, n * (c.v_dim + 2), 0};
 }
 
 bool launch_attend_decode(const AttendParams& A, bool bf16, cudaStream_t s) {

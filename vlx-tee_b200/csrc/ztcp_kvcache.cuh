@@ -51,12 +51,13 @@ struct AttendParams {
   Cut* cuts;       // one per CTA
   float* part;     // two per CTA, part_floats each: o [part_rows][v_dim], m [part_rows], l [part_rows]
   int32_t part_rows, part_floats;
+  int32_t tiled;   // o lies as [v_dim / 4][part_rows][4]
   int32_t grid;    // CTAs that share the work
 };
 
 // Grid and partials of a kernel.
 struct AttendShape {
-  int32_t grid, part_rows, part_floats;
+  int32_t grid, part_rows, part_floats, tiled;
 };
 
 struct MassParams {

@@ -128,6 +128,7 @@ int64_t plan(Kernel k, const ztcp::CacheParams& c, const ztcp_queries* q, void* 
   P->grid = s.grid;
   P->part_rows = s.part_rows;
   P->part_floats = s.part_floats;
+  P->tiled = s.tiled;
   P->cuts = static_cast<ztcp::Cut*>(base);
   P->part = reinterpret_cast<float*>(P->cuts + s.grid);
   return s.grid * ((int64_t)sizeof(ztcp::Cut) + 2 * (int64_t)s.part_floats * (int64_t)sizeof(float));

@@ -460,16 +460,6 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-// Q as [token][KV head][head of the group][head_dim], boxes of `tokens` tokens x `heads` of a group x 64 columns.
-bool query_map(CUtensorMap* map, const CacheParams& c, bool bf16, int tokens, int heads) {
-  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.group, (cuuint64_t)c.kv_heads, (cuuint64_t)c.total_rows};
-  const cuuint64_t strides[3] = {(cuuint64_t)c.q_head_stride * 2, (cuuint64_t)c.q_head_stride * 2 * c.group, (cuuint64_t)c.q_token_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)heads, 1, (cuuint32_t)tokens}, elem[4] = {1, 1, 1, 1};
-  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t*>(c.q), dims, strides,
-                        box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool BF16, int KG, int N>
 void launch_kernel(const MassTcParams& P, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t s) {
   auto* const f = page_mass_tc_kernel<BF16, KG, N>;

@@ -159,49 +159,45 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t t) {
 }
 
 // ---- the line of items ----------------------------------------------------------------------------
-// Items of up to ROWS (token, head-of-the-group) rows of one sequence and KV head form one line, sequence by
+// Items of up to `rows` (token, head-of-the-group) rows of one sequence and KV head form one line, sequence by
 // sequence, row tile by row tile, head by head, that the CTAs share evenly, in units of keys x group: an item's
 // length is what its last row sees plus its own rows, which sums over row tiles in closed form.  Shares are rounded
 // to tiles of KEYS keys.
-template <int ROWS>
 struct Line {
   int64_t head;  // units of row tile 0's items, without the rows' share
   int64_t step;  // what each further row tile adds
-  int32_t row_tiles, heads;
-  __device__ __forceinline__ int64_t cost(int rt) const { return head + (rt + 1) * step + ROWS; }
+  int32_t row_tiles, heads, rows;
+  __device__ __forceinline__ int64_t cost(int rt) const { return head + (rt + 1) * step + rows; }
   __device__ __forceinline__ int64_t before(int rt) const {  // units of one head's row tiles [0, rt)
-    return rt * (head + ROWS) + step * ((int64_t)rt * (rt + 1) / 2);
+    return rt * (head + rows) + step * ((int64_t)rt * (rt + 1) / 2);
   }
   __device__ __forceinline__ int64_t total() const { return before(row_tiles) * heads; }
 };
-template <int ROWS>
-__device__ __forceinline__ Line<ROWS> line_of(const CacheParams& c, const Seq& s) {
-  Line<ROWS> l;
-  l.row_tiles = (int)(((int64_t)s.q_len * c.group + ROWS - 1) / ROWS);
+__device__ __forceinline__ Line line_of(const CacheParams& c, int rows, const Seq& s) {
+  Line l;
+  l.rows = rows;
+  l.row_tiles = (int)div_pos((int64_t)s.q_len * c.group + rows - 1, rows);
   l.heads = c.kv_heads;
   const int64_t seen = c.causal ? (s.kv_len > s.q_len ? s.kv_len - s.q_len : 0) : s.kv_len;
   l.head = seen * c.group;
-  l.step = c.causal ? ROWS : 0;
+  l.step = c.causal ? rows : 0;
   return l;
 }
-template <int ROWS>
-__device__ __forceinline__ int64_t seq_work(const CacheParams& c, int b) {
-  return line_of<ROWS>(c, load_seq(c, b)).total();
-}
+__device__ __forceinline__ int64_t seq_work(const CacheParams& c, int rows, int b) { return line_of(c, rows, load_seq(c, b)).total(); }
 
 // An item and the tiles [ta, tb) of its `nt` that a share [pos, end) of the line covers.
-template <int ROWS, int KEYS>
+template <int KEYS>
 struct Item {
   Seq s;
-  Line<ROWS> line;
+  Line line;
   int64_t seq_start, start, cost;
-  int32_t b, rt, h, nt, ta, tb, rows, row;
+  int32_t b, rt, h, nt, ta, tb, rows, row, snap;
   bool inside;  // the share begins inside the item
-  __device__ __forceinline__ void load_seq_at(const CacheParams& c, int seq, int64_t first) {
+  __device__ __forceinline__ void load_seq_at(const CacheParams& c, int rows_max, int seq, int64_t first) {
     b = seq;
     seq_start = first;
     s = load_seq(c, seq);
-    line = line_of<ROWS>(c, s);
+    line = line_of(c, rows_max, s);
   }
   __device__ __forceinline__ void find(const CacheParams& c, int64_t pos) {  // pos lies in sequence b
     const int64_t x = pos - seq_start;
@@ -215,15 +211,16 @@ struct Item {
     cost = line.cost(rt);
     h = (int)div_pos(x - line.before(rt) * line.heads, cost);
     start = seq_start + line.before(rt) * line.heads + h * cost;
-    row = rt * ROWS;
-    rows = min(s.q_len * c.group - row, ROWS);
+    row = rt * line.rows;
+    rows = min(s.q_len * c.group - row, line.rows);
     const int vis = visible_keys(c, s, (row + rows - 1) / c.group);
     nt = vis > 0 ? (vis + KEYS - 1) / KEYS : 1;
   }
-  // The first tile of a share that begins at pos: whole tiles of keys x group before it, rounded down.
+  // The first tile of a share that begins at pos: whole tiles of keys x group before it, rounded down -- and a cut
+  // that would leave fewer than `snap` tiles on a side moves to the item's end (joining a part costs as much).
   __device__ __forceinline__ int tile_at(const CacheParams& c, int64_t pos) const {
     const int64_t t = div_pos(pos - start, (int64_t)c.group * KEYS);
-    return t < nt ? (int)t : nt;
+    return t < snap ? 0 : t > nt - snap ? nt : (int)t;
   }
   __device__ __forceinline__ void clip(const CacheParams& c, int64_t pos, int64_t end) {
     inside = pos > start;
@@ -233,21 +230,22 @@ struct Item {
 };
 
 // Walks the items of a share; every role of the CTA walks the same ones.
-template <int ROWS, int KEYS>
+template <int KEYS>
 struct Walk {
-  Item<ROWS, KEYS> it;
+  Item<KEYS> it;
   int64_t pos, end;
-  __device__ __forceinline__ void begin(const CacheParams& c, const Spot& spot, int64_t p, int64_t e) {
+  __device__ __forceinline__ void begin(const CacheParams& c, int rows, int snap, const Spot& spot, int64_t p, int64_t e) {
     pos = p;
     end = e;
-    it.load_seq_at(c, spot.seq, spot.first);
+    it.load_seq_at(c, rows, spot.seq, spot.first);
     it.start = it.cost = 0;  // no item yet
     it.rt = it.h = it.nt = it.ta = it.tb = it.rows = it.row = 0;
     it.inside = false;
+    it.snap = snap;
   }
   __device__ __forceinline__ bool next(const CacheParams& c) {  // the next item with tiles, in `it`
     while (pos < end) {
-      while (pos >= it.seq_start + it.line.total()) it.load_seq_at(c, it.b + 1, it.seq_start + it.line.total());
+      while (pos >= it.seq_start + it.line.total()) it.load_seq_at(c, it.line.rows, it.b + 1, it.seq_start + it.line.total());
       it.find(c, pos);
       it.clip(c, pos, end);
       pos = min(end, it.start + it.cost);
@@ -310,15 +308,15 @@ struct Job {
 };
 constexpr int kJobs = 4;
 
-template <int ROWS, int KEYS>
+template <int KEYS>
 struct Publisher {
-  Walk<ROWS, KEYS> walk;
+  Walk<KEYS> walk;
   Cut cut;
   uint32_t n;  // published so far
   // Publishes the next item (lane 0 of the warp writes) and keeps it in `job`; false after a timeout.
   __device__ __forceinline__ bool next(const CacheParams& c, const SplitSpan& S, Job* jobs, uint32_t full, uint32_t empty, int lane, volatile int* dead,
                                        Job* job) {
-    Item<ROWS, KEYS>& it = walk.it;
+    Item<KEYS>& it = walk.it;
     const int64_t begin = S.begin(blockIdx.x);
     const bool have = walk.next(c);
     job->row0 = it.s.row0;
@@ -399,6 +397,16 @@ inline bool pool_map(CUtensorMap* map, const void* pool, const CacheParams& c, b
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+
+// Q as [token][KV head][head of the group][head_dim], boxes of `tokens` tokens x `heads` of a group x 64 columns.
+inline bool query_map(CUtensorMap* map, const CacheParams& c, bool bf16, int tokens, int heads) {
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.group, (cuuint64_t)c.kv_heads, (cuuint64_t)c.total_rows};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.q_head_stride * 2, (cuuint64_t)c.q_head_stride * 2 * c.group, (cuuint64_t)c.q_token_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)heads, 1, (cuuint32_t)tokens}, elem[4] = {1, 1, 1, 1};
+  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t*>(c.q), dims, strides,
+                        box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 // Pages must fill TMA boxes of whole swizzle groups (8 rows) that fit a tile of `keys` evenly.
 inline bool pages_fit(const CacheParams& c, int keys) {
