@@ -171,15 +171,12 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     pub.cut = Cut{};
     pub.n = 0;
     Job job;
+    PageRows pages;
     bool ok = true;
     while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
+      pages.start(job.ta);
       for (int t = job.ta; ok && t < job.tb; ++t) {
-        const int j = t * kTileKeys + lane * P.box.rows;
-        int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
-        if (lane < per_tile && j < job.kv_len) {
-          const int64_t r = pool_row(c, job.b, j);
-          if (r >= 0) row = (int32_t)r;
-        }
+        const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
 #pragma unroll
         for (int s = 0; s < kTS; ++s, ++pos) {
           const uint32_t slot = pos % kSlots;

@@ -2,23 +2,25 @@
 // tensor cores, for items of more than one MMA row block: prefill chunks, wide groups.
 //
 // The mathematics is that of ztcp_attend.cu.  An item is up to 256 (token, head-of-the-group) rows of one sequence
-// and KV head, as two row tiles of 128: S = Q K^T and O += P V are tcgen05.mma of 128 x 128 x 16, K and V tiles of
-// 128 keys arrive by TMA page by page (boxes of one page's rows, 128-byte swizzle), and S, P and O live in TMEM:
-// S0 S1 O0 O1 fill its 512 columns, P overwrites the first half of its S.
+// and KV head, as two row tiles of 128: S = Q K^T (128 x 64 x 16 a step) and O += P V (128 x head_dim x 16) are
+// tcgen05.mma, K and V tiles of 64 keys arrive by TMA page by page (boxes of one page's rows, 128-byte swizzle), Q as
+// boxes of tokens x group.  S, P and O live in TMEM: per row tile two buffers of 64 scores, each overwritten by its own
+// P, and O; the two row tiles fill its 512 columns.
 //
-// Warps.  0-3 and 4-7: the softmax of row tiles 0 and 1, a thread per row; 8: one thread issues the products; 9: TMA (10, 11 fill
-// the warpgroup).
-// The products of one row tile run under the softmax of the other:
-//   tensor core   PV0(j-1) QK0(j) | PV1(j-1) QK1(j) | PV0(j) QK0(j+1) | ...
-//   softmax 0                       ---- S0(j) ----
-//   softmax 1                                         ---- S1(j) ----
-// S_q(j) is committed after PV_q(j-1), so whoever sees S_q(j) may also change O_q.  O is rescaled only when a row's
-// maximum has grown by more than 2^8 over the one in use (the weights then stay below 2^8, which the 16-bit types
-// hold without loss); m, l and O are fp32.
+// Warps.  0-3 and 4-7: the softmax of row tiles 0 and 1, a thread per row; 8: one thread issues the products; 9: TMA.
+// With two buffers the scores of a row tile's next 64 keys are there when it has finished with these, so that the
+// exponentials and the products run side by side:
+//   tensor core   PV0(u) QK0(u+2) PV1(u) QK1(u+2) | PV0(u+1) QK0(u+3) ...
+//   softmax 0     -- S0(u+1) -- -- S0(u+2) --
+//   softmax 1     ---- S1(u+1) -- -- S1(u+2) --
+// (With tiles of 128 keys P and the next S take the same columns, and softmax and products of a row tile take turns:
+// measured 3,750 cycles for 256 x 128 scores.)  A tile's exponentials are taken under the maximum in use, without
+// looking for a new one first; only when a score has grown by more than 2^8 over it (the weights then stay below 2^8,
+// which the 16-bit types hold without loss) is the maximum replaced and O rescaled.  m, l and O are fp32.
 //
-// Bound.  Per 128 x 128 scores the tensor core needs 2 x 512 cycles (head_dim 128) and the exponentials 1,024 of the
-// 16-per-cycle unit, so the two take turns at being the limit; a share of the exponentials is computed by a
-// polynomial on the FMA pipes instead (exp2_poly).
+// Bound.  Per 256 x 128 scores the tensor core needs 2,560 cycles (head_dim 128: products of 64 keys read Q at the limit
+// of shared memory's 128 bytes a cycle, else they would need 2,048) and the exponentials 2,048 of the
+// special-function unit's 16 a cycle.
 //
 // Work.  As in ztcp_attend.cu the items form one line that the CTAs (one per SM) share evenly, in units of
 // keys x group (Line); attend_merge_kernel joins items that several CTAs share.
@@ -34,7 +36,8 @@ namespace {
 
 constexpr int kRowTile = 128;
 constexpr int kItemRows = 256;
-constexpr int kThreads = 384;  // three warpgroups: 64,512 registers at launch (168 each)
+constexpr int kTileKeys = 64;
+constexpr int kThreads = 320;
 constexpr int kMmaWarp = 8, kTmaWarp = 9;
 
 struct TcParams {
@@ -43,19 +46,21 @@ struct TcParams {
   int32_t item_tokens;  // whole tokens of a group each: at most 256 rows
 };
 
-constexpr int kBars = 40;  // barrier slots at the start of shared memory
+constexpr int kBars = 56;  // barrier slots at the start of shared memory
 
 template <bool BF16, int HALVES, int SLOTS>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const __grid_constant__ CUtensorMap qmap) {
-  constexpr int kHalf = kGroupBytes;
-  constexpr int kTile = HALVES * kHalf;        // a K or V tile, or a Q row tile
+  constexpr int kHalf = kTileKeys * 128;       // 64 columns of a K or V tile,
+  constexpr int kTile = HALVES * kHalf;        // the tile
+  constexpr int kQHalf = kItemRows * 128;      // and 64 columns of Q
   constexpr int kCols = HALVES * 64;           // head_dim rounded up
   extern __shared__ uint8_t smem_raw[];
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
   __shared__ Job s_jobs[kJobs];
+  __shared__ unsigned s_bad[16];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   volatile int* const dead = &dead_s;
@@ -64,12 +69,12 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t bars = raw;
   const uint32_t tiles = (raw + kBars * 8 + 1023) & ~1023u;
-  const uint32_t qtile = tiles, ring = tiles + 2 * kTile;
+  const uint32_t qtile = tiles, ring = tiles + HALVES * kQHalf;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + (SLOTS + s) * 8; };
-  const uint32_t q_full = bars + 2 * SLOTS * 8, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 16, o_full = p_full + 16,
-                 job_full = o_full + 16, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
-  static_assert(2 * SLOTS + 9 + 2 * kJobs <= kBars, "barrier slots");
+  const uint32_t q_full = bars + 2 * SLOTS * 8, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 32, pv_done = p_full + 32,
+                 job_full = pv_done + 32, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
+  static_assert(2 * SLOTS + 15 + 2 * kJobs <= kBars, "barrier slots");
 
   if (tid == 0) {
     dead_s = 0;
@@ -78,9 +83,11 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       mbar_init(empty(s), 1);
     }
     for (int q = 0; q < 2; ++q) {
-      mbar_init(s_full + 8 * q, 1);
-      mbar_init(p_full + 8 * q, 128);
-      mbar_init(o_full + 8 * q, 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(s_full + 16 * q + 8 * b, 1);
+        mbar_init(p_full + 16 * q + 8 * b, 4);
+        mbar_init(pv_done + 16 * q + 8 * b, 1);
+      }
     }
     for (int e = 0; e < kJobs; ++e) {
       mbar_init(job_full + 8 * e, 1);
@@ -101,156 +108,146 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   const uint32_t tmem = tmem_s;
   cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up meanwhile; it waits for this one's end
 
-  // The softmax warps hold a row of scores: of the block's registers they take 208 a thread, the others 88 (8 x 32 x 208
-  // + 4 x 32 x 88 = 64,512, what the block was launched with).
-  if (warp >= kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kTmaWarp) {
-      // ---- TMA: K and V tiles in turn through the ring; lane p fetches page p of the tile ------------
-      const int per_tile = kKeys / P.box.rows;
-      const int item_rows = P.item_tokens * c.group;
-      uint32_t items = 0;
-      uint32_t pos = 0;  // tiles so far: K of step t is 2 t, V is 2 t + 1
-      int64_t at;
-      Spot spot;
-      const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work(c, item_rows, b); }, &at, &spot);
-      Publisher<kKeys> pub;
-      pub.walk.begin(c, item_rows, 2, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
-      pub.cut = Cut{};
-      pub.n = 0;
-      Job job;
-      bool ok = true;
-      while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
-        // Q as it lies: tokens x group rows, each half of the columns [256][64] (rows past the item's are other tokens', or
-        // left over; nothing of theirs is stored)
-        if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, dead))) break;
-        ++items;
-        if (lane == 0) mbar_expect(q_full, HALVES * item_rows * 128);
-        __syncwarp();
-        if (lane < HALVES) tma_load4(qtile + lane * 2 * kHalf, &qmap, lane * 64, 0, job.head, (int)job.row0 + job.row / c.group, q_full);
-        for (int t = job.ta; ok && t < job.tb; ++t) {
-          const int j = t * kKeys + lane * P.box.rows;
-          int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
-          if (lane < per_tile && j < job.kv_len) {
-            const int64_t r = pool_row(c, job.b, j);
-            if (r >= 0) row = (int32_t)r;
+  if (warp == kTmaWarp) {
+    // ---- TMA: K and V tiles in turn through the ring; lane p fetches page p of the tile ------------
+    const int per_tile = kTileKeys / P.box.rows;
+    const int item_rows = P.item_tokens * c.group;
+    uint32_t items = 0;
+    uint32_t pos = 0, steps = 0;  // K of step u is tile 2 u, V is 2 u + 1
+    int64_t at;
+    Spot spot;
+    const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work(c, item_rows, b); }, &at, &spot);
+    Publisher<kTileKeys> pub;
+    pub.walk.begin(c, item_rows, 4, spot, at < 0 ? 0 : at, at < 0 ? 0 : S.begin(blockIdx.x + 1));
+    pub.cut = Cut{};
+    pub.n = 0;
+    Job job;
+    PageRows pages;
+    bool ok = true;
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
+      // Q as it lies: tokens x group rows, each half of the columns [256][64] (rows past the item's are other tokens', or
+      // left over; nothing of theirs is stored)
+      if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, dead))) break;
+      ++items;
+      if (lane == 0) mbar_expect(q_full, HALVES * item_rows * 128);
+      __syncwarp();
+      if (lane < HALVES) tma_load4(qtile + lane * kQHalf, &qmap, lane * 64, 0, job.head, (int)job.row0 + job.row / c.group, q_full);
+      pages.start(job.ta);
+      for (int t = job.ta; ok && t < job.tb; ++t) {
+        const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
+        // Pages outside the pool count as masked; the softmax warps learn of them here (16 tiles back all have read
+        // theirs: the K tile that was in this slot, at most 6 tiles back, has been multiplied, and P two tiles before
+        // that is written).
+        const unsigned bad = __ballot_sync(0xffffffffu, lane < per_tile && t * kTileKeys + (lane << P.box.shift) < job.kv_len && row == P.box.pool_rows);
+        if (lane == 0) s_bad[steps++ & 15] = bad;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++pos) {
+          const uint32_t slot = pos % SLOTS;
+          ok = ok && (pos < SLOTS || mbar_wait(empty(slot), (pos / SLOTS - 1) & 1, dead));
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
           }
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv, ++pos) {
-            const int slot = pos % SLOTS;
-            ok = ok && (pos < SLOTS || mbar_wait(empty(slot), (pos / SLOTS - 1) & 1, dead));
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_expect(full(slot), kTile);
-            __syncwarp();
-            if (lane < per_tile)
-#pragma unroll
-              for (int x = 0; x < HALVES; ++x)
-                tma_load(ring + slot * kTile + x * kHalf + lane * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, job.head, row, full(slot));
+          if (lane == 0) mbar_expect(full(slot), kTile);
+          __syncwarp();
+          if (lane < HALVES * per_tile) {  // a box of each 64 columns
+            const int x = HALVES > 1 && lane >= per_tile;
+            tma_load(ring + slot * kTile + x * kHalf + (lane & (per_tile - 1)) * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, job.head, row, full(slot));
           }
         }
       }
-      if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
-      if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
-        int none = 0;
-        for (uint32_t p = pos > SLOTS ? pos - SLOTS : 0; p < pos; ++p) mbar_wait(full(p % SLOTS), (p / SLOTS) & 1, &none);
-        if (items > 0) mbar_wait(q_full, (items - 1) & 1, &none);
-      }
-    } else if (warp == kMmaWarp) {
-      // ---- products: one thread ------------------------------------------------------------------------
-      if (elect_one()) {
-        constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
-        const uint32_t qk = inst_desc(BF16, 128, kKeys, false, false), pv = inst_desc(BF16, 128, kCols, false, true);
-        const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kHalf), q_lo = desc_lo(qtile, 16);
-        uint32_t kslot = 0, kphase = 0;    // of the next K tile; V's follows it
-        uint32_t vslot = 1, vphase = 0;
-        uint32_t items = 0;                // items so far
-        uint32_t softs[2] = {0, 0};        // tiles so far, per row tile
-        bool ok = true;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-          ok = ok && mbar_wait(bar, parity & 1, dead);
-          return ok;
-        };
-        auto advance = [&](uint32_t& slot, uint32_t& phase) {  // two slots on
-          slot += 2;
-          if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
-        };
-        const uint32_t tm = tmem;
-        // Step t multiplies P of tile t - 1 by V and computes the scores of tile t; per row tile in turn, so that each
-        // has the other's products to hide its softmax under.
-        Job job;
-        uint32_t njobs = 0;
-        int cur = 0, n = 0;  // row tiles of the step before, and tiles of its item
-        int t = 0;           // of the item's tiles, those whose scores are out
-        while (ok) {
-          const bool fresh = t == n;  // the step's scores are those of the next item
-          if (fresh) {  // published once the loads of the item before are out
-            if (!(ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job))) break;
-            if (cur == 0 && job.ta == job.tb) break;
-          }
-          const int nxt = fresh ? (job.ta < job.tb ? (job.rows > kRowTile ? 2 : 1) : 0) : cur;
-          if (cur && !wait(full(vslot), vphase)) break;
-          bool k_there = false;
+    }
+    if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
+    if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
+      int none = 0;
+      for (uint32_t p = pos > SLOTS ? pos - SLOTS : 0; p < pos; ++p) mbar_wait(full(p % SLOTS), (p / SLOTS) & 1, &none);
+      if (items > 0) mbar_wait(q_full, (items - 1) & 1, &none);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- products: one thread ------------------------------------------------------------------------
+    if (elect_one()) {
+      constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
+      const uint32_t qk = inst_desc(BF16, 128, kTileKeys, false, false), pv = inst_desc(BF16, 128, kCols, false, true);
+      const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kHalf), q_lo = desc_lo(qtile, 16);
+      uint32_t kslot = 0, kphase = 0;      // of the next K tile,
+      uint32_t vslot = 1, vphase = 0;      // and the next V tile
+      uint32_t items = 0;                  // items so far,
+      uint32_t qks[2] = {0, 0}, pvs[2] = {0, 0};  // and, per row tile, scores and products with V
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = ok && mbar_wait(bar, parity & 1, dead);
+        return ok;
+      };
+      auto advance = [&](uint32_t& slot, uint32_t& phase) {  // two slots on
+        slot += 2;
+        if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+      };
+      // One row tile's scores of the K tile at kslot.  Its buffer was last read by the product with V two tiles ago, which
+      // has been issued, and products run in order.
+      auto scores = [&](int q) {
+        const uint32_t a = q_lo + q * (kRowTile * 128 >> 4), b = k_lo + kslot * (kTile >> 4), buf = qks[q] & 1;
+#pragma unroll
+        for (int k = 0; k < HALVES * 4; ++k)
+          mma_ss(tmem + q * 128 + buf * 64, a + (((k >> 2) * kQHalf + (k & 3) * 32) >> 4), kHi, b + (((k >> 2) * kHalf + (k & 3) * 32) >> 4), kHi, qk,
+                 k > 0);
+        tc_commit(s_full + 16 * q + 8 * buf);
+        ++qks[q];
+      };
+      Job job;
+      uint32_t njobs = 0;
+      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job)) && job.ta < job.tb) {
+        const int n = job.tb - job.ta, nq = job.rows > kRowTile ? 2 : 1;
+        if (!wait(q_full, items)) break;
+        ++items;
+        for (int u = -2; ok && u < n; ++u) {  // tile u's product with V, then tile u + 2's scores
+          const bool more = u + 2 < n;
+          if (u >= 0 && !wait(full(vslot), vphase)) break;
+          if (u < 0 && !more) continue;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            if (q < cur) {
-              if (!wait(p_full + 8 * q, softs[q])) break;
-              ++softs[q];
+            if (q >= nq) break;
+            if (u >= 0) {
+              const uint32_t buf = pvs[q] & 1;
+              if (!wait(p_full + 16 * q + 8 * buf, pvs[q] >> 1)) break;
+              ++pvs[q];
               tc_fence_after();
               const uint32_t b = v_lo + vslot * (kTile >> 4);
 #pragma unroll
-              for (int k = 0; k < kKeys / 16; ++k)
-                mma_ts(tm + 256 + q * 128, tm + q * 128 + k * 8, b + (k * 2048 >> 4), kHi, pv, t > 1 || k > 0);
-              if (fresh) tc_commit(o_full + 8 * q);
+              for (int k = 0; k < kTileKeys / 16; ++k)
+                mma_ts(tmem + 256 + q * 128, tmem + q * 128 + buf * 64 + k * 8, b + (k * 2048 >> 4), kHi, pv, u > 0 || k > 0);
+              tc_commit(pv_done + 16 * q + 8 * buf);
             }
-            if (q < nxt) {
-              if (!k_there && ((fresh && !wait(q_full, items)) || !wait(full(kslot), kphase))) break;
-              k_there = true;
+            if (more) {
+              if (q == 0 && !wait(full(kslot), kphase)) break;
               tc_fence_after();
-              const uint32_t a = q_lo + q * (kHalf >> 4), b = k_lo + kslot * (kTile >> 4);
-#pragma unroll
-              for (int k = 0; k < HALVES * 4; ++k) {
-                const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4, qoff = ((k >> 2) * 2 * kHalf + (k & 3) * 32) >> 4;
-                mma_ss(tm + q * 128, a + qoff, kHi, b + off, kHi, qk, k > 0);
-              }
-              tc_commit(s_full + 8 * q);
+              scores(q);
             }
           }
           if (!ok) break;
-          if (cur) {
+          if (u >= 0) {
             tc_commit(empty(vslot));
             advance(vslot, vphase);
           }
-          if (nxt) {
+          if (more) {
             tc_commit(empty(kslot));
             advance(kslot, kphase);
+            if (u + 3 == n) tc_commit(q_empty);  // the item's last scores are out
           }
-          if (fresh) {
-            if (nxt == 0) break;
-            n = job.tb - job.ta;
-            t = 0;
-            ++items;
-          }
-          cur = nxt;
-          if (++t == n) tc_commit(q_empty);  // the item's last scores are out
-        }
-        if (*dead) {  // no product may be in flight when TMEM is freed
-          int none = 0;
-          tc_commit(drain);
-          mbar_wait(drain, 0, &none);
         }
       }
-      __syncwarp();
+      if (*dead) {  // no product may be in flight when TMEM is freed
+        int none = 0;
+        tc_commit(drain);
+        mbar_wait(drain, 0, &none);
+      }
     }
+    __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of row tile q: a thread per row -----------------------------------------------------
     const int q = warp >> 2, wg = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const uint32_t ts = tmem + lanes + q * 128, to = tmem + lanes + 256 + q * 128;
-    uint32_t step = 0, mine = 0, done = 0;  // tiles of the CTA, tiles and items of this row tile
+    const uint32_t to = tmem + lanes + 256 + q * 128;
+    uint32_t step = 0, mine = 0;  // tiles of the CTA, and of this row tile
     Job job;
     uint32_t njobs = 0;
     auto open = [&] { return take_job(s_jobs, job_full, job_empty, njobs, lane, dead, &job); };
@@ -266,82 +263,78 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       const int lim = r < it.rows ? visible_keys(c, Seq{it.kv_len, it.q_len, it.row0}, (it.row + r) / c.group) : 0;
       float m = -INFINITY, l = 0.f;
       for (int t = it.ta; t < it.tb; ++t, ++step, ++mine) {
-        const int j0 = t * kKeys;
-        // pages of this tile outside the pool count as masked
-        unsigned bad = 0;
-        {
-          const int j = j0 + lane * P.box.rows;
-          const bool b = lane < kKeys / P.box.rows && j < it.kv_len && pool_row(c, it.b, j) < 0;
-          bad = __ballot_sync(0xffffffffu, b);
-        }
-        if (!(ok = warp_wait(s_full + 8 * q, mine & 1, dead))) break;
+        const int j0 = t * kTileKeys;
+        const uint32_t buf = mine & 1, ts = tmem + lanes + q * 128 + buf * 64;
+        if (!(ok = warp_wait(s_full + 16 * q + 8 * buf, (mine >> 1) & 1, dead))) break;
         tc_fence_after();
-        uint32_t x[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(ts + i * 32, x + i * 32);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ready32(x + i * 32);
-        const uint64_t sc2 = pair(c.scale_log2, c.scale_log2);
-        // A tile that every row sees whole, once a maximum is in use: its exponentials need no new one unless a score
-        // has grown by 2^8, which shows by the way; the scores are then read again below.  Of eight pairs, three
-        // exponentials go to the FMA pipes.
-        bool done = false;
-        if (__all_sync(0xffffffffu, lim >= j0 + kKeys && m > -INFINITY) && !bad) {
-          const uint64_t z2 = pair(-m, -m);
+        const unsigned bad = s_bad[step & 15];
+        uint32_t x[64];
+        tmem_ld32(ts, x);
+        tmem_ld32(ts + 32, x + 32);
+        tmem_ready32(x);
+        tmem_ready32(x + 32);
+        // A tile that every row sees whole, once a maximum is in use: whether a score has outgrown it shows by the way.
+        // (Computing a share of the exponentials by a polynomial, as ztcp_mass_tc.cu does, was measured slower here:
+        // 1,570 against 1,490 cycles for 128 of them in a warp alone, 2,120 against 2,100 with four warps a scheduler.)
+        bool ready = false;
+        if (__all_sync(0xffffffffu, lim >= j0 + kTileKeys && m > -INFINITY) && !bad) {
+          const uint64_t sc2 = pair(c.scale_log2, c.scale_log2), z2 = pair(-m, -m);
           uint64_t sum = pair(0.f, 0.f), sum1 = sum;
           float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 128; i += 4) {
+          for (int i = 0; i < 64; i += 4) {
             top = fmaxf(top, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
             top1 = fmaxf(top1, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
-            uint64_t u = fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, z2);
-            uint64_t v = fma2(pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), sc2, z2);
             float a, b, d, e;
-            if (i % 16 == 4) u = exp2_poly(u), unpair(u, a, b);
-            else unpair(u, a, b), a = fast_exp2(a), b = fast_exp2(b), u = pair(a, b);
-            if (i % 8 == 0) v = exp2_poly(v), unpair(v, d, e);
-            else unpair(v, d, e), d = fast_exp2(d), e = fast_exp2(e), v = pair(d, e);
-            sum = add2(sum, u);
-            sum1 = add2(sum1, v);
+            unpair(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, z2), a, b);
+            unpair(fma2(pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), sc2, z2), d, e);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
+            d = fast_exp2(d);
+            e = fast_exp2(e);
+            sum = add2(sum, pair(a, b));
+            sum1 = add2(sum1, pair(d, e));
             x[i / 2] = pack2<BF16>(a, b);
             x[i / 2 + 1] = pack2<BF16>(d, e);
           }
-          done = __all_sync(0xffffffffu, fmaxf(top, top1) * c.scale_log2 <= m + 8.f);
-          if (done) {
+          ready = __all_sync(0xffffffffu, fmaxf(top, top1) * c.scale_log2 <= m + 8.f);
+          if (ready) {
             float s0, s1, s2, s3;
             unpair(sum, s0, s1);
             unpair(sum1, s2, s3);
             l += (s0 + s1) + (s2 + s3);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(ts + i * 32, x + i * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ready32(x + i * 32);
+          } else {  // the scores once more
+            tmem_ld32(ts, x);
+            tmem_ld32(ts + 32, x + 32);
+            tmem_ready32(x);
+            tmem_ready32(x + 32);
           }
         }
-        if (!done) {
-          if (!__all_sync(0xffffffffu, lim >= j0 + kKeys) || bad) {
+        if (!ready) {
+          if (!__all_sync(0xffffffffu, lim >= j0 + kTileKeys) || bad) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
+            for (int i = 0; i < 64; ++i)
               if (j0 + i >= lim || (bad >> (i >> P.box.shift) & 1)) x[i] = 0xff800000u;
           }
           float mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+          for (int i = 0; i < 64; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
           mx *= c.scale_log2;
           const bool grow = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
             const float mn = grow ? mx : m;
             const float f = grow ? fast_exp2(m - mn) : 1.f;  // 0 for the first maximum
-            if (t > it.ta) {
-              uint32_t o[32];
+            if (t > it.ta) {  // O is this thread's to change between its products
+              if (!(ok = warp_wait(pv_done + 16 * q + 8 * ((mine - 1) & 1), ((mine - 1) >> 1) & 1, dead))) break;
+              tc_fence_after();
 #pragma unroll 1
-              for (int i = 0; i < HALVES * 2; ++i) {
-                tmem_ld32(to + i * 32, o);
+              for (int i = 0; i < kCols; i += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + i, o);
                 tmem_ready32(o);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(to + i * 32, o);
+                tmem_st32(to + i, o);
               }
             }
             l *= f;
@@ -350,7 +343,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           const float z = m == -INFINITY ? 0.f : -m;
           float sum = 0.f, sum1 = 0.f;
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) {
+          for (int i = 0; i < 64; i += 2) {
             const float a = fast_exp2(fmaf(__uint_as_float(x[i]), c.scale_log2, z)), b = fast_exp2(fmaf(__uint_as_float(x[i + 1]), c.scale_log2, z));
             sum += a;
             sum1 += b;
@@ -359,13 +352,12 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           l += sum + sum1;
         }
         tmem_st32(ts, x);
-        tmem_st32(ts + 32, x + 32);
         // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V
         const int end = it.kv_len - j0;
-        if (q == 0 && end < kKeys && it.kv_len % c.page_tokens != 0) {
+        if (q == 0 && end < kTileKeys && it.kv_len % c.page_tokens != 0) {
           const uint32_t vp = 2 * step + 1;
           if (!(ok = warp_wait(full(vp % SLOTS), (vp / SLOTS) & 1, dead))) break;
-          if (wg >= end)
+          if (wg >= end && wg < kTileKeys)
 #pragma unroll
             for (int i = 0; i < HALVES * 8; ++i)
               asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + (vp % SLOTS) * kTile + (i >> 3) * kHalf + wg * 128 + (i & 7) * 16),
@@ -374,47 +366,46 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         }
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full + 8 * q);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 16 * q + 8 * buf);
       }
       if (!ok) break;
       if (!(ok = open())) break;
 
-      if (!(ok = warp_wait(o_full + 8 * q, done & 1, dead))) break;
-      ++done;
+      if (!(ok = warp_wait(pv_done + 16 * q + 8 * ((mine - 1) & 1), ((mine - 1) >> 1) & 1, dead))) break;
       tc_fence_after();
-      const bool whole = it.whole;
       const int tok = (it.row + r) / c.group, gh = (it.row + r) - tok * c.group;
       const int64_t o = (it.row0 + tok) * (int64_t)(c.kv_heads * c.group) + it.head * c.group + gh;
       float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll 1
-      for (int i = 0; i < HALVES * 2; ++i) {
+      for (int i = 0; i < kCols; i += 32) {
         uint32_t v[32];
-        tmem_ld32(to + i * 32, v);
+        tmem_ld32(to + i, v);
         tmem_ready32(v);
         if (r < it.rows) {
-          if (whole) {
+          if (it.whole) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
-              if (i * 32 + e < c.v_dim) {
+              if (i + e < c.v_dim) {
                 uint4 w;
                 w.x = pack2<BF16>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
                 w.y = pack2<BF16>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
                 w.z = pack2<BF16>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
                 w.w = pack2<BF16>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
-                *reinterpret_cast<uint4*>(P.a.out + o * c.v_dim + i * 32 + e) = w;
+                *reinterpret_cast<uint4*>(P.a.out + o * c.v_dim + i + e) = w;
               }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              if (i * 32 + e < c.v_dim)  // rows contiguous, so that a warp's store is one
-                *reinterpret_cast<uint4*>(part + ((i * 8 + e / 4) * P.a.part_rows + r) * 4) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              if (i + e < c.v_dim)  // rows contiguous, so that a warp's store is one
+                *reinterpret_cast<uint4*>(part + ((i + e) / 4 * P.a.part_rows + r) * 4) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
       }
       tc_fence_before();
       if (r < it.rows) {
-        if (!whole) {
+        if (!it.whole) {
           part[kItemRows * c.v_dim + r] = m;
           part[kItemRows * (c.v_dim + 1) + r] = l;
         } else if (P.a.lse) {
@@ -435,27 +426,27 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
 template <bool BF16, int HALVES, int SLOTS>
 void launch_kernel(const TcParams& P, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, cudaStream_t s) {
   auto* const f = attend_tc_kernel<BF16, HALVES, SLOTS>;
-  const int smem = kBars * 8 + 1024 + (2 + SLOTS) * HALVES * kKeys * 128;
+  const int smem = kBars * 8 + 1024 + HALVES * (kItemRows + SLOTS * kTileKeys) * 128;
   cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   f<<<P.a.grid, kThreads, smem, s>>>(P, k, v, q);
 }
 
 }  // namespace
 
-bool attend_tc_fits(const CacheParams& c) { return c.v && c.head_dim <= 128 && c.group <= kItemRows && pages_fit(c, kKeys); }
+bool attend_tc_fits(const CacheParams& c) { return c.v && c.head_dim <= 128 && c.group <= kItemRows && pages_fit(c, kTileKeys); }
 
 AttendShape attend_tc_shape(const CacheParams& c, int sms) { return {sms, kItemRows, kItemRows * (c.v_dim + 2), 1}; }
 
 bool launch_attend_tc(const AttendParams& A, bool bf16, cudaStream_t s) {
   TcParams P;
   P.a = A;
-  P.box = pool_boxes(A.c, kKeys);
+  P.box = pool_boxes(A.c, kTileKeys);
   P.item_tokens = kItemRows / A.c.group;
   CUtensorMap k, v, q;
   if (!pool_map(&k, A.c.k, A.c, bf16, P.box) || !pool_map(&v, A.c.v, A.c, bf16, P.box) || !query_map(&q, A.c, bf16, P.item_tokens, A.c.group))
     return false;
-  if (A.c.head_dim <= 64) bf16 ? launch_kernel<true, 1, 8>(P, k, v, q, s) : launch_kernel<false, 1, 8>(P, k, v, q, s);
-  else bf16 ? launch_kernel<true, 2, 5>(P, k, v, q, s) : launch_kernel<false, 2, 5>(P, k, v, q, s);
+  if (A.c.head_dim <= 64) bf16 ? launch_kernel<true, 1, 12>(P, k, v, q, s) : launch_kernel<false, 1, 12>(P, k, v, q, s);
+  else bf16 ? launch_kernel<true, 2, 10>(P, k, v, q, s) : launch_kernel<false, 2, 10>(P, k, v, q, s);
   return true;
 }
 

@@ -158,6 +158,28 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t t) {
   return pair(__int_as_float(__float_as_int(x) + (__float_as_int(m) << 23)), __int_as_float(__float_as_int(y) + (__float_as_int(n) << 23)));
 }
 
+// ---- pages of the tiles to come ---------------------------------------------------------------------
+// The pool rows of the next 32 boxes of a sequence, a lane each: one look at the page table serves 32 / per_tile tiles.
+// (A look per tile, 600 to 900 cycles each, was the limit of the loading warp: chunk attention took 1,880 cycles per
+// 64 keys with it, whatever products and exponentials took.)
+struct PageRows {
+  int32_t row, t0;
+  __device__ __forceinline__ void start(int t) { t0 = t - 32; }  // a new item that begins with tile t
+  // Lane p, p + per_tile, ..: the row of tile t's box p; pool_rows past the sequence's end and for a page outside the pool.
+  __device__ __forceinline__ int32_t at(const CacheParams& c, const PoolBoxes& box, int per_tile, int b, int kv_len, int t, int lane) {
+    if ((t - t0) * per_tile >= 32) {
+      t0 = t;
+      const int64_t j = ((int64_t)t * per_tile + lane) << box.shift;
+      row = box.pool_rows;
+      if (j < kv_len) {
+        const int64_t r = pool_row(c, b, (int)j);
+        if (r >= 0) row = (int32_t)r;
+      }
+    }
+    return __shfl_sync(0xffffffffu, row, (t - t0) * per_tile + (lane & (per_tile - 1)));
+  }
+};
+
 // ---- the line of items ----------------------------------------------------------------------------
 // Items of up to `rows` (token, head-of-the-group) rows of one sequence and KV head form one line, sequence by
 // sequence, row tile by row tile, head by head, that the CTAs share evenly, in units of keys x group: an item's
