@@ -37,8 +37,8 @@ namespace {
 constexpr int kRowTile = 128;
 constexpr int kItemRows = 256;
 constexpr int kTileKeys = 64;
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kThreads = 352;
+constexpr int kMmaWarp = 8, kTmaWarp = 10;  // a warp of products for each row tile
 
 struct TcParams {
   AttendParams a;
@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const __grid_constant__ CUtensorMap qmap) {
   constexpr int kHalf = kTileKeys * 128;       // 64 columns of a K or V tile,
-  constexpr int kTile = HALVES * kHalf;        // the tile
+  constexpr int kTile = HALVES * kHalf;        // the tile,
+  constexpr int kStage = 2 * kTile;            // a stage of the ring
   constexpr int kQHalf = kItemRows * 128;      // and 64 columns of Q
   constexpr int kCols = HALVES * 64;           // head_dim rounded up
   extern __shared__ uint8_t smem_raw[];
@@ -72,30 +73,32 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   const uint32_t qtile = tiles, ring = tiles + HALVES * kQHalf;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + (SLOTS + s) * 8; };
-  const uint32_t q_full = bars + 2 * SLOTS * 8, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 32, pv_done = p_full + 32,
-                 job_full = pv_done + 32, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
-  static_assert(2 * SLOTS + 15 + 2 * kJobs <= kBars, "barrier slots");
+  const uint32_t q_full = bars + 2 * SLOTS * 8, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 32, pv_last = p_full + 32,
+                 pv_prev = pv_last + 16, job_full = pv_prev + 16, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
+  static_assert(2 * SLOTS + 16 + 2 * kJobs <= kBars, "barrier slots");
 
   if (tid == 0) {
     dead_s = 0;
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), 2);
     }
     for (int q = 0; q < 2; ++q) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(s_full + 16 * q + 8 * b, 1);
         mbar_init(p_full + 16 * q + 8 * b, 4);
-        mbar_init(pv_done + 16 * q + 8 * b, 1);
       }
+      mbar_init(pv_last + 8 * q, 1);
+      mbar_init(pv_prev + 8 * q, 1);
     }
     for (int e = 0; e < kJobs; ++e) {
       mbar_init(job_full + 8 * e, 1);
-      mbar_init(job_empty + 8 * e, 9);
+      mbar_init(job_empty + 8 * e, 10);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     mbar_init(drain, 1);
+    mbar_init(drain + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -109,11 +112,10 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up meanwhile; it waits for this one's end
 
   if (warp == kTmaWarp) {
-    // ---- TMA: K and V tiles in turn through the ring; lane p fetches page p of the tile ------------
-    const int per_tile = kTileKeys / P.box.rows;
+    // ---- TMA: the CTA's tiles in a row, items or not.  Stage g of the ring: K of tile g and V of tile g - 2 ----
+    const int per_tile = kTileKeys / P.box.rows, boxes = HALVES * per_tile;
     const int item_rows = P.item_tokens * c.group;
-    uint32_t items = 0;
-    uint32_t pos = 0, steps = 0;  // K of step u is tile 2 u, V is 2 u + 1
+    uint32_t items = 0, pos = 0;
     int64_t at;
     Spot spot;
     const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work(c, item_rows, b); }, &at, &spot);
@@ -124,38 +126,49 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     Job job;
     PageRows pages;
     bool ok = true;
-    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
-      // Q as it lies: tokens x group rows, each half of the columns [256][64] (rows past the item's are other tokens', or
-      // left over; nothing of theirs is stored)
-      if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, dead))) break;
-      ++items;
-      if (lane == 0) mbar_expect(q_full, HALVES * item_rows * 128);
+    int32_t row1 = 0, row2 = 0, head1 = 0, head2 = 0;  // pool rows and heads of the last tile and the one before
+    // Lane p loads box p of V, of 64 columns and one page each, and lane boxes + p that of K.
+    auto stage = [&](bool v_on, bool k_on, int32_t row, int32_t head) {
+      const uint32_t slot = pos % SLOTS;
+      if (pos >= SLOTS && !warp_wait(empty(slot), (pos / SLOTS - 1) & 1, dead)) return false;
+      if (lane == 0) mbar_expect(full(slot), (v_on ? kTile : 0) + (k_on ? kTile : 0));
       __syncwarp();
-      if (lane < HALVES) tma_load4(qtile + lane * kQHalf, &qmap, lane * 64, 0, job.head, (int)job.row0 + job.row / c.group, q_full);
+      const bool isk = lane >= boxes;
+      const int p = isk ? lane - boxes : lane;
+      if (p < boxes && (isk ? k_on : v_on)) {
+        const int x = HALVES > 1 && p >= per_tile;
+        tma_load(ring + slot * kStage + (isk ? kTile : 0) + x * kHalf + (p & (per_tile - 1)) * P.box.rows * 128, isk ? &kmap : &vmap, x * 64,
+                 isk ? head : head2, isk ? row : row2, full(slot));
+      }
+      __syncwarp();
+      ++pos;
+      row2 = row1;
+      head2 = head1;
+      row1 = row;
+      head1 = head;
+      return true;
+    };
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
       pages.start(job.ta);
-      for (int t = job.ta; ok && t < job.tb; ++t) {
+      for (int t = job.ta; t < job.tb; ++t) {
         const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
         // Pages outside the pool count as masked; the softmax warps learn of them here (16 tiles back all have read
-        // theirs: the K tile that was in this slot, at most 6 tiles back, has been multiplied, and P two tiles before
-        // that is written).
+        // theirs: the stage that was in this slot, at most 8 tiles back, is spent).
         const unsigned bad = __ballot_sync(0xffffffffu, lane < per_tile && t * kTileKeys + (lane << P.box.shift) < job.kv_len && row == P.box.pool_rows);
-        if (lane == 0) s_bad[steps++ & 15] = bad;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++pos) {
-          const uint32_t slot = pos % SLOTS;
-          ok = ok && (pos < SLOTS || mbar_wait(empty(slot), (pos / SLOTS - 1) & 1, dead));
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_expect(full(slot), kTile);
-          __syncwarp();
-          if (lane < HALVES * per_tile) {  // a box of each 64 columns
-            const int x = HALVES > 1 && lane >= per_tile;
-            tma_load(ring + slot * kTile + x * kHalf + (lane & (per_tile - 1)) * P.box.rows * 128, kv ? &vmap : &kmap, x * 64, job.head, row, full(slot));
-          }
-        }
+        if (lane == 0) s_bad[pos & 15] = bad;
+        if (!(ok = stage(pos >= 2, true, row, job.head))) break;
+        if (t > job.ta) continue;
+        // Q as it lies: tokens x group rows, each half of the columns [256][64] (rows past the item's are other tokens',
+        // or left over; nothing of theirs is stored).  The item before needs its own Q for one tile less than V.
+        if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, dead))) break;
+        ++items;
+        if (lane == 0) mbar_expect(q_full, HALVES * item_rows * 128);
+        __syncwarp();
+        if (lane < HALVES) tma_load4(qtile + lane * kQHalf, &qmap, lane * 64, 0, job.head, (int)job.row0 + job.row / c.group, q_full);
       }
+    }
+    if (ok && pos > 0) {  // the last two tiles' V (one tile in all: an empty stage before it)
+      ok = stage(pos >= 2, false, 0, 0) && stage(true, false, 0, 0);
     }
     if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
     if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
@@ -163,83 +176,73 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       for (uint32_t p = pos > SLOTS ? pos - SLOTS : 0; p < pos; ++p) mbar_wait(full(p % SLOTS), (p / SLOTS) & 1, &none);
       if (items > 0) mbar_wait(q_full, (items - 1) & 1, &none);
     }
-  } else if (warp == kMmaWarp) {
-    // ---- products: one thread ------------------------------------------------------------------------
+  } else if (warp >= kMmaWarp) {
+    // ---- products of row tile q: one thread ----------------------------------------------------------
+    const int q = warp - kMmaWarp;
     if (elect_one()) {
       constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
       const uint32_t qk = inst_desc(BF16, 128, kTileKeys, false, false), pv = inst_desc(BF16, 128, kCols, false, true);
-      const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kHalf), q_lo = desc_lo(qtile, 16);
-      uint32_t kslot = 0, kphase = 0;      // of the next K tile,
-      uint32_t vslot = 1, vphase = 0;      // and the next V tile
-      uint32_t items = 0;                  // items so far,
-      uint32_t qks[2] = {0, 0}, pvs[2] = {0, 0};  // and, per row tile, scores and products with V
-      bool ok = true;
+      const uint32_t v_lo = desc_lo(ring, kHalf), k_lo = desc_lo(ring + kTile, 16), q_lo = desc_lo(qtile + q * kRowTile * 128, 16);
+      const uint32_t s_at = tmem + q * 128, o_at = tmem + 256 + q * 128, s_done = s_full + 16 * q, p_there = p_full + 16 * q;
+      uint32_t slot = 0, phase = 0;  // of the stage
+      uint32_t items = 0, njobs = 0;
+      uint32_t qks = 0, pvs = 0;  // scores and products with V so far
+      // What tile g, g + 1 and g + 2 of the CTA are, for one stage after the other:
+      constexpr int kTile1 = 1, kMine = 2, kFirst = 4, kLast = 8;  // a tile; with rows of this row tile; the item's first, its last
+      int now = 0, next = 0, t = 0;
+      bool more = true, ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
         ok = ok && mbar_wait(bar, parity & 1, dead);
         return ok;
       };
-      auto advance = [&](uint32_t& slot, uint32_t& phase) {  // two slots on
-        slot += 2;
-        if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
-      };
-      // One row tile's scores of the K tile at kslot.  Its buffer was last read by the product with V two tiles ago, which
-      // has been issued, and products run in order.
-      auto scores = [&](int q) {
-        const uint32_t a = q_lo + q * (kRowTile * 128 >> 4), b = k_lo + kslot * (kTile >> 4), buf = qks[q] & 1;
-#pragma unroll
-        for (int k = 0; k < HALVES * 4; ++k)
-          mma_ss(tmem + q * 128 + buf * 64, a + (((k >> 2) * kQHalf + (k & 3) * 32) >> 4), kHi, b + (((k >> 2) * kHalf + (k & 3) * 32) >> 4), kHi, qk,
-                 k > 0);
-        tc_commit(s_full + 16 * q + 8 * buf);
-        ++qks[q];
-      };
       Job job;
-      uint32_t njobs = 0;
-      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job)) && job.ta < job.tb) {
-        const int n = job.tb - job.ta, nq = job.rows > kRowTile ? 2 : 1;
-        if (!wait(q_full, items)) break;
-        ++items;
-        for (int u = -2; ok && u < n; ++u) {  // tile u's product with V, then tile u + 2's scores
-          const bool more = u + 2 < n;
-          if (u >= 0 && !wait(full(vslot), vphase)) break;
-          if (u < 0 && !more) continue;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (q >= nq) break;
-            if (u >= 0) {
-              const uint32_t buf = pvs[q] & 1;
-              if (!wait(p_full + 16 * q + 8 * buf, pvs[q] >> 1)) break;
-              ++pvs[q];
-              tc_fence_after();
-              const uint32_t b = v_lo + vslot * (kTile >> 4);
-#pragma unroll
-              for (int k = 0; k < kTileKeys / 16; ++k)
-                mma_ts(tmem + 256 + q * 128, tmem + q * 128 + buf * 64 + k * 8, b + (k * 2048 >> 4), kHi, pv, u > 0 || k > 0);
-              tc_commit(pv_done + 16 * q + 8 * buf);
-            }
-            if (more) {
-              if (q == 0 && !wait(full(kslot), kphase)) break;
-              tc_fence_after();
-              scores(q);
-            }
-          }
-          if (!ok) break;
-          if (u >= 0) {
-            tc_commit(empty(vslot));
-            advance(vslot, vphase);
-          }
-          if (more) {
-            tc_commit(empty(kslot));
-            advance(kslot, kphase);
-            if (u + 3 == n) tc_commit(q_empty);  // the item's last scores are out
-          }
+      job.tb = 0;
+      while (true) {
+        int then = 0;
+        if (more && t == job.tb) {
+          if (!(ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job))) break;
+          more = job.ta < job.tb;
+          t = job.ta;
+          then = kFirst;
         }
+        if (more) {
+          ++t;
+          then |= kTile1 | (q == 0 || job.rows > kRowTile ? kMine : 0) | (t == job.tb ? kLast : 0);
+        } else {
+          then = 0;
+        }
+        if ((now | next | then) == 0 || !wait(full(slot), phase)) break;
+        if (now & kMine) {
+          const uint32_t buf = pvs & 1, b = v_lo + slot * (kStage >> 4);
+          if (!wait(p_there + 8 * buf, pvs >> 1)) break;
+          ++pvs;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            mma_ts(o_at, s_at + buf * 64 + k * 8, b + (k * 2048 >> 4), kHi, pv, !(now & kFirst) || k > 0);
+          // Scores that follow say that this product is done; the item's last two have barriers of their own.
+          if (now & kLast) tc_commit(pv_last + 8 * q);
+          else if ((next & (kFirst | kLast)) == kLast) tc_commit(pv_prev + 8 * q);
+        }
+        if ((then & kFirst) && !wait(q_full, items++)) break;
+        if (then & kMine) {
+          // the scores' buffer was last read by a product with V that has been issued, and products run in order
+          tc_fence_after();
+          const uint32_t buf = qks++ & 1, b = k_lo + slot * (kStage >> 4);
+#pragma unroll
+          for (int k = 0; k < HALVES * 4; ++k)
+            mma_ss(s_at + buf * 64, q_lo + (((k >> 2) * kQHalf + (k & 3) * 32) >> 4), kHi, b + (((k >> 2) * kHalf + (k & 3) * 32) >> 4), kHi, qk, k > 0);
+          tc_commit(s_done + 8 * buf);
+        }
+        tc_commit(empty(slot));
+        if (then & kLast) tc_commit(q_empty);
+        if (++slot == SLOTS) slot = 0, phase ^= 1;
+        now = next;
+        next = then;
       }
-      if (*dead) {  // no product may be in flight when TMEM is freed
-        int none = 0;
-        tc_commit(drain);
-        mbar_wait(drain, 0, &none);
-      }
+      int none = 0;  // no product may be in flight when TMEM is freed, after a timeout either
+      tc_commit(drain + 8 * q);
+      mbar_wait(drain + 8 * q, 0, &none);
     }
     __syncwarp();
   } else {
@@ -248,6 +251,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t to = tmem + lanes + 256 + q * 128;
     uint32_t step = 0, mine = 0;  // tiles of the CTA, and of this row tile
+    uint32_t ends = 0, prevs = 0;  // items of this row tile, and those of more than one tile
     Job job;
     uint32_t njobs = 0;
     auto open = [&] { return take_job(s_jobs, job_full, job_empty, njobs, lane, dead, &job); };
@@ -260,7 +264,11 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         continue;
       }
       const int r = q * kRowTile + wg;
-      const int lim = r < it.rows ? visible_keys(c, Seq{it.kv_len, it.q_len, it.row0}, (it.row + r) / c.group) : 0;
+      // (rows past the item's see what its last row sees: they slow no tile down)
+      const int lim = visible_keys(c, Seq{it.kv_len, it.q_len, it.row0}, (it.row + min(r, it.rows - 1)) / c.group);
+      const int clear = __reduce_min_sync(0xffffffffu, lim) / kTileKeys;  // tiles that all of the warp's rows see whole
+      bool live = false;  // all of them have a maximum
+      const bool prev = it.tb - it.ta > 1;
       float m = -INFINITY, l = 0.f;
       for (int t = it.ta; t < it.tb; ++t, ++step, ++mine) {
         const int j0 = t * kTileKeys;
@@ -277,7 +285,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         // (Computing a share of the exponentials by a polynomial, as ztcp_mass_tc.cu does, was measured slower here:
         // 1,570 against 1,490 cycles for 128 of them in a warp alone, 2,120 against 2,100 with four warps a scheduler.)
         bool ready = false;
-        if (__all_sync(0xffffffffu, lim >= j0 + kTileKeys && m > -INFINITY) && !bad) {
+        if (t < clear && live && !bad) {
           const uint64_t sc2 = pair(c.scale_log2, c.scale_log2), z2 = pair(-m, -m);
           uint64_t sum = pair(0.f, 0.f), sum1 = sum;
           float top = -INFINITY, top1 = -INFINITY;
@@ -311,7 +319,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           }
         }
         if (!ready) {
-          if (!__all_sync(0xffffffffu, lim >= j0 + kTileKeys) || bad) {
+          if (t >= clear || bad) {
 #pragma unroll
             for (int i = 0; i < 64; ++i)
               if (j0 + i >= lim || (bad >> (i >> P.box.shift) & 1)) x[i] = 0xff800000u;
@@ -325,7 +333,9 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
             const float mn = grow ? mx : m;
             const float f = grow ? fast_exp2(m - mn) : 1.f;  // 0 for the first maximum
             if (t > it.ta) {  // O is this thread's to change between its products
-              if (!(ok = warp_wait(pv_done + 16 * q + 8 * ((mine - 1) & 1), ((mine - 1) >> 1) & 1, dead))) break;
+              if (t + 1 < it.tb) ok = warp_wait(s_full + 16 * q + 8 * (buf ^ 1), ((mine + 1) >> 1) & 1, dead);
+              else ok = warp_wait(pv_prev + 8 * q, prevs & 1, dead);
+              if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
               for (int i = 0; i < kCols; i += 32) {
@@ -339,6 +349,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
             }
             l *= f;
             m = mn;
+            live = __all_sync(0xffffffffu, m > -INFINITY);
           }
           const float z = m == -INFINITY ? 0.f : -m;
           float sum = 0.f, sum1 = 0.f;
@@ -352,15 +363,16 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
           l += sum + sum1;
         }
         tmem_st32(ts, x);
-        // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V
+        // rows of V past the sequence's end lie in its last page and may hold anything: zero them for 0 * V (both row
+        // tiles' warps do, each for its own product)
         const int end = it.kv_len - j0;
-        if (q == 0 && end < kTileKeys && it.kv_len % c.page_tokens != 0) {
-          const uint32_t vp = 2 * step + 1;
+        if (end < kTileKeys && it.kv_len % c.page_tokens != 0) {
+          const uint32_t vp = step + 2;
           if (!(ok = warp_wait(full(vp % SLOTS), (vp / SLOTS) & 1, dead))) break;
           if (wg >= end && wg < kTileKeys)
 #pragma unroll
             for (int i = 0; i < HALVES * 8; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + (vp % SLOTS) * kTile + (i >> 3) * kHalf + wg * 128 + (i & 7) * 16),
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + (vp % SLOTS) * kStage + (i >> 3) * kHalf + wg * 128 + (i & 7) * 16),
                            "r"(0) : "memory");
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
@@ -372,8 +384,10 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       if (!ok) break;
       if (!(ok = open())) break;
 
-      if (!(ok = warp_wait(pv_done + 16 * q + 8 * ((mine - 1) & 1), ((mine - 1) >> 1) & 1, dead))) break;
+      if (!(ok = warp_wait(pv_last + 8 * q, ends & 1, dead))) break;
       tc_fence_after();
+      ++ends;
+      prevs += prev;
       const int tok = (it.row + r) / c.group, gh = (it.row + r) - tok * c.group;
       const int64_t o = (it.row0 + tok) * (int64_t)(c.kv_heads * c.group) + it.head * c.group + gh;
       float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
@@ -426,7 +440,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
 template <bool BF16, int HALVES, int SLOTS>
 void launch_kernel(const TcParams& P, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, cudaStream_t s) {
   auto* const f = attend_tc_kernel<BF16, HALVES, SLOTS>;
-  const int smem = kBars * 8 + 1024 + HALVES * (kItemRows + SLOTS * kTileKeys) * 128;
+  const int smem = kBars * 8 + 1024 + HALVES * (kItemRows + SLOTS * 2 * kTileKeys) * 128;
   cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   f<<<P.a.grid, kThreads, smem, s>>>(P, k, v, q);
 }
@@ -445,8 +459,8 @@ bool launch_attend_tc(const AttendParams& A, bool bf16, cudaStream_t s) {
   CUtensorMap k, v, q;
   if (!pool_map(&k, A.c.k, A.c, bf16, P.box) || !pool_map(&v, A.c.v, A.c, bf16, P.box) || !query_map(&q, A.c, bf16, P.item_tokens, A.c.group))
     return false;
-  if (A.c.head_dim <= 64) bf16 ? launch_kernel<true, 1, 12>(P, k, v, q, s) : launch_kernel<false, 1, 12>(P, k, v, q, s);
-  else bf16 ? launch_kernel<true, 2, 10>(P, k, v, q, s) : launch_kernel<false, 2, 10>(P, k, v, q, s);
+  if (A.c.head_dim <= 64) bf16 ? launch_kernel<true, 1, 7>(P, k, v, q, s) : launch_kernel<false, 1, 7>(P, k, v, q, s);
+  else bf16 ? launch_kernel<true, 2, 5>(P, k, v, q, s) : launch_kernel<false, 2, 5>(P, k, v, q, s);
   return true;
 }
 
