@@ -282,8 +282,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         tmem_ready32(x);
         tmem_ready32(x + 32);
         // A tile that every row sees whole, once a maximum is in use: whether a score has outgrown it shows by the way.
-        // (Computing a share of the exponentials by a polynomial, as ztcp_mass_tc.cu does, was measured slower here:
-        // 1,570 against 1,490 cycles for 128 of them in a warp alone, 2,120 against 2,100 with four warps a scheduler.)
+        // (A share of the exponentials as a polynomial on the FMA pipes: measured 4 to 11 % slower in all, an eighth to 3/8.)
         bool ready = false;
         if (t < clear && live && !bad) {
           const uint64_t sc2 = pair(c.scale_log2, c.scale_log2), z2 = pair(-m, -m);

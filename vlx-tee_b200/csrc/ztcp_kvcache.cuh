@@ -87,7 +87,7 @@ void launch_attend_merge(const AttendParams& P, bool bf16, int64_t rows, cudaStr
 void launch_page_mass(const MassParams& P, bool bf16, cudaStream_t s);
 // Tensor-core kernel (ztcp_mass_tc.cu): whether it can take a call, workspace bytes, launch (false: no tensor map).
 bool page_mass_tc_fits(const CacheParams& c);
-int64_t page_mass_tc_workspace(const CacheParams& c, int sms);
+int64_t page_mass_tc_workspace(const CacheParams& c, int64_t rows, int sms);
 bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s);
 
 // ------------------------------------------------------------------------------------------------

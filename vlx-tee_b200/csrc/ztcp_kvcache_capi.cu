@@ -184,7 +184,7 @@ int64_t ztcp_page_mass_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_qu
     launched("ztcp_page_mass_workspace_bytes");
     return -1;
   }
-  return ztcp::page_mass_tc_fits(c) ? ztcp::page_mass_tc_workspace(c, sms) : 16;
+  return ztcp::page_mass_tc_fits(c) ? ztcp::page_mass_tc_workspace(c, c.group * queries->max_q_len, sms) : 16;
 }
 
 int32_t ztcp_page_mass(const ztcp_kv_cache* cache, const ztcp_queries* queries, const float* lse, const float* mass,
@@ -199,7 +199,7 @@ int32_t ztcp_page_mass(const ztcp_kv_cache* cache, const ztcp_queries* queries, 
   const int sms = sm_count();
   if (sms <= 0) return launched("ztcp_page_mass") != ZTCP_OK ? ZTCP_ECUDA : set_last_error(ZTCP_ECUDA, "no CUDA device");
   const bool tc = ztcp::page_mass_tc_fits(P.c);
-  if (workspace_bytes < (tc ? ztcp::page_mass_tc_workspace(P.c, sms) : 16)) return invalid("workspace smaller than ztcp_page_mass_workspace_bytes");
+  if (workspace_bytes < (tc ? ztcp::page_mass_tc_workspace(P.c, P.c.group * queries->max_q_len, sms) : 16)) return invalid("workspace smaller than ztcp_page_mass_workspace_bytes");
   P.c.status = status;
   P.lse = lse;
   P.mass = mass;

@@ -3,8 +3,12 @@
 // The mathematics is that of ztcp_mass.cu: weights exp(scale * q.k - lse) summed over rows, heads and a page's keys.
 //   S^T[128 keys, N rows] = K Q^T   (tcgen05.mma, keys on the 128 lanes)
 // puts a key's weights into one thread, which adds them up over the columns; a warp's 32 keys (or a smaller page's)
-// are then one segment, whose sum goes to the workspace per KV head.  page_mass_join_kernel adds a page's segments
-// and heads in a fixed order, so there are no atomics and results repeat bit for bit.
+// are then one segment, whose sum goes to the workspace per KV head.  With 256 rows the product is turned over,
+//   S[2 x 128 rows, 128 keys] = Q K^T   (rows on the lanes)
+// so that a thread's lse is a register (read from shared memory for every column it took the bandwidth that the
+// products need: 87 us, now 80, for windows of 64 tokens of four sequences, 32 heads over 84,800 keys); a warp adds its 32
+// rows up by shuffles, segment by segment.  page_mass_join_kernel adds a page's segments and heads in a fixed order,
+// so there are no atomics and results repeat bit for bit.
 //
 // Accuracy.  The exponent is formed as fma(s, scale, -lse) -- one rounding of a value that is small wherever the
 // weight is not -- and only then multiplied by log2 e: folding log2 e into the scale would round s * scale * log2 e
@@ -12,7 +16,10 @@
 //
 // Work.  An item is one KV head of one sequence, a tile 128 of its keys times as many chunks of N rows as its queries
 // need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
-// Bound: for few rows the reading of K; for an observation window the exponentials, N x 128 a tile.
+// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 90 us, 5.6 TB/s, of
+// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (80 us, of 43 us that the special-function units need; giving a quarter or 3/8 of them to
+// the FMA pipes as a polynomial, a second warp of products, or loads of the next 32 scores under the arithmetic of these
+// were measured and gave 82 to 88 us).
 //
 // Warps.  Groups of four: sums of every other step, a thread per key, no warp waiting for another; then one for the
 // products and one for TMA (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
@@ -25,7 +32,7 @@ namespace ztcp {
 namespace {
 
 constexpr int kBars = 40;
-constexpr int kSlotSums = 4;  // sums of a segment in the workspace: by step parity and half of the columns
+constexpr int kRowSums = 8;  // sums of a segment that a step with rows on the lanes leaves: one per warp; else one in all
 
 struct MassTcParams {
   MassParams m;
@@ -36,22 +43,21 @@ struct MassTcParams {
   int32_t part_heads;    // heads of the group in a chunk
   int32_t seg_shift;     // log2 of the keys of a segment: 32, or a smaller page's
   int32_t segs;          // segments of a sequence in the workspace
-  int32_t halves;        // groups that share a step's columns
+  int32_t sums;          // sums of a segment that a step leaves in the workspace
 };
 
 template <int KG, int N>
 struct Shape {
-  // Warps of the sums: two groups of four by turns; for 256 rows, where their arithmetic is the limit, as many again,
-  // each with half of the columns (measured: see the top).
-  static constexpr int kHalves = N == 256 ? 2 : 1;
-  static constexpr int kSumWarps = 8 * kHalves;
+  static constexpr bool kRows = N == 256;                   // rows on the lanes
+  // Warps of the sums: two groups by turns, of as many warps as a step has lanes' quarters.
+  static constexpr int kSumWarps = kRows ? 16 : 8;
   static constexpr int kThreads = (kSumWarps + 2) * 32;
   static constexpr int kGroups = KG == 1 ? 1 : 2;           // column groups of a slot
   static constexpr int kSlotBytes = kGroups * kGroupBytes;
   static constexpr int kTileSlots = (KG + kGroups - 1) / kGroups;
   static constexpr int kQBytes = KG * N * 128;
   static constexpr int kQSlots = kQBytes > 32 * 1024 ? 1 : 2;
-  static constexpr int kNegBytes = 8 * N * 4;               // every warp its copy of its columns' -lse
+  static constexpr int kNegBytes = kRows ? 0 : 8 * N * 4;    // every warp its copy of its columns' -lse
   static constexpr int kRoom = (232448 - 4096 - kQSlots * kQBytes - kNegBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 8 ? kRoom : 8;
   static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kQSlots * kQBytes + kNegBytes;
@@ -83,6 +89,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
   __shared__ Job s_jobs[kJobs];  // row: chunks of the item; whole, inside: not used
+  __shared__ unsigned s_bad[16];  // a tile's boxes that lie outside the pool
   const CacheParams& c = P.m.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   volatile int* const dead = &dead_s;
@@ -133,7 +140,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     int64_t first = spot.first;
     int b = spot.seq;
     const int per_tile = kKeys / P.box.rows;
-    uint32_t kpos = 0, qpos = 0, n = 0;
+    uint32_t kpos = 0, qpos = 0, n = 0, tile = 0;
     bool ok = true;
     auto next = [&](Job* job) {  // publishes the share's next item (none: ta == tb)
       *job = Job{};
@@ -164,6 +171,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
       return true;
     };
     Job job;
+    PageRows pages;
     while (ok && (ok = next(&job)) && job.ta < job.tb) {
       auto load_q = [&](int ch) {
         const uint32_t slot = qpos % kQS;
@@ -178,13 +186,13 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         return true;
       };
       if (job.row == 1) ok = load_q(0);
+      pages.start(job.ta);
       for (int t = job.ta; ok && t < job.tb; ++t) {
-        const int j = t * kKeys + lane * P.box.rows;
-        int32_t row = P.box.pool_rows;  // past the sequence's end, or a bad page: zeros
-        if (lane < per_tile && j < job.kv_len) {
-          const int64_t r = pool_row(c, job.b, j);
-          if (r >= 0) row = (int32_t)r;
-        }
+        const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
+        // (16 tiles back everyone has read theirs: at most 8 are in the ring and 2 more in TMEM)
+        const unsigned bad = __ballot_sync(0xffffffffu, lane < per_tile && row == P.box.pool_rows && t * kKeys + (lane << P.box.shift) < job.kv_len);
+        if (lane == 0) s_bad[tile & 15] = bad;
+        ++tile;
 #pragma unroll
         for (int s = 0; s < kTS; ++s, ++kpos) {
           const uint32_t slot = kpos % kSlots;
@@ -209,7 +217,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     // ---- products: one thread ---------------------------------------------------------------------------
     if (elect_one()) {
       constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
-      const uint32_t qk = inst_desc(BF16, 128, N, false, false);
+      const uint32_t qk = inst_desc(BF16, 128, Sh::kRows ? kKeys : N, false, false);
       const uint32_t k_lo = desc_lo(ring, 16), q_lo = desc_lo(qbuf, 16);
       uint32_t kpos = 0, qpos = 0, step = 0, jobs = 0;
       bool ok = true;
@@ -234,6 +242,16 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
               if (ch == 0 && !wait(full(slot), pos / kSlots)) break;
               tc_fence_after();
               const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), q = q_lo + qslot * (Sh::kQBytes >> 4), d = tmem + buf * N;
+              if constexpr (Sh::kRows) {
+                const bool two = (P.parts == 1 ? (job.q_len - ch * P.chunk_tokens) * (int64_t)c.group : c.group - ch % P.parts * N) > 128;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (h == 0 || two)
+#pragma unroll
+                    for (int k = 0; k < KG * 4; ++k)
+                      mma_ss(d + h * 128, q + (((k >> 2) * N * 128 + h * 128 * 128 + (k & 3) * 32) >> 4), kHi, a + (((k >> 2) * kGroupBytes + (k & 3) * 32) >> 4),
+                             kHi, qk, k > 0);
+              } else
 #pragma unroll
               for (int g = 0; g < Sh::kGroups; ++g)
                 if (s * Sh::kGroups + g < KG)
@@ -260,15 +278,112 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
       }
     }
     __syncwarp();
+  } else if constexpr (Sh::kRows) {
+    // ---- sums: a thread per row -------------------------------------------------------------------------
+    const int wg = (warp >> 2) & 1, half = warp >> 3, r = half * 128 + (tid & 127);
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N + half * 128;
+    const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
+    const int tok_in = r / P.part_heads, head_in = r - tok_in * P.part_heads;
+    uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
+    Job job;
+    bool ok = true;
+    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
+      const int chunks = job.row;
+      float neg = -INFINITY;  // -lse; -inf where the row adds nothing
+      int lim = 0, clear = 0;  // keys that the row sees, and that all of the warp's rows see
+      bool any = false;        // a row of the warp adds something
+      auto load_row = [&](int ch) {
+        const int tok = ch / P.parts * P.chunk_tokens + tok_in, g = ch % P.parts * N + head_in;
+        neg = -INFINITY;
+        if (tok_in < P.chunk_tokens && tok < job.q_len && g < c.group) {
+          neg = -__ldg(P.m.lse + (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + g);
+          if (neg == INFINITY) neg = -INFINITY;
+        }
+        lim = neg == -INFINITY ? INT_MAX : visible_keys(c, Seq{job.kv_len, job.q_len, job.row0}, tok);
+        clear = __reduce_min_sync(0xffffffffu, lim);
+        any = __any_sync(0xffffffffu, neg != -INFINITY);
+      };
+      if (chunks == 1) load_row(0);
+      for (int t = job.ta; ok && t < job.tb; ++t, ++tile) {
+        const int j0 = t * kKeys;
+        unsigned bad = 0;
+        float total = 0.f;  // lane i: the tile's segment i
+        bool some = false;
+        for (int ch = 0; ch < chunks; ++ch, ++step) {
+          if ((step & 1) != wg) continue;
+          some = true;
+          if (chunks > 1) load_row(ch);
+          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
+          ++mine;
+          tc_fence_after();
+          bad = s_bad[tile & 15];
+          const uint64_t neg2 = pair(neg, neg);
+          auto add_block = [&](uint32_t* x, int n0) {
+            if (j0 + n0 + 32 > clear) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (j0 + n0 + i >= lim) x[i] = 0xff800000u;
+            }
+            uint64_t acc[4];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              uint64_t u = mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, neg2), log2e);
+              float a, b2;
+              unpair(u, a, b2);
+              u = pair(fast_exp2(a), fast_exp2(b2));
+              acc[i / 8] = i % 8 == 0 ? u : add2(acc[i / 8], u);
+            }
+            auto put = [&](uint64_t pr, int seg) {
+              float a, b2;
+              unpair(pr, a, b2);
+              float v = neg == -INFINITY ? 0.f : a + b2;
+#pragma unroll
+              for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+              if (lane == seg) total += v;
+            };
+            if (P.seg_shift == 5) {
+              put(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), n0 >> 5);
+            } else if (P.seg_shift == 4) {
+              put(add2(acc[0], acc[1]), n0 >> 4);
+              put(add2(acc[2], acc[3]), (n0 >> 4) + 1);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) put(acc[k], (n0 >> 3) + k);
+            }
+          };
+          if (any) {
+#pragma unroll 1
+            for (int n0 = 0; n0 < kKeys; n0 += 32) {
+              uint32_t x[32];
+              tmem_ld32(ts + n0, x);
+              tmem_ready32(x);
+              if (n0 + 32 == kKeys) {  // S has been read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_read + 8 * wg);
+              }
+              add_block(x, n0);
+            }
+          } else {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read + 8 * wg);
+          }
+        }
+        if (!ok) break;
+        const int seg = (j0 >> P.seg_shift) + lane;
+        if (some && lane < kKeys >> P.seg_shift && seg << P.seg_shift < job.kv_len) {
+          if (bad >> (lane << P.seg_shift >> P.box.shift) & 1) total = 0.f;
+          P.m.part[(((int64_t)((chunks > 1 ? kRowSums * wg : 0) + half * 4 + (warp & 3)) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + seg] = total;
+        }
+      }
+    }
   } else {
     // ---- sums: a thread per key -------------------------------------------------------------------------
-    constexpr int kOwn = N / Sh::kHalves;  // columns of a group
-    const int wg = (warp >> 2) & 1, half = warp >> 3, key = tid & 127;
-    const int col0 = half * kOwn;
-    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N + col0;
-    float* const neg = negs + warp * kOwn;
+    const int wg = warp >> 2, key = tid & 127;
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N;
+    float* const neg = negs + warp * N;
     const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
-    uint32_t step = 0, mine = 0, jobs = 0;
+    uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
     bool ok = true;
     while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
@@ -279,8 +394,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         __syncwarp();
         bool inf = false;
 #pragma unroll 1
-        for (int i = lane; i < kOwn; i += 32) {
-          const int r = col0 + i, t = r / P.part_heads, tok = ch / P.parts * P.chunk_tokens + t, g = ch % P.parts * N + r - t * P.part_heads;
+        for (int i = lane; i < N; i += 32) {
+          const int r = i, t = r / P.part_heads, tok = ch / P.parts * P.chunk_tokens + t, g = ch % P.parts * N + r - t * P.part_heads;
           float x = -INFINITY;
           if (t < P.chunk_tokens && tok < job.q_len && g < c.group) {
             x = -__ldg(P.m.lse + (job.row0 + tok) * (int64_t)(c.kv_heads * c.group) + job.head * c.group + g);
@@ -292,9 +407,9 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         none = __any_sync(0xffffffffu, inf);
       };
       if (chunks == 1) load_neg(0);
-      for (int t = job.ta; ok && t < job.tb; ++t) {
+      for (int t = job.ta; ok && t < job.tb; ++t, ++tile) {
         const int j = t * kKeys + key;
-        const bool there = j < job.kv_len && pool_row(c, job.b, j) >= 0;
+        bool there = false;
         float sum = 0.f;
         bool some = false;
         for (int ch = 0; ch < chunks; ++ch, ++step) {
@@ -303,37 +418,20 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           if (chunks > 1) load_neg(ch);
           const int tok0 = ch / P.parts * P.chunk_tokens;
           const int valid = P.parts == 1 ? min(P.chunk_tokens, job.q_len - tok0) * c.group : min(N, c.group - ch % P.parts * N);  // the chunk's rows
-          const int mine_valid = valid - col0;  // of them, in this group's columns: those below this
           // token i of the chunk sees key j when j < kv_len - q_len + tok0 + i + 1: rows from `from` on
-          const int from = (c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0) - col0;
+          const int from = (c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0);
           if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
           ++mine;
           tc_fence_after();
+          there = j < job.kv_len && !(s_bad[tile & 15] >> (key >> P.box.shift) & 1);
           uint64_t acc0 = pair(0.f, 0.f), acc1 = acc0;
           constexpr int kBlock = N < 32 ? N : 32;
-          // columns [n0, n0 + kBlock); of eight pairs, three exponentials go to the FMA pipes (measured: see the top)
-          auto add_block = [&](const uint32_t* x, int n0) {
-            if (n0 >= mine_valid) return;
-            const bool whole = !none && n0 + kBlock <= mine_valid && __all_sync(0xffffffffu, from <= n0);
-            if (whole && N >= 64) {
-#pragma unroll
-              for (int i = 0; i < kBlock; i += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
-                uint64_t u = mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, pair(w.x, w.y)), log2e);
-                uint64_t v = mul2(fma2(pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, pair(w.z, w.w)), log2e);
-                float a, b2;
-                if (i % 16 == 4) u = exp2_poly(u);
-                else unpair(u, a, b2), u = pair(fast_exp2(a), fast_exp2(b2));
-                if (i % 8 == 0) v = exp2_poly(v);
-                else unpair(v, a, b2), v = pair(fast_exp2(a), fast_exp2(b2));
-                acc0 = add2(acc0, u);
-                acc1 = add2(acc1, v);
-              }
-              return;
-            }
+          auto add_block = [&](const uint32_t* x, int n0) {  // columns [n0, n0 + kBlock)
+            if (n0 >= valid) return;
+            const bool whole = !none && n0 + kBlock <= valid && __all_sync(0xffffffffu, from <= n0);
 #pragma unroll
             for (int i = 0; i < kBlock; i += 4) {
-              if (N < 32 && i >= mine_valid) break;
+              if (N < 32 && i >= valid) break;
               const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
               float a, b2, d, e;
               unpair(mul2(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, pair(w.x, w.y)), log2e), a, b2);
@@ -344,10 +442,10 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
               e = fast_exp2(e);
               if (!whole) {
                 const int r = n0 + i;
-                a = r >= from && r < mine_valid ? a : 0.f;
-                b2 = r + 1 >= from && r + 1 < mine_valid ? b2 : 0.f;
-                d = r + 2 >= from && r + 2 < mine_valid ? d : 0.f;
-                e = r + 3 >= from && r + 3 < mine_valid ? e : 0.f;
+                a = r >= from && r < valid ? a : 0.f;
+                b2 = r + 1 >= from && r + 1 < valid ? b2 : 0.f;
+                d = r + 2 >= from && r + 2 < valid ? d : 0.f;
+                e = r + 3 >= from && r + 3 < valid ? e : 0.f;
               }
               acc0 = add2(acc0, pair(a, b2));
               acc1 = add2(acc1, pair(d, e));
@@ -367,27 +465,16 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
             }
             release();
             add_block(x, 0);
-          } else if constexpr (Sh::kHalves == 2) {
-#pragma unroll 1
-            for (int n0 = 0; n0 < kOwn; n0 += 32) {
-              uint32_t x[32];
-              tmem_ld32(ts + n0, x);
-              tmem_ready32(x);
-              const bool more = n0 + 32 < kOwn && n0 + 32 < mine_valid;
-              if (!more) release();
-              add_block(x, n0);
-              if (!more) break;
-            }
           } else {  // one block's loads under the other's arithmetic
             uint32_t x[32], y[32];
             tmem_ld32(ts, x);
 #pragma unroll 1
-            for (int n0 = 0; n0 < kOwn; n0 += 64) {
+            for (int n0 = 0; n0 < N; n0 += 64) {
               tmem_ready32(x);
               tmem_ld32(ts + n0 + 32, y);
               add_block(x, n0);
               tmem_ready32(y);
-              const bool more = n0 + 64 < kOwn && n0 + 64 < mine_valid;
+              const bool more = n0 + 64 < N && n0 + 64 < valid;
               if (more) tmem_ld32(ts + n0 + 64, x);
               else release();
               add_block(y, n0 + 32);
@@ -405,7 +492,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           const int seg = 1 << P.seg_shift;
           for (int d = seg >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
           if ((lane & (seg - 1)) == 0 && j < job.kv_len)
-            P.m.part[(((int64_t)(chunks > 1 ? 2 * wg + half : half) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + (j >> P.seg_shift)] = sum;
+            P.m.part[(((int64_t)(chunks > 1 ? wg : 0) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + (j >> P.seg_shift)] = sum;
         }
       }
     }
@@ -448,9 +535,9 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
   float sum = 0.f;
   const int64_t s0 = (int64_t)p * c.page_tokens >> P.seg_shift;
   for (int slot = 0; slot < slots; ++slot)
-    for (int half = 0; half < P.halves; ++half)
+    for (int k0 = 0; k0 < P.sums; ++k0)
       for (int h = sub; h < c.kv_heads; h += 8) {
-        const float* const q = P.m.part + (((int64_t)(2 * slot + half) * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
+        const float* const q = P.m.part + (((int64_t)(P.sums * slot + k0) * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
 #pragma unroll 2
         for (int k = 0; k < n; ++k) sum += __ldcg(q + k);
       }
@@ -483,6 +570,7 @@ int chunk_rows(const CacheParams& c, int64_t rows) {
   if (c.head_dim > 256) return 32;
   return rows <= 64 || c.head_dim > 128 ? 64 : 256;
 }
+int sums_of(int n) { return n == 256 ? kRowSums : 1; }
 int seg_shift(const CacheParams& c) { return c.page_tokens >= 32 ? 5 : c.page_tokens == 16 ? 4 : 3; }
 int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_tokens >> seg_shift(c); }
 
@@ -490,8 +578,8 @@ int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_t
 
 bool page_mass_tc_fits(const CacheParams& c) { return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31); }
 
-int64_t page_mass_tc_workspace(const CacheParams& c, int sms) {
-  return (sms + 3) / 4 * 16 + kSlotSums * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+int64_t page_mass_tc_workspace(const CacheParams& c, int64_t rows, int sms) {  // sums by step parity
+  return (sms + 3) / 4 * 16 + 2 * sums_of(chunk_rows(c, rows)) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
 }
 
 bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s) {
@@ -507,7 +595,7 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   P.part_heads = m.c.group < n ? m.c.group : n;
   P.seg_shift = seg_shift(m.c);
   P.segs = (int32_t)seg_count(m.c);
-  P.halves = n == 256 ? 2 : 1;
+  P.sums = sums_of(n);
   CUtensorMap k, q;
   if (!pool_map(&k, m.c.k, m.c, bf16, P.box) || !query_map(&q, m.c, bf16, P.chunk_tokens, P.part_heads)) return false;
   if (bf16) launch_any<true>(P, n, k, q, s);

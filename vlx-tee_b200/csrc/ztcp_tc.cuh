@@ -136,28 +136,6 @@ __device__ __forceinline__ uint32_t inst_desc(bool bf16, int m, int n, bool a_mn
   return 1u << 4 | t << 7 | t << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
-// ---- 2^t -----------------------------------------------------------------------------------------------
-// 2^t of a pair on the FMA pipes, for finite t: 2^n by the exponent bits, n = round(t), and 2^f for |f| <= 1/2 by the
-// polynomial of degree 5 with the least relative error there (fitted for this; 7.5e-8, and 2.2e-7 with its fp32
-// evaluation, against 2.4e-7 of ex2.approx).  Below 2^-126 it stays there.  The special-function unit gives 16
-// exponentials a cycle and SM and is the limit where each score costs one; a share of them is moved here.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t t) {
-  float a, b;
-  unpair(t, a, b);
-  t = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t r = add2(t, pair(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's low bits are n
-  const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), t);
-  uint64_t p = fma2(pair(0.0013276471f, 0.0013276471f), f, pair(0.009675541f, 0.009675541f));
-  p = fma2(p, f, pair(0.05550713f, 0.05550713f));
-  p = fma2(p, f, pair(0.2402212f, 0.2402212f));
-  p = fma2(p, f, pair(0.69314694f, 0.69314694f));
-  p = fma2(p, f, pair(1.0000001f, 1.0000001f));
-  float x, y, m, n;
-  unpair(p, x, y);
-  unpair(r, m, n);
-  return pair(__int_as_float(__float_as_int(x) + (__float_as_int(m) << 23)), __int_as_float(__float_as_int(y) + (__float_as_int(n) << 23)));
-}
-
 // ---- pages of the tiles to come ---------------------------------------------------------------------
 // The pool rows of the next 32 boxes of a sequence, a lane each: one look at the page table serves 32 / per_tile tiles.
 // (A look per tile, 600 to 900 cycles each, was the limit of the loading warp: chunk attention took 1,880 cycles per
