@@ -316,10 +316,13 @@ __global__ void __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) attend_kernel(const
 }
 
 // Joins the partial results of the item that CTA x's share began and did not end (Cut): partial 1 of CTA x and
-// partial 0 of the CTAs behind it.  Blocks y share its rows.  A thread holds four value columns of one row; the
-// block's four groups of 64 threads take every fourth partial each, so that the loads of an item cut into many are
-// in flight together, and add up in shared memory in a fixed order.
-constexpr int kMergeThreads = 256, kMergeQuads = 64;
+// partial 0 of the CTAs behind it.  Blocks y share its rows.  A thread holds four value columns of one row.  An item cut
+// into few (a chunk's: two or three) has a thread for each, which adds up all partials; of one cut into many, the
+// block's four groups of 64 threads take every fourth partial each, so that their loads are in flight together, and add
+// up in shared memory in a fixed order.  (Measured, attention and join: groups for all, 281 us for five ragged chunks
+// and 65.5 for the latent cache of 32 sequences cut into four to eight; a thread for all, 244 and 62; but one sequence
+// of 1,021 keys cut into 19 per item 16.8 us, with groups 13.2.)
+constexpr int kMergeThreads = 256, kMergeQuads = 64, kMergeFew = 16;
 
 template <bool BF16>
 __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __grid_constant__ AttendParams P) {
@@ -354,9 +357,11 @@ __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __gri
   auto part = [&](int i) { return P.part + (int64_t)(2 * (x + i) + (i == 0 ? 1 : 0)) * P.part_floats; };
   const int quads = c.v_dim / 4;
   const int count = (P.tiled ? (rows + 7) / 8 * 8 : rows) * quads;
-  for (int base = blockIdx.y * kMergeQuads; base < count; base += gridDim.y * kMergeQuads) {
+  const bool few = n <= kMergeFew;
+  const int across_block = few ? kMergeThreads : kMergeQuads, first = few ? 0 : grp, by = few ? 1 : 4;
+  for (int base = blockIdx.y * across_block; base < count; base += gridDim.y * across_block) {
     // rows by quads; tiled partials are read as 8 rows by 4 quads a warp, whole sectors on both sides
-    const int i = base + quad;
+    const int i = base + (few ? tid : quad);
     int r, col;
     if (P.tiled) {
       const int blk = i >> 5, across = quads >> 2;
@@ -370,12 +375,12 @@ __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __gri
     if (!live) r = 0;
     float m = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = grp; k0 < n; k0 += 16) {  // four partials in flight
+    for (int k0 = first; k0 < n; k0 += 4 * by) {  // four partials in flight
       float pm[4], pl[4];
       float4 po[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int k = k0 + 4 * u;
+        const int k = k0 + by * u;
         pm[u] = -INFINITY;
         pl[u] = 0.f;
         po[u] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -399,34 +404,37 @@ __global__ void __launch_bounds__(kMergeThreads) attend_merge_kernel(const __gri
         a.w = a.w * f + po[u].w * e;
       }
     }
-    s_m[grp][quad] = m;
-    s_l[grp][quad] = l;
-    s_o[grp][quad] = a;
-    __syncthreads();
-    if (grp == 0 && live) {
-      float t = m;
+    if (!few) {
+      s_m[grp][quad] = m;
+      s_l[grp][quad] = l;
+      s_o[grp][quad] = a;
+      __syncthreads();
+      if (grp == 0) {
 #pragma unroll
-      for (int u = 1; u < 4; ++u) t = fmaxf(t, s_m[u][quad]);
-      const float z = t == -INFINITY ? 0.f : t;
-      l = 0.f;
-      a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 1; u < 4; ++u) m = fmaxf(m, s_m[u][quad]);
+        const float z = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+        a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float f = fast_exp2(s_m[u][quad] - z);
-        const float4 o = s_o[u][quad];
-        l = fmaf(s_l[u][quad], f, l);
-        a.x = fmaf(o.x, f, a.x);
-        a.y = fmaf(o.y, f, a.y);
-        a.z = fmaf(o.z, f, a.z);
-        a.w = fmaf(o.w, f, a.w);
+        for (int u = 0; u < 4; ++u) {
+          const float f = fast_exp2(s_m[u][quad] - z);
+          const float4 o = s_o[u][quad];
+          l = fmaf(s_l[u][quad], f, l);
+          a.x = fmaf(o.x, f, a.x);
+          a.y = fmaf(o.y, f, a.y);
+          a.z = fmaf(o.z, f, a.z);
+          a.w = fmaf(o.w, f, a.w);
+        }
       }
+      __syncthreads();
+    }
+    if ((few || grp == 0) && live) {
       const int tok = (cut.row + r) / c.group, gh = (cut.row + r) - tok * c.group;
       const int64_t o = (cut.row0 + tok) * (int64_t)(c.kv_heads * c.group) + cut.head * c.group + gh;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       *reinterpret_cast<uint2*>(P.out + o * c.v_dim + col) = make_uint2(pack2<BF16>(a.x * inv, a.y * inv), pack2<BF16>(a.z * inv, a.w * inv));
-      if (col == 0 && P.lse) P.lse[o] = l == 0.f ? -INFINITY : fmaf(t, 0.693147180559945f, logf(l));
+      if (col == 0 && P.lse) P.lse[o] = l == 0.f ? -INFINITY : fmaf(m, 0.693147180559945f, logf(l));
     }
-    __syncthreads();
   }
 }
 

@@ -107,6 +107,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   __shared__ int dead_s;
   __shared__ uint32_t tmem_s;
+  __shared__ unsigned s_bad[16];  // a tile's boxes that lie outside the pool
   __shared__ float4 s_max[2][2][N], s_sum[2][N];  // per group (and tile, by turns) and row: one value of each warp
   __shared__ float s_top[2][N];                   // per group and row: the maximum in use
   __shared__ float2 s_mix[2][N];                     // per row: what the groups' O count
@@ -162,7 +163,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   if (warp == kTmaWarp) {
     // ---- TMA: a tile's slots in turn through the ring; lane p fetches page p of the tile ------------
     const int per_tile = kTileKeys / P.box.rows;
-    uint32_t pos = 0;
+    uint32_t pos = 0, tile = 0;
     int64_t at;
     Spot spot;
     const SplitSpan S = locate_warp(c.n_seqs, P.a.grid, lane, [&](int b) { return seq_work(c, N, b); }, &at, &spot);
@@ -177,6 +178,10 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       pages.start(job.ta);
       for (int t = job.ta; ok && t < job.tb; ++t) {
         const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
+        // (16 tiles back everyone has read theirs: fewer than four are in the ring and two more in TMEM)
+        const unsigned bad = __ballot_sync(0xffffffffu, lane < per_tile && row == P.box.pool_rows && t * kTileKeys + (lane << P.box.shift) < job.kv_len);
+        if (lane == 0) s_bad[tile & 15] = bad;
+        ++tile;
 #pragma unroll
         for (int s = 0; s < kTS; ++s, ++pos) {
           const uint32_t slot = pos % kSlots;
@@ -342,10 +347,10 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       const uint32_t last = step + it.tb - it.ta - 1;
       for (int t = it.ta + ((int)(step & 1) ^ wg); t < it.tb; t += 2, ++mine) {
         const int j0 = t * kTileKeys, j = j0 + key;
-        const bool there = holds && j < it.kv_len && pool_row(c, it.b, j) >= 0;
         const uint32_t g = 2 * mine + wg;  // the CTA's tile
         if (!(ok = tile_wait(s_full, g))) break;
         tc_fence_after();
+        const bool there = holds && j < it.kv_len && !(s_bad[g & 15] >> (key >> P.box.shift) & 1);
         uint32_t x[N];
         tmem_ld_cols<N>(ts, x);
         if (fresh && !(ok = meet_warps())) break;  // the item's tables are written

@@ -6,7 +6,7 @@
 // are then one segment, whose sum goes to the workspace per KV head.  With 256 rows the product is turned over,
 //   S[2 x 128 rows, 128 keys] = Q K^T   (rows on the lanes)
 // so that a thread's lse is a register (read from shared memory for every column it took the bandwidth that the
-// products need: 87 us, now 80, for windows of 64 tokens of four sequences, 32 heads over 84,800 keys); a warp adds its 32
+// products need: 87 us against 80, before the join got faster, for windows of 64 tokens of four sequences, 32 heads over 84,800 keys); a warp adds its 32
 // rows up by shuffles, segment by segment.  page_mass_join_kernel adds a page's segments and heads in a fixed order,
 // so there are no atomics and results repeat bit for bit.
 //
@@ -16,10 +16,10 @@
 //
 // Work.  An item is one KV head of one sequence, a tile 128 of its keys times as many chunks of N rows as its queries
 // need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
-// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 90 us, 5.6 TB/s, of
-// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (80 us, of 43 us that the special-function units need; giving a quarter or 3/8 of them to
-// the FMA pipes as a polynomial, a second warp of products, or loads of the next 32 scores under the arithmetic of these
-// were measured and gave 82 to 88 us).
+// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 89 us, 5.7 TB/s, of
+// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (74 us, of 43 us that the
+// special-function units need; a quarter or 3/8 of them as a polynomial on the FMA pipes, a second warp of products, or
+// loads of the next 32 scores under the arithmetic of these were measured, at 2 to 8 us more).
 //
 // Warps.  Groups of four: sums of every other step, a thread per key, no warp waiting for another; then one for the
 // products and one for TMA (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
@@ -505,12 +505,12 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   }
 }
 
-// A page's weight: its segments' sums, head by head, in a fixed order.  Eight threads per page, each with every eighth
-// head, then a tree; also the status.
+// A page's weight: its segments' sums in a fixed order.  A warp per page, a lane with every 32nd sum, then a tree (eight
+// threads per page took 14 us for 2,048 pages of 128 sums); also the status.
 __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_constant__ MassTcParams P) {
   const CacheParams& c = P.m.c;
-  const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const int sub = threadIdx.x & 7;
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
   const int b = (int)(i / c.max_pages), p = (int)(i - (int64_t)b * c.max_pages);
   float before = 0.f;
   int n = 0, slots = 0;
@@ -533,17 +533,15 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
     else if (threadIdx.x % 32 == 0) c.status[s] = ZTCP_SEQ_TIMEOUT;
   }
   float sum = 0.f;
-  const int64_t s0 = (int64_t)p * c.page_tokens >> P.seg_shift;
-  for (int slot = 0; slot < slots; ++slot)
-    for (int k0 = 0; k0 < P.sums; ++k0)
-      for (int h = sub; h < c.kv_heads; h += 8) {
-        const float* const q = P.m.part + (((int64_t)(P.sums * slot + k0) * c.n_seqs + b) * c.kv_heads + h) * P.segs + s0;
-#pragma unroll 2
-        for (int k = 0; k < n; ++k) sum += __ldcg(q + k);
-      }
+  const float* const first = P.m.part + (int64_t)b * c.kv_heads * P.segs + ((int64_t)p * c.page_tokens >> P.seg_shift);
+  const int64_t per_sum = (int64_t)c.n_seqs * c.kv_heads * P.segs;
+  for (int x = lane; x < slots * P.sums * c.kv_heads * n; x += 32) {
+    const int y = x / n, k = x - y * n, z = y / c.kv_heads, h = y - z * c.kv_heads;
+    sum += __ldcg(first + z * per_sum + (int64_t)h * P.segs + k);
+  }
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (b < c.n_seqs && sub == 0) P.m.out[i] = P.m.mass ? fmaf(P.m.decay, before, sum) : sum;
+  for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (b < c.n_seqs && lane == 0) P.m.out[i] = P.m.mass ? fmaf(P.m.decay, before, sum) : sum;
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -603,7 +601,7 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   if (cudaPeekAtLastError() != cudaSuccess) return true;
   cudaLaunchConfig_t cfg = {};
   const int64_t pages = (int64_t)m.c.n_seqs * m.c.max_pages;
-  cfg.gridDim = dim3((unsigned)((pages + 31) / 32));
+  cfg.gridDim = dim3((unsigned)((pages + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
