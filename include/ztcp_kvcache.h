@@ -32,7 +32,7 @@ extern "C" {
 
 /* Status of a sequence (or of an appended token), int32: */
 #define ZTCP_SEQ_OK 0
-#define ZTCP_SEQ_BAD_LENGTH 5 /* kv_lens outside [0, max_pages * num_tokens], or q_starts not ascending within
+#define ZTCP_SEQ_BAD_LENGTH 5 /* kv_lens outside [0, max_pages * num_tokens] or beyond 2^31 - 4096, or q_starts not ascending within
                                  [0, total_rows]: clamped to that range */
 #define ZTCP_SEQ_BAD_BLOCK 6  /* a block-table entry outside the pool: its page counts as masked; append: a slot
                                  or position out of range: the token is not written */
@@ -65,7 +65,7 @@ typedef struct ztcp_queries {
   const int32_t* q_starts;  /* [n_seqs + 1], or NULL: one row per sequence (total_rows = n_seqs) */
   int64_t total_rows;
   int64_t num_heads;        /* a multiple of the KV heads; query head h reads KV head h / (num_heads / KV heads) */
-  int64_t max_q_len;        /* longest q_len to expect: chooses the kernel; any q_len is computed */
+  int64_t max_q_len;        /* longest q_len to expect (below 2^31): chooses the kernel; any q_len is computed */
   float scale;              /* of the scores */
   int32_t causal;
 } ztcp_queries;

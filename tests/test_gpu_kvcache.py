@@ -130,6 +130,47 @@ def test_large_scores():
     check_attend([500, 260], [3, 100], 64, 2, 4, 128, BF16, scale=1.0)
 
 
+@pytest.mark.parametrize("G,D,T", [(8, 128, 64), (3, 64, 16), (1, 128, 128)])
+def test_many_short_items(G, D, T):
+    """Items of a tile or two, of one and of two row tiles, many to a CTA: the next ones' tiles follow without a gap."""
+    kv, q_lens = ref.ragged(D + T, 400, 130, 60)
+    check_attend(kv, q_lens, T, 2, G, D, BF16)
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+def test_growing_scores(dtype, q_len):
+    """Every tile's scores lie far above the last's, so that each replaces the maximum, the last one's too."""
+    kv = [700, 65]
+    k, v, tables, lens = ref.make_cache(kv, 64, 1, 128, dtype, 5)
+    for b, n in enumerate(kv):
+        for j in range(n):
+            k[tables[b, j // 64], j % 64] = k[tables[b, j // 64], j % 64] * 0.125 + 6 * j / 700
+    q = queries(2 * q_len, 4, 128, dtype, 6) * 0.125 + 1
+    out, lse, status = run_attend(q, k, v, tables, lens, [q_len] * 2)
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv, [q_len] * 2, 128 ** -0.5)
+    assert not status.any()
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_broadcast_queries(q_len):
+    """Queries expanded over rows or heads (strides of 0) read as their copies do."""
+    from ztcp_b200 import kvcache
+
+    k, v, tables, lens = ref.make_cache([200, 77], 64, 2, 128, BF16, 5)
+    one = queries(1, 8, 128, BF16, 6)
+    for q in (one.expand(2 * q_len, 8, 128), one[:, :1].expand(1, 8, 128).expand(2 * q_len, 8, 128)):
+        got = run_attend(q, k, v, tables, lens, [q_len] * 2)
+        want = run_attend(q.contiguous(), k, v, tables, lens, [q_len] * 2)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        a, b = (torch.empty(tables.shape, device=DEV) for _ in range(2))
+        for x, mass in ((q, a), (q.contiguous(), b)):
+            kvcache.page_mass(x, k, tables, lens, want[1], None, mass, q_starts=ref.starts_of([q_len] * 2), max_q_len=q_len)
+        assert torch.equal(a, b)
+
+
 def test_rows_behind_the_last_sequence_stay():
     from ztcp_b200 import kvcache
 
@@ -312,6 +353,13 @@ def test_mass_bad_blocks(q_len):
     check_mass([200, 130, 64], [q_len] * 3, 64, 2, 4, 128, BF16, bad=[(0, 1), (1, 0)])
 
 
+@pytest.mark.parametrize("H,G,T,q_lens", [(1, 272, 64, [3, 1, 2]), (2, 100, 16, [7, 2, 1]), (1, 8, 8, [90, 33, 32]), (2, 7, 32, [80, 36, 37])])
+def test_mass_wide_chunks(H, G, T, q_lens):
+    """Rows beyond a chunk of 256, groups wider than one, chunks that whole tokens do not fill, bad pages among them."""
+    check_mass([300, 77, 140], q_lens, T, H, G, 64, BF16, bad=[(0, 1), (2, 0)])
+    check_mass([300, 77, 140], q_lens, T, H, G, 128, F16, causal=False, empty=False)
+
+
 def test_mass_sums_to_the_rows():
     """Without earlier weight, a sequence's pages add up to its rows times heads: every row's weights sum to 1."""
     from ztcp_b200 import kvcache
@@ -454,6 +502,22 @@ def test_select(kv, T, keep, sink, recent):
         else:
             assert got.tolist() == exp, name
     assert not sel.status.any()
+
+
+@pytest.mark.parametrize("n,keep", [(1024, 1), (1025, 500), (2048, 2047), (2049, 1), (4096, 4000), (4097, 100), (9001, 4500)])
+def test_select_page_counts(n, keep):
+    """Page counts about what a CTA holds at once; weights in a narrow range, all alike, and of every size."""
+    from ztcp_b200 import kvcache
+
+    g = torch.Generator().manual_seed(n)
+    mass = torch.stack([1 + torch.rand(n, generator=g) / 4096, torch.full((n,), 0.5), torch.randn(n, generator=g).exp() ** 8])
+    tables = torch.randint(0, 1 << 20, (3, n), generator=g, dtype=torch.int32)
+    lens = [n, n - 1, n]
+    want = ref.select(mass.numpy(), tables, lens, 1, keep, 1, 1)
+    sel = kvcache.select_cold_pages(mass.to(DEV), tables.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                    page_tokens=1, keep=keep, sink=1, recent=1)
+    for got, exp, name in zip(sel, want, sel._fields):
+        assert torch.equal(got.cpu(), torch.tensor(exp, dtype=got.dtype).view(got.shape)), name
 
 
 def test_select_clamps_lengths():

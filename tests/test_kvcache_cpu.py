@@ -62,6 +62,7 @@ CACHE_REFUSALS = [
     ({}, dict(q_starts=None), "without q_starts there is one row per sequence"),
     ({}, dict(num_heads=12), "query heads must be a multiple of the KV heads"),
     ({}, dict(max_q_len=0), "max_q_len must be positive"),
+    ({}, dict(max_q_len=1 << 60), "max_q_len must be below 2^31"),
     ({}, dict(scale=0.0), "scale must be positive and finite"),
     ({}, dict(scale=float("nan")), "scale must be positive and finite"),
     ({}, dict(scale=float("inf")), "scale must be positive and finite"),

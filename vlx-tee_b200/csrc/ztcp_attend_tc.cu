@@ -7,20 +7,24 @@
 // boxes of tokens x group.  S, P and O live in TMEM: per row tile two buffers of 64 scores, each overwritten by its own
 // P, and O; the two row tiles fill its 512 columns.
 //
-// Warps.  0-3 and 4-7: the softmax of row tiles 0 and 1, a thread per row; 8: one thread issues the products; 9: TMA.
-// With two buffers the scores of a row tile's next 64 keys are there when it has finished with these, so that the
-// exponentials and the products run side by side:
-//   tensor core   PV0(u) QK0(u+2) PV1(u) QK1(u+2) | PV0(u+1) QK0(u+3) ...
-//   softmax 0     -- S0(u+1) -- -- S0(u+2) --
-//   softmax 1     ---- S1(u+1) -- -- S1(u+2) --
-// (With tiles of 128 keys P and the next S take the same columns, and softmax and products of a row tile take turns:
-// measured 3,750 cycles for 256 x 128 scores.)  A tile's exponentials are taken under the maximum in use, without
-// looking for a new one first; only when a score has grown by more than 2^8 over it (the weights then stay below 2^8,
-// which the 16-bit types hold without loss) is the maximum replaced and O rescaled.  m, l and O are fp32.
+// Warps.  0-3 and 4-7: the softmax of row tiles 0 and 1, a thread per row; 8 and 9: one thread each issues the products
+// of row tile 0 and 1 (one for both was the limit: an SS product takes 39 cycles to issue, a wait 100); 10: TMA.  A
+// CTA's tiles pass through in a row, whatever items they belong to: stage g of the ring holds K of tile g and V of tile
+// g - 2, so that with two buffers the scores of the next 64 keys are there when a row tile's softmax has finished with
+// these, also where an item ends:
+//   tensor core   PV(g) QK(g+2) | PV(g+1) QK(g+3) ...     (for each row tile)
+//   softmax       -- S(g+1) ---- -- S(g+2) ------
+// (With tiles of 128 keys P and the next S take the same columns, and softmax and products take turns: 3,750 cycles per
+// 256 x 128 scores.)  A tile's exponentials are taken under the maximum in use, without looking for a new one first;
+// only when a score has grown by more than 2^8 over it (the weights then stay below 2^8, which the 16-bit types hold
+// without loss) is the maximum replaced and O rescaled.  m, l and O are fp32.
 //
-// Bound.  Per 256 x 128 scores the tensor core needs 2,560 cycles (head_dim 128: products of 64 keys read Q at the limit
-// of shared memory's 128 bytes a cycle, else they would need 2,048) and the exponentials 2,048 of the
-// special-function unit's 16 a cycle.
+// Bound.  Per 256 x 64 scores the tensor core needs 1,260 cycles (head_dim 128; products of 64 keys read Q at the limit of
+// shared memory's 128 bytes a cycle, else they would need 1,024), the exponentials 1,024 of the special-function units'
+// 16 a cycle, in a thread's chain of score loads, exponentials and P stores that takes 1,590 when both row tiles are in
+// it; together 1,800 were measured.  2,048 new tokens over 32,768 keys, 32 heads of 128: 1,100 us, 970 TFLOP/s (the GPU
+// runs at 1.35 to 1.7 GHz then, as its power allows); five ragged chunks of up to 777 tokens over 800 to 8,192 keys:
+// 244 us, 720 TFLOP/s.
 //
 // Work.  As in ztcp_attend.cu the items form one line that the CTAs (one per SM) share evenly, in units of
 // keys x group (Line); attend_merge_kernel joins items that several CTAs share.

@@ -186,7 +186,8 @@ struct Seq {
 };
 __device__ __forceinline__ Seq load_seq(const CacheParams& c, int b) {
   Seq s;
-  const int64_t cap = (int64_t)c.max_pages * c.page_tokens;
+  // (tiles that end behind the last token have to fit 32 bits)
+  const int64_t cap = min((int64_t)c.max_pages * c.page_tokens, (int64_t)INT32_MAX - 4095);
   const int32_t n = __ldg(c.kv_lens + b);
   s.kv_len = n < 0 ? 0 : ((int64_t)n > cap ? (int32_t)cap : n);
   int64_t r0 = b, r1 = b + 1;
