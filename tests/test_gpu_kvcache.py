@@ -171,6 +171,26 @@ def test_broadcast_queries(q_len):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("hint", [1, 4, 16, 1000])
+def test_any_length_is_computed(hint):
+    """max_q_len chooses the kernel; rows beyond it, and fewer, come out right with every kernel."""
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = [300, 70, 0, 513], [90, 1, 0, 17]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 5)
+    q = queries(sum(q_lens), 8, 128, BF16, 6)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    mass = torch.empty(tables.shape, device=DEV)
+    kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=ref.starts_of(q_lens), max_q_len=hint)
+    kvcache.page_mass(q, k, tables, lens, lse, None, mass, q_starts=ref.starts_of(q_lens), max_q_len=hint)
+    torch.cuda.synchronize()
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv, q_lens, 128 ** -0.5, True)
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+    want, tol = ref.mass(cpu(q), cpu(k), cpu(tables), kv, q_lens, cpu(lse), None, 1.0, 128 ** -0.5, True)
+    ref.assert_close(mass, want, tol, "mass")
+
+
 def test_rows_behind_the_last_sequence_stay():
     from ztcp_b200 import kvcache
 

@@ -31,7 +31,8 @@ struct CacheParams {
   int32_t head_dim, v_dim, v_col;
   int32_t causal;
   float scale;
-  float scale_log2;  // scale * log2(e): scores enter exp2
+  float scale_more;  // what a score of the tensor cores is small by, times the scale
+  float scale_log2;  // (scale + scale_more) * log2(e): scores enter exp2
   int32_t* status;
 };
 

@@ -40,8 +40,9 @@ bool bad_rows(const void* p, int64_t token_stride, int64_t head_stride) {
 // its last bit, once per product of 16 columns.  Measured on normally distributed queries and keys against 64 bits, the
 // same in every kernel here (mma.sync and tcgen05): 0.30 (n + 1) units of 2^-24 after n products in fp16 (0.60, 0.91,
 // 1.52, 2.64, 5.08, 10.8 for n = 1, 2, 4, 8, 16, 36), 0.235 n in bf16, whose products have fewer bits to drop (0.22,
-// 0.49, 0.97, 1.76, 3.69, 8.5).  Exponents of 9 lost 1.4e-6 of their weight to it at a head_dim of 128; the scale takes
-// it back to within its own rounding.
+// 0.49, 0.97, 1.76, 3.69, 8.5).  Exponents of 9 lost 1.4e-6 of their weight to it at a head_dim of 128.  Attention's
+// scale takes it back to within its own rounding; page weights, which nothing rounds to 16 bits, add it in a step of
+// its own.
 double mean_loss(int head_dim, bool bf16) {
   const int n = (head_dim + 15) / 16;
   return (bf16 ? 0.235 * n : 0.30 * (n + 1)) * 0x1p-24;
@@ -93,9 +94,10 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   c->v_col = k->v_pool ? 0 : (int32_t)g.rope_dim;
   c->v_dim = c->head_dim - c->v_col;
   c->causal = q->causal != 0;
-  const double scale = q->scale * (1 + mean_loss(c->head_dim, k->dtype == ZTCP_DTYPE_BF16));
-  c->scale = (float)scale;
-  c->scale_log2 = (float)(scale * 1.4426950408889634);
+  const double loss = mean_loss(c->head_dim, k->dtype == ZTCP_DTYPE_BF16);
+  c->scale = q->scale;
+  c->scale_more = (float)(q->scale * loss);
+  c->scale_log2 = (float)(q->scale * (1 + loss) * 1.4426950408889634);
   return ZTCP_OK;
 }
 

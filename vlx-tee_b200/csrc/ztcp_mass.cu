@@ -2,7 +2,8 @@
 //
 // Mathematics.  out[b, p] = decay * mass[b, p] + sum over rows r, heads and tokens j of page p of
 // exp(s_rj - lse_r): with the log-sum-exp known, weights need one product and no second pass.  (s - lse is formed by
-// one fma and then multiplied by log2 e, so that it is rounded once, as a small number.)
+// one fma, corrected by a second for the accumulator's mean loss, and then multiplied by log2 e, so that it is rounded
+// as a small number.)
 //
 // Work.  A unit is as many whole pages as fit 64 keys (one, where a page is larger), of one sequence, all KV heads:
 // its sums never cross CTAs, so there are no atomics and results repeat bit for bit.  Units of all sequences form
@@ -157,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
           const int r = rg * 16 + n * 8 + 2 * t4 + e;
           const float neg = s_neg[stage][r];
           const int lim = s_lim[stage][r];
-          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale, neg) * 1.44269504088896f);
-          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale, neg) * 1.44269504088896f);
+          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale_more, fmaf(sc[n][e], c.scale, neg)) * 1.44269504088896f);
+          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale_more, fmaf(sc[n][2 + e], c.scale, neg)) * 1.44269504088896f);
         }
     }
 
