@@ -232,8 +232,12 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ ztc
 // and with one chunk a lane the norm's weights stay in registers: the instructions are the limit.  Measured:
 // 8,191 tokens of 32 + 8 + 8 vectors of 128 columns, 46.6 us, 4.3 TB/s (57 with addresses and weights looked up for every
 // vector); 4,096 of 16 + 1 of 576, 36.6 us, 4.4 TB/s.
+// CTAs per SM: with halves paired a third one's registers were not enough (spilled; 8,192 tokens 75 us, with two 58).
+template <bool INTER, int CH>
+constexpr int kStreamCtas = CH == 1 && INTER ? 3 : 2;
+
 template <bool BF16, bool INTER, int GROUP, int CH, int STAGES>
-__global__ void __launch_bounds__(256, CH == 1 ? 3 : 2) append_stream_kernel(const __grid_constant__ ztcp_append A, int32_t* status) {
+__global__ void __launch_bounds__(256, kStreamCtas<INTER, CH>) append_stream_kernel(const __grid_constant__ ztcp_append A, int32_t* status) {
   extern __shared__ uint4 ring[];  // [STAGES][CH][256], then the angles [2][4][256]
   constexpr int kPer = 32 / GROUP;
   const int tid = threadIdx.x, lane = tid % GROUP, sub = tid % 32 / GROUP;
@@ -371,13 +375,15 @@ __global__ void __launch_bounds__(256, CH == 1 ? 3 : 2) append_stream_kernel(con
   }
 }
 
-// Streams when every warp of a full grid gets several steps.
+// Streams when every warp of a full grid gets enough steps for its start.  Measured, few against many tokens' kernel: 32 + 8
+// + 8 vectors of 128, halves paired, 1,024 tokens 13.7 / 13.9 us, 2,048 24.7 / 20.9 (neighbours paired 10.5 / 10.3 and
+// 20.0 / 16.9); 8 + 8 + 8 of 64, 2,048 tokens 8.2 / 9.6, 4,096 17.1 / 15.5; 16 + 1 of 576, 512 tokens 11.8 / 8.6.
 template <bool BF16, bool INTER, int GROUP, int CH, int STAGES>
 void launch_one(const ztcp_append& A, int32_t* status, int sms, cudaStream_t s) {
   const int64_t vectors = (A.q ? A.num_q_heads : 0) + (A.v ? 2 : 1) * A.geom.num_heads;
   const int64_t steps = A.n_tokens * ((vectors + 32 / GROUP - 1) / (32 / GROUP));
-  constexpr int kPerSm = CH == 1 ? 3 : 2;
-  if (steps >= (int64_t)sms * kPerSm * 8 * 4) {
+  constexpr int kPerSm = kStreamCtas<INTER, CH>, kDeep = CH == 1 ? 10 : 3;
+  if (steps >= (int64_t)sms * kPerSm * 8 * kDeep) {
     constexpr int smem = (STAGES * CH + 8) * 256 * 16;
     auto* const k = append_stream_kernel<BF16, INTER, GROUP, CH, STAGES>;
     cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
