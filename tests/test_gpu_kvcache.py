@@ -623,3 +623,42 @@ def test_append_attend_mass_select_egress_ingress():
     kvcache.attend_pages(q1, kp, vp, restored, lens, o1)
     want, _, tol, _ = ref.attend(cpu(q1), cpu(kp), cpu(vp), cpu(restored), prompts, [1, 1], q_scale)
     ref.assert_close(o1, want, tol, "restored")
+
+
+def test_cold_pages_through_the_staging_ring():
+    """Selection -> store_cold -> load: the chosen pages, by sequence and page, come back as their own blobs' decode."""
+    import test_gpu_hooks as hooks
+    from ztcp_b200 import kvcache
+    from ztcp_b200.cold_page_spec import ColdPageGeometry
+    from ztcp_b200.hooks import CompactStagingRing, HiCachePageCodec
+    from ztcp_b200.keyring import SessionKeyRing
+    from ztcp_b200.session import ColdPageCodec
+
+    ring = SessionKeyRing(b"h" * 32)
+    hc = HiCachePageCodec(ColdPageCodec(ColdPageGeometry(num_tokens=64, num_kv_heads=8, head_dim=128, rope_dim=64), ring, DEV),
+                          CompactStagingRing(32, 98352))
+    k, v, tables, lens = ref.make_cache([640, 100, 300], 64, 8, 128, BF16, 3)
+    k, v = k.nan_to_num(nan=0.0), v.nan_to_num(nan=0.0)  # unused rows of the pages are encrypted as well
+    P = tables.shape[1]
+    mass = torch.rand(tables.shape, generator=torch.Generator().manual_seed(4)).to(DEV)
+    hashes = torch.arange(3 * P, device=DEV).view(3, P) * 7919 + 11
+    sel = kvcache.select_cold_pages(mass, tables, lens, page_tokens=64, keep=3)
+    n = int(sel.cold_starts[-1])
+    assert n == 9
+    view = hc.store_cold(sel, k, v, hashes, "tenant-h", "s", hooks._aad(ring.next_sequence_nonce("tenant-h", "s", n)))
+    got_k, got_v = (torch.empty((n, 64, 8, 128), dtype=F16, device=DEV) for _ in range(2))
+    assert hc.load(view, got_k, got_v, "tenant-h", "s", "model-h", 9).all()
+    blocks = torch.tensor([int(tables[i // P, i % P]) for i in sel.cold_index[:n].tolist()], device=DEV)
+    assert blocks.tolist() == sel.cold_blocks[:n].tolist()
+    again = hc.store(k[blocks], v[blocks], hashes.view(-1)[sel.cold_index[:n].long()], "tenant-h", "s",
+                     hooks._aad(ring.next_sequence_nonce("tenant-h", "s", n)))
+    want_k, want_v = torch.empty_like(got_k), torch.empty_like(got_v)
+    assert hc.load(again, want_k, want_v, "tenant-h", "s", "model-h", 9).all()
+    assert torch.equal(got_k, want_k) and torch.equal(got_v, want_v)
+    with pytest.raises(RuntimeError, match="page_token_hashes must have the block tables' shape"):
+        hc.store_cold(sel, k, v, hashes[:2], "tenant-h", "s", hooks._aad(1))
+    with pytest.raises(RuntimeError, match="block_tables entries must lie in"):
+        hc.store_cold(sel, k[:1], v[:1], hashes, "tenant-h", "s", hooks._aad(1))
+    none = kvcache.select_cold_pages(mass, tables, lens, page_tokens=64, keep=100)
+    with pytest.raises(RuntimeError, match="no cold page"):
+        hc.store_cold(none, k, v, hashes, "tenant-h", "s", hooks._aad(1))

@@ -16,7 +16,8 @@ freshness around every call):
 * ``HiCachePageCodec`` -- ``store`` encodes GPU pages into a view (device encode, then one asynchronous
   copy into the pinned slots; the view's ``ready`` event marks completion), ``load`` decodes a view's blobs
   back into GPU pages and returns the hit bitmap.  A page whose check fails is zeroed and reported False;
-  a shredded session makes every page a miss.
+  a shredded session makes every page a miss.  ``store_cold`` stores the pages that ``kvcache.select_cold_pages``
+  has chosen from a paged pool.
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ import torch
 
 from . import errors as _errors
 from .cold_page_spec import ColdPageAAD
+from .kvcache import ColdSelection
 from .session import ColdPageCodec
 
 
@@ -120,6 +122,25 @@ class HiCachePageCodec:
             self.ring.release(view)
             raise
         return view
+
+    def store_cold(self, sel: ColdSelection, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
+                   page_token_hashes_i64: torch.Tensor, tenant_id: str, session_id: str,
+                   aad_template: ColdPageAAD) -> StagingView:
+        """``store`` of the pages that ``kvcache.select_cold_pages`` chose, sequence by sequence as in
+        ``sel.cold_index``; page_token_hashes_i64 is [sequences, pages] like the block tables.  The pages number
+        ``int(sel.cold_starts[-1])`` (at least one; reserve as many nonces); waits for the selection."""
+        if page_token_hashes_i64.shape != sel.kept_tables.shape:
+            raise RuntimeError(f"page_token_hashes must have the block tables' shape {tuple(sel.kept_tables.shape)}")
+        n = int(sel.cold_starts[-1])
+        if n == 0:
+            raise RuntimeError("the selection holds no cold page")
+        blocks = sel.cold_blocks[:n].long()
+        lo, hi = torch.stack([blocks.min(), blocks.max()]).tolist()
+        if lo < 0 or hi >= k_pool.shape[0]:
+            raise RuntimeError(f"block_tables entries must lie in [0, {k_pool.shape[0]})")
+        hashes = page_token_hashes_i64.to(self.device).reshape(-1)[sel.cold_index[:n].long()]
+        return self.store(k_pool[blocks], None if v_pool is None else v_pool[blocks], hashes, tenant_id, session_id,
+                          aad_template)
 
     def load(self, view: StagingView, out_k_pages: torch.Tensor, out_v_pages: torch.Tensor | None,
              expected_tenant_id: str, session_id: str, expected_model_id: str, expected_layer_id: int,
