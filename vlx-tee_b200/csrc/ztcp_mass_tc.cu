@@ -17,8 +17,8 @@
 //
 // Work.  An item is one KV head of one sequence, a tile 128 of its keys times as many chunks of N rows as its queries
 // need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
-// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 89 us, 5.7 TB/s, of
-// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (74 us, of 27 us that the
+// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 91 us, 5.5 TB/s, of
+// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (73 us, of 27 us that the
 // special-function units need; a quarter or 3/8 of them as a polynomial on the FMA pipes, a second warp of products, or
 // loads of the next 32 scores under the arithmetic of these were measured, at 2 to 8 us more).
 //
