@@ -290,6 +290,38 @@ def test_prepared_call_streams_and_graph(q_lens):
     ref.assert_close(out, want, tol, "out")
 
 
+def test_calls_side_by_side():
+    """Different operators, each with its own workspace, on four streams at once, as a batch of requests runs them."""
+    from ztcp_b200 import kvcache
+
+    k, v, tables, lens = ref.make_cache([900, 70, 300, 1500], 64, 2, 128, BF16, 5)
+    one, chunk = queries(4, 8, 128, BF16, 6), queries(4 * 50, 8, 128, BF16, 7)
+    starts = ref.starts_of([50] * 4)
+    o1, o2 = torch.empty_like(one), torch.empty_like(chunk)
+    l1, l2 = (torch.empty(q.shape[:2], device=DEV) for q in (one, chunk))
+    kvcache.attend_pages(one, k, v, tables, lens, o1, lse=l1)
+    kvcache.attend_pages(chunk, k, v, tables, lens, o2, lse=l2, q_starts=starts, max_q_len=50)
+    m1, m2 = (torch.empty(tables.shape, device=DEV) for _ in range(2))
+    calls = [kvcache.prepare_attend(one, k, v, tables, lens, o1, lse=torch.empty_like(l1)),
+             kvcache.prepare_attend(chunk, k, v, tables, lens, o2, lse=torch.empty_like(l2), q_starts=starts, max_q_len=50),
+             kvcache.prepare_page_mass(one, k, tables, lens, l1, None, m1),
+             kvcache.prepare_page_mass(chunk, k, tables, lens, l2, None, m2, q_starts=starts, max_q_len=50)]
+    for c in calls:
+        c()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (o1, o2, m1, m2)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for t in (o1, o2, m1, m2):
+        t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, s in zip(calls, streams):
+            assert not c(s) is None
+    torch.cuda.synchronize()
+    for got, w in zip((o1, o2, m1, m2), want):
+        assert torch.equal(got, w)
+
+
 def test_one_shot_calls_on_another_stream():
     kv = [400, 65]
     k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
