@@ -138,8 +138,7 @@ __device__ __forceinline__ uint32_t inst_desc(bool bf16, int m, int n, bool a_mn
 
 // ---- pages of the tiles to come ---------------------------------------------------------------------
 // The pool rows of the next 32 boxes of a sequence, a lane each: one look at the page table serves 32 / per_tile tiles.
-// (A look per tile, 600 to 900 cycles each, was the limit of the loading warp: chunk attention took 1,880 cycles per
-// 64 keys with it, whatever products and exponentials took.)
+// (A look per tile costs the loading warp 600 to 900 cycles of a tile's 1,800 to 3,000.)
 struct PageRows {
   int32_t row, t0;
   __device__ __forceinline__ void start(int t) { t0 = t - 32; }  // a new item that begins with tile t
