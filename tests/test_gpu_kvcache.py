@@ -396,6 +396,47 @@ def test_mass_long_sequences(H, G, D, T, q_max, batch):
     ref.assert_close(mass, want, tol, "mass")
 
 
+@pytest.mark.parametrize("G,D,n,q_len", [(128, 576, (1 << 24) + 130, 1), (64, 64, (1 << 25) + 77, 1), (16, 128, (1 << 27) + 5, 1),
+                                         (128, 256, (1 << 24) + 1, 2)])
+def test_mass_keys_far_before_the_window(G, D, n, q_len):
+    """Keys whose distance to the window times the group passes 2^31 weigh what they should.  The table repeats a few
+    pages, so that the pool is small and a page's weight follows from its contents."""
+    from ztcp_b200 import kvcache
+
+    T, pool = 64, 5
+    g = torch.Generator().manual_seed(G)
+    k = torch.randn((pool, T, 1, D), generator=g).to(BF16).to(DEV)
+    q = queries(q_len, G, D, BF16, 3)
+    P = -(-n // T)
+    tables = (torch.arange(P, dtype=torch.int32, device=DEV) % pool)[None].contiguous()
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    scale = D ** -0.5
+    s = torch.einsum("rgd,ptd->rgpt", q.double(), k[:, :, 0].double()) * scale
+    # the log-sum-exp over the whole of the pages (the last one's unseen tokens are among 2^21 and more: left out)
+    lse = (torch.logsumexp(s.flatten(2), 2) + torch.log(torch.tensor(n / (pool * T), dtype=torch.float64))).float()
+    out = torch.empty((1, P), device=DEV)
+    status = kvcache.page_mass(q, k, tables, lens, lse, None, out, q_starts=ref.starts_of([q_len]), max_q_len=q_len,
+                               scale=scale, check_block_table=False)
+    assert not status.any()
+    size = torch.einsum("rgd,ptd->rgpt", q.double().abs(), k[:, :, 0].double().abs()) * scale
+    w = torch.exp(s - lse.double()[..., None, None])
+    e = (D + 3) * ref.U32 * size + 4 * ref.U32 * (s.abs() + lse.double().abs()[..., None, None]) + (T + q_len * G + 8) * ref.U32
+    want, tol = w.sum((0, 1, 3)), (w * e).sum((0, 1, 3))
+    whole = (n - q_len) // T  # pages that every row sees whole
+    at = torch.arange(whole, device=DEV) % pool
+    off = (out[0, :whole].double() - want[at]).abs() - tol[at] - 4 * ref.U32 * want[at]
+    assert float(off.max()) <= 0, f"page {int(off.argmax())}: {float(off.max()):.3e} beyond the bound"
+    last = torch.arange(whole * T, n, device=DEV)  # the others, token by token
+    for p in range(whole, P):
+        want_p = tol_p = 0.0
+        for j in last[last // T == p].tolist():
+            for i in range(q_len):
+                if j <= n - q_len + i:
+                    want_p += float(w[i, :, p % pool, j % T].sum())
+                    tol_p += float((w * e)[i, :, p % pool, j % T].sum())
+        assert abs(float(out[0, p]) - want_p) <= tol_p + 4 * ref.U32 * want_p
+
+
 def test_mass_more_rows_than_tokens():
     check_mass([3, 10], [40, 200], 16, 1, 4, 64, F16)
 

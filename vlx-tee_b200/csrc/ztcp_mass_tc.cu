@@ -420,8 +420,10 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           if (chunks > 1) load_neg(ch);
           const int tok0 = ch / P.parts * P.chunk_tokens;
           const int valid = P.parts == 1 ? min(P.chunk_tokens, job.q_len - tok0) * c.group : min(N, c.group - ch % P.parts * N);  // the chunk's rows
-          // token i of the chunk sees key j when j < kv_len - q_len + tok0 + i + 1: rows from `from` on
-          const int from = (c.causal ? max(0, (j - (job.kv_len - job.q_len + tok0)) * c.group) : 0);
+          // token i of the chunk sees key j when j < kv_len - q_len + tok0 + i + 1: rows from `from` on.  (Clamped to the
+          // chunk's tokens first: a key far before the window times a wide group does not fit 32 bits.)
+          const int unseen = c.causal ? min(max(j - (job.kv_len - job.q_len + tok0), 0), P.chunk_tokens) : 0;
+          const int from = unseen * c.group;
           if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
           ++mine;
           tc_fence_after();
