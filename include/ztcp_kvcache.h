@@ -66,7 +66,7 @@ typedef struct ztcp_queries {
   int64_t total_rows;
   int64_t num_heads;        /* a multiple of the KV heads; query head h reads KV head h / (num_heads / KV heads) */
   int64_t max_q_len;        /* longest q_len to expect (below 2^31): chooses the kernel; any q_len is computed */
-  float scale;              /* of the scores */
+  float scale;              /* of the scores: positive, finite times log2(e) */
   int32_t causal;
 } ztcp_queries;
 

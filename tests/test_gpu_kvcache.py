@@ -397,7 +397,7 @@ def test_mass_long_sequences(H, G, D, T, q_max, batch):
 
 
 @pytest.mark.parametrize("G,D,n,q_len", [(128, 576, (1 << 24) + 130, 1), (64, 64, (1 << 25) + 77, 1), (16, 128, (1 << 27) + 5, 1),
-                                         (128, 256, (1 << 24) + 1, 2)])
+                                         (128, 256, (1 << 24) + 300, 2)])
 def test_mass_keys_far_before_the_window(G, D, n, q_len):
     """Keys whose distance to the window times the group passes 2^31 weigh what they should.  The table repeats a few
     pages, so that the pool is small and a page's weight follows from its contents."""
@@ -435,6 +435,25 @@ def test_mass_keys_far_before_the_window(G, D, n, q_len):
                     want_p += float(w[i, :, p % pool, j % T].sum())
                     tol_p += float((w * e)[i, :, p % pool, j % T].sum())
         assert abs(float(out[0, p]) - want_p) <= tol_p + 4 * ref.U32 * want_p
+
+
+@pytest.mark.parametrize("q_len", [1, 12, 70])
+def test_tiny_scale(q_len):
+    """A scale near the smallest fp32 makes every score 0: every token weighs the same, masked ones nothing."""
+    from ztcp_b200 import kvcache
+
+    kv = [200, 70, 300]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 5)
+    q = queries(3 * q_len, 8, 128, BF16, 6)
+    out, lse, status = run_attend(q, k, v, tables, lens, [q_len] * 3, scale=1e-39)
+    want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables), kv, [q_len] * 3, 1e-39)
+    assert not status.any()
+    ref.assert_close(lse, wl, ltol, "lse")
+    ref.assert_close(out, want, tol, "out")
+    mass = torch.empty(tables.shape, device=DEV)
+    kvcache.page_mass(q, k, tables, lens, lse, None, mass, q_starts=ref.starts_of([q_len] * 3), max_q_len=q_len, scale=1e-39)
+    want, tol = ref.mass(cpu(q), cpu(k), cpu(tables), kv, [q_len] * 3, cpu(lse), None, 1.0, 1e-39)
+    ref.assert_close(mass, want, tol, "mass")
 
 
 def test_mass_more_rows_than_tokens():

@@ -79,6 +79,16 @@ def test_attend_and_mass_refusals(lib, ckw, qkw, msg):
     assert lib.ztcp_last_error().decode() == msg
 
 
+def test_scale_too_large_for_base_2(lib):
+    """Scores enter exp2: a scale that is finite but not times log2(e) would make every score infinite."""
+    c, q = cache(), rows(scale=3e38)
+    msg = "scale must be positive and finite, times log2(e) too"
+    assert lib.ztcp_attend_pages(c, q, FAKE, None, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
+    assert lib.ztcp_last_error().decode() == msg
+    assert lib.ztcp_page_mass(c, q, FAKE, None, 1.0, FAKE, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
+    assert lib.ztcp_last_error().decode() == msg
+
+
 def test_attend_refusals(lib):
     def refuse(msg, c=None, out=FAKE, status=FAKE, ws=FAKE):
         rc = lib.ztcp_attend_pages(c or cache(), rows(), out, None, status, ws, 1 << 40, None)

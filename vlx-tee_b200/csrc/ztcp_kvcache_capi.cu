@@ -1,5 +1,6 @@
 // ztcp_kvcache_capi.cu -- host layer of include/ztcp_kvcache.h: validates arguments and launches the kernels on the
 // caller's stream.  Nothing here allocates memory or synchronizes.
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -96,8 +97,10 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   c->causal = q->causal != 0;
   const double loss = mean_loss(c->head_dim, k->dtype == ZTCP_DTYPE_BF16);
   c->scale = q->scale;
-  c->scale_more = (float)(q->scale * loss);
+  // (0 times a masked score of -inf would be a NaN, where a scale is so small that its correction rounds to 0)
+  c->scale_more = fmaxf((float)(q->scale * loss), FLT_TRUE_MIN);
   c->scale_log2 = (float)(q->scale * (1 + loss) * 1.4426950408889634);
+  if (isinf(c->scale_log2)) return invalid("scale must be positive and finite, times log2(e) too");
   return ZTCP_OK;
 }
 
