@@ -334,6 +334,131 @@ def test_one_shot_calls_on_another_stream():
         assert torch.equal(out, want)
 
 
+def long_work(stream=None):
+    """About a tenth of a second of work on a stream (default: the current one)."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)
+
+
+def left_over(sizes):
+    """Memory that the current stream's allocator hands out next, in these sizes, and that the stream overwrites with
+    ones only after its long work."""
+    torch.cuda.synchronize()
+    blocks = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(3)]
+    long_work()
+    for x in blocks:
+        x.fill_(255)
+
+
+@pytest.mark.parametrize("op", ["attend", "mass", "append", "select"])
+def test_own_buffers_while_the_current_stream_is_busy(op):
+    """A one-shot call on another stream does not take memory that the current stream's earlier work still writes; nor
+    does a prepared call that runs on one."""
+    from ztcp_b200 import kvcache
+
+    kv = [1500, 65, 900]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    q = queries(3 * 30, 8, 128, BF16, 9)
+    starts = ref.starts_of([30] * 3)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=DEV)
+    kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=starts, max_q_len=30)
+    mass = torch.rand(tables.shape, device=DEV)
+    summed = torch.empty_like(mass)
+    new = queries(8000, 2 + 2, 128, BF16, 10)
+    kp, vp = (torch.zeros((8000 // 64 + 1, 64, 2, 128), dtype=BF16, device=DEV) for _ in range(2))
+    slots = torch.arange(8000, device=DEV)
+    kw = dict(q_starts=starts, max_q_len=30, check_block_table=False)
+    if op == "attend":
+        args, once, prepare = (q, k, v, tables, lens, out), kvcache.attend_pages, kvcache.prepare_attend
+        kw["lse"] = lse
+        results = [out, lse]
+    elif op == "mass":
+        args, once, prepare = (q, k, tables, lens, lse.clone(), None, summed), kvcache.page_mass, kvcache.prepare_page_mass
+        results = [summed]
+    elif op == "append":
+        args, kw = (None, new[:, :2], new[:, 2:], kp, vp, slots, None, None, None), {}
+        once, prepare = kvcache.append_tokens, kvcache.prepare_append
+        results = [kp, vp]
+    else:
+        args, kw = (mass, tables, lens), dict(page_tokens=64, keep=4)
+        once, results = kvcache.select_cold_pages, []
+    first = once(*args, **kw)
+    torch.cuda.synchronize()
+    results += list(first) if op == "select" else [first]
+    want = [t.clone() for t in results]
+    sizes = [t.numel() * t.element_size() for t in results]
+    if op != "select":
+        sizes += [t.numel() * t.element_size() for t in prepare(*args, **kw)._own]
+    del first
+    results = results[:len(results) if op == "select" else -1]
+    side = torch.cuda.Stream(DEV)
+    for prepared in (False, True):
+        if prepared and op == "select":
+            continue
+        for t in results:
+            t.zero_()
+        left_over(sizes)
+        got = prepare(*args, **kw)(side) if prepared else once(*args, stream=side, **kw)
+        if not prepared:
+            assert not torch.cuda.current_stream().query()  # the call did not wait for the current stream
+        torch.cuda.synchronize()
+        got = list(got) if op == "select" else [*results, got]
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
+
+
+def test_prepared_call_dropped_while_it_runs():
+    """The buffers of a prepared call that another stream still runs are not handed out."""
+    from ztcp_b200 import kvcache
+
+    kv = [1500, 65, 900]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    q = queries(3, 8, 128, BF16, 9)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    kvcache.attend_pages(q, k, v, tables, lens, want)
+    call = kvcache.prepare_attend(q, k, v, tables, lens, out)
+    size = call._own[0].numel()
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    long_work(side)
+    status = call(side)
+    taken = call._own[0].data_ptr()
+    del call
+    fresh = [torch.full((size,), 255, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    assert taken not in [t.data_ptr() for t in fresh]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not status.any()
+
+
+def test_host_check_reads_in_the_calls_stream():
+    """Lengths and tables that the call's own stream has just been told to write are checked as they will be."""
+    from ztcp_b200 import kvcache
+
+    kv = [700, 65, 900]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    q = queries(3, 8, 128, BF16, 9)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    kvcache.attend_pages(q, k, v, tables, lens, want)
+    side = torch.cuda.Stream(DEV)
+    late_tables, late_lens = torch.full_like(tables, -1), torch.full_like(lens, 1 << 30)
+    torch.cuda.synchronize()
+    long_work(side)
+    with torch.cuda.stream(side):
+        late_tables.copy_(tables)
+        late_lens.copy_(lens)
+    status = kvcache.attend_pages(q, k, v, late_tables, late_lens, out, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not status.any()
+    long_work(side)
+    with torch.cuda.stream(side):
+        late_tables.fill_(-1)
+    with pytest.raises(RuntimeError, match="block_tables entries must lie"):
+        kvcache.attend_pages(q, k, v, late_tables, late_lens, out, stream=side.cuda_stream)
+    with pytest.raises(RuntimeError, match="q must have shape|must be"):  # refusals name the argument on any stream
+        kvcache.attend_pages(q[:, :, :64], k, v, tables, lens, out, stream=side)
+
+
 # ---- attention weight per page ----------------------------------------------------------------------------------
 def check_mass(kv, q_lens, T, H, G, D, dtype, *, causal=True, seed=1, decay=0.75, empty=True, bad=()):
     from ztcp_b200 import kvcache

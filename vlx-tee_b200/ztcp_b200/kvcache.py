@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import capi
-from .codec import PreparedCall, _ptr, _require_cuda
+from .codec import PreparedCall, _ptr, _require_cuda, _stream_arg, _stream_handle
 
 SEQ_OK = 0
 SEQ_BAD_LENGTH = 5  # ZTCP_SEQ_BAD_LENGTH
@@ -202,16 +202,60 @@ def _workspace(size_of, cache, queries, dev) -> torch.Tensor:
     return torch.empty(size, dtype=torch.uint8, device=dev)
 
 
-def _run_once(call: PreparedCall, stream):
-    """Enqueues a call whose own buffers die with it: memory that a stream other than the current one still uses is
-    handed back only when that stream is done with it."""
-    result = call(stream)
-    if stream is not None:
-        other = torch.cuda.ExternalStream(stream, device=call._dev) if isinstance(stream, int) else stream
-        if other != torch.cuda.current_stream(call._dev):
-            for t in call._keep:
-                if isinstance(t, torch.Tensor):
-                    t.record_stream(other)
+class _OwningCall(PreparedCall):
+    """A prepared call with buffers of its own (workspace, status, new outputs).  They come from the stream that was
+    current when it was prepared, where earlier work may still be using the memory, and may be dropped while another
+    stream runs it.  So each further stream that it runs on waits for that point once, and the buffers are handed back only
+    when all of these streams are done with them."""
+
+    __slots__ = ("_own", "_made", "_streams")
+
+    def __init__(self, fn, args, dev, keep, result, own):
+        super().__init__(fn, args, dev, keep, result)
+        with torch.cuda.device(dev):
+            self._own = own
+            self._streams = {_stream_handle(dev)}
+            self._made = None
+            if not torch.cuda.is_current_stream_capturing():
+                self._made = torch.cuda.Event()
+                self._made.record()
+
+    def __call__(self, stream=None):
+        handle = _stream_arg(self._dev, stream)
+        if handle not in self._streams:
+            self._meet(handle)
+        return super().__call__(handle)
+
+    def _meet(self, handle: int) -> None:
+        other = torch.cuda.ExternalStream(handle, device=self._dev)
+        with torch.cuda.stream(other):
+            # (a capture begins behind a synchronization, and cannot wait for work outside itself)
+            if self._made is not None and not torch.cuda.is_current_stream_capturing():
+                other.wait_event(self._made)
+        for t in self._own:
+            t.record_stream(other)
+        self._streams.add(handle)
+
+
+def _run_once(prepare, first: torch.Tensor | None, stream):
+    """Prepares and enqueues a call whose own buffers die with it, on `stream` (None: the current one) of the device of
+    `first`, an argument.  On another stream than the current one, all of it happens in that stream's order: the host's
+    check reads lengths and tables there, and the buffers are its own.  Whatever the call was given may be dropped at
+    once, and what it returns is used on the current stream: both are handed back only when both streams are done."""
+    if stream is None or not isinstance(first, torch.Tensor) or not first.is_cuda:
+        return prepare()(stream)
+    dev, handle = first.device, _stream_arg(first.device, stream)
+    if handle == _stream_handle(dev):
+        return prepare()(handle)
+    here, other = torch.cuda.current_stream(dev), torch.cuda.ExternalStream(handle, device=dev)
+    with torch.cuda.stream(other):
+        call = prepare()
+        result = call(handle)
+    for t in call._keep:
+        if isinstance(t, torch.Tensor):
+            t.record_stream(other)
+    for t in (result if isinstance(result, tuple) else (result,)):
+        t.record_stream(here)
     return result
 
 
@@ -250,13 +294,13 @@ def prepare_attend(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor |
     lib = _load()
     workspace = _workspace(lib.ztcp_attend_workspace_bytes, cache, queries, dev)
     args = (cache, queries, out.data_ptr(), _ptr(lse), status.data_ptr(), workspace.data_ptr(), workspace.numel())
-    return PreparedCall(lib.ztcp_attend_pages, args, dev, (*keep, out, lse, workspace, status), status)
+    return _OwningCall(lib.ztcp_attend_pages, args, dev, (*keep, out, lse, workspace, status), status, (workspace, status))
 
 
 def attend_pages(q, k_pool, v_pool, block_tables, kv_lens, out, *, stream=None, **kw) -> torch.Tensor:
     """Attention of packed query rows over the sequences' pages, enqueued on `stream` (default: the current
     stream); arguments as for ``prepare_attend``.  Returns status[n] int32 (device)."""
-    return _run_once(prepare_attend(q, k_pool, v_pool, block_tables, kv_lens, out, **kw), stream)
+    return _run_once(lambda: prepare_attend(q, k_pool, v_pool, block_tables, kv_lens, out, **kw), k_pool, stream)
 
 
 # ---- attention weight per page ----------------------------------------------------------------------------------
@@ -292,13 +336,14 @@ def prepare_page_mass(q: torch.Tensor, k_pool: torch.Tensor, block_tables: torch
     workspace = _workspace(lib.ztcp_page_mass_workspace_bytes, cache, queries, dev)
     args = (cache, queries, lse.data_ptr(), _ptr(mass), float(decay), out_mass.data_ptr(), status.data_ptr(),
             workspace.data_ptr(), workspace.numel())
-    return PreparedCall(lib.ztcp_page_mass, args, dev, (*keep, lse, mass, out_mass, workspace, status), status)
+    return _OwningCall(lib.ztcp_page_mass, args, dev, (*keep, lse, mass, out_mass, workspace, status), status,
+                       (workspace, status))
 
 
 def page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, *, stream=None, **kw) -> torch.Tensor:
     """Attention weight per page, enqueued on `stream` (default: the current stream); arguments as for
     ``prepare_page_mass``.  Returns status[n] int32 (device)."""
-    return _run_once(prepare_page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, **kw), stream)
+    return _run_once(lambda: prepare_page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, **kw), k_pool, stream)
 
 
 # ---- append -----------------------------------------------------------------------------------------------------
@@ -365,13 +410,13 @@ def prepare_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | No
                     n, 0 if q is None else q.shape[1], pages, max_pos, capi.geometry(T, H, D, R, v_pool is None),
                     _dtype(k_pool), int(norm_from), int(bool(interleaved)), float(eps))
     keep = (q, k, v, k_pool, v_pool, slots, positions, rope_table, q_out, q_weight, k_weight, status)
-    return PreparedCall(_load().ztcp_append_tokens, (block, status.data_ptr()), dev, keep, status)
+    return _OwningCall(_load().ztcp_append_tokens, (block, status.data_ptr()), dev, keep, status, (status,))
 
 
 def append_tokens(q, k, v, k_pool, v_pool, slots, positions, rope_table, q_out, *, stream=None, **kw) -> torch.Tensor:
     """Norm, rotation and append of new tokens, enqueued on `stream` (default: the current stream); arguments as
     for ``prepare_append``.  Returns status[n] int32 (device)."""
-    return _run_once(prepare_append(q, k, v, k_pool, v_pool, slots, positions, rope_table, q_out, **kw), stream)
+    return _run_once(lambda: prepare_append(q, k, v, k_pool, v_pool, slots, positions, rope_table, q_out, **kw), k_pool, stream)
 
 
 # ---- eviction ---------------------------------------------------------------------------------------------------
@@ -418,7 +463,7 @@ def prepare_select(mass: torch.Tensor, block_tables: torch.Tensor, kv_lens: torc
                     [("mass", mass), ("block_tables", block_tables), ("kv_lens", kv_lens)])
     block = _Selection(mass.data_ptr(), block_tables.data_ptr(), kv_lens.data_ptr(), n, P, int(page_tokens), int(keep),
                        int(sink), int(recent), *(t.data_ptr() for t in outs))
-    return PreparedCall(_load().ztcp_select_cold_pages, (block,), dev, (mass, block_tables, kv_lens, *outs), outs)
+    return _OwningCall(_load().ztcp_select_cold_pages, (block,), dev, (mass, block_tables, kv_lens, *outs), outs, (status,))
 
 
 def select_cold_pages(mass: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor, *, page_tokens: int,
@@ -429,8 +474,11 @@ def select_cold_pages(mass: torch.Tensor, block_tables: torch.Tensor, kv_lens: t
     _require_cuda("mass", mass, (torch.float32,))
     if mass.dim() != 2:
         raise RuntimeError("mass and block_tables must have the same shape [sequences, pages]")
-    n, P = mass.shape
-    ints = lambda *s: torch.empty(s, dtype=torch.int32, device=mass.device)  # noqa: E731
-    return _run_once(prepare_select(mass, block_tables, kv_lens, ints(n * P), ints(n * P), ints(n + 1), ints(n, P),
-                                    torch.empty_like(mass), ints(n), page_tokens=page_tokens, keep=keep, sink=sink,
-                                    recent=recent), stream)
+
+    def prepare():
+        n, P = mass.shape
+        ints = lambda *s: torch.empty(s, dtype=torch.int32, device=mass.device)  # noqa: E731
+        return prepare_select(mass, block_tables, kv_lens, ints(n * P), ints(n * P), ints(n + 1), ints(n, P),
+                              torch.empty_like(mass), ints(n), page_tokens=page_tokens, keep=keep, sink=sink, recent=recent)
+
+    return _run_once(prepare, mass, stream)
