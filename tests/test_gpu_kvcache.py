@@ -459,6 +459,51 @@ def test_host_check_reads_in_the_calls_stream():
         kvcache.attend_pages(q[:, :, :64], k, v, tables, lens, out, stream=side)
 
 
+def test_one_shot_calls_in_a_graph():
+    """A whole step of one-shot calls, host checks at their default, captured and replayed over new contents."""
+    from ztcp_b200 import kvcache
+
+    T, H, G, D, R = 64, 2, 4, 128, 64
+    kv = [700, 65, 300]
+    k, v, tables, lens = ref.make_cache(kv, T, H, D, BF16, 8, poison=False)
+    k0, v0 = k.clone(), v.clone()
+    fused = queries(3, H * G + 2 * H, D, BF16, 9)
+    q, new_k, new_v = fused.split([H * G, H, H], dim=1)
+    table = kvcache.rope_table(1024, R)
+    slots = torch.empty(3, dtype=torch.int64, device=DEV)
+    pos = torch.empty(3, dtype=torch.int32, device=DEV)
+    rot, out = (torch.empty((3, H * G, D), dtype=BF16, device=DEV) for _ in range(2))
+    lse, mass = torch.empty((3, H * G), device=DEV), torch.zeros(tables.shape, device=DEV)
+
+    def set_inputs(n, seed):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        pos.copy_(lens - 1)
+        slots.copy_(tables.gather(1, ((lens - 1) // T).long()[:, None])[:, 0].long() * T + (lens - 1) % T)
+        fused.copy_(queries(3, H * G + 2 * H, D, BF16, seed))
+        k.copy_(k0), v.copy_(v0), mass.zero_()
+
+    def step():
+        st = [kvcache.append_tokens(q, new_k, new_v, k, v, slots, pos, table, rot)]
+        st.append(kvcache.attend_pages(rot, k, v, tables, lens, out, lse=lse))
+        st.append(kvcache.page_mass(rot, k, tables, lens, lse, mass, mass, decay=0.5))
+        sel = kvcache.select_cold_pages(mass, tables, lens, page_tokens=T, keep=3)
+        return [out, lse, mass, k, v, *st, *sel]
+
+    set_inputs(kv, 9)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for n, seed in ((kv, 9), ([640, 1, 129], 10)):
+        set_inputs(n, seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        set_inputs(n, seed)
+        for g, w in zip(got, step()):
+            assert torch.equal(g, w)
+
+
 # ---- attention weight per page ----------------------------------------------------------------------------------
 def check_mass(kv, q_lens, T, H, G, D, dtype, *, causal=True, seed=1, decay=0.75, empty=True, bad=()):
     from ztcp_b200 import kvcache

@@ -10,10 +10,13 @@ ingress restores, and chooses the pages that leave the pool.
 The pool is the codec's: [pool_pages, T, H, D] contiguous fp16 or bf16, addressed through int32 block tables, one
 row per sequence; ``v_pool=None`` is a single-buffer (MLA) pool whose values are columns [rope_dim, D) of K.  Every
 operator has a one-shot form and a ``prepare_*`` form that checks and packs the call once (``codec.PreparedCall``);
-both enqueue on `stream` (default: the current stream) without synchronizing.  Lengths, tables, slots and positions
-are read on the device at every call and checked there before they address memory: the int32 status tensor that the
-calls return holds 0, or ``SEQ_BAD_LENGTH`` / ``SEQ_BAD_BLOCK`` for a sequence (or appended token) that had a bad
-one.  The reference has no operator of this kind (its research/baseline_codec encodes and decodes pages only).
+both enqueue on `stream` (default: the current stream).  Lengths, tables, slots and positions are read on the device at
+every call and checked there before they address memory: the int32 status tensor that the calls return holds 0, or
+``SEQ_BAD_LENGTH`` / ``SEQ_BAD_BLOCK`` for a sequence (or appended token) that had a bad one.  ``attend_pages``,
+``page_mass`` and their ``prepare_*`` forms also check lengths and tables on the host, which waits for the stream;
+``check_block_table=False`` leaves that out, and so does a stream that is being captured into a CUDA graph.  Nothing else
+synchronizes.  A batch holds at least one sequence, query row or token: an empty one is refused.  The reference has no
+operator of this kind (its research/baseline_codec encodes and decodes pages only).
 """
 from __future__ import annotations
 
@@ -146,8 +149,9 @@ def _check_pool(k_pool, v_pool) -> torch.device:
 
 def _check_tables(block_tables, kv_lens, pool_pages, page_tokens, check) -> None:
     """Host check of the entries that the lengths reach, at the cost of one synchronizing reduction.  The kernels
-    check every entry on the device as well; this turns a bad table into an exception before launch."""
-    if not check:
+    check every entry on the device as well; this turns a bad table into an exception before launch.  A stream that is
+    being captured cannot be waited for: there the device's check stands alone."""
+    if not check or torch.cuda.is_current_stream_capturing():
         return
     used = (torch.arange(block_tables.shape[1], device=block_tables.device) * page_tokens)[None] < kv_lens[:, None]
     bad = (used & ((block_tables < 0) | (block_tables >= pool_pages))).any()
