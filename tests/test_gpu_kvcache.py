@@ -924,3 +924,49 @@ def test_cold_pages_through_the_staging_ring():
     none = kvcache.select_cold_pages(mass, tables, lens, page_tokens=64, keep=100)
     with pytest.raises(RuntimeError, match="no cold page"):
         hc.store_cold(none, k, v, hashes, "tenant-h", "s", hooks._aad(1))
+
+
+def test_store_cold_waits_for_the_selections_stream():
+    """A selection on another stream, still to run when store_cold is called; selections that it must not follow."""
+    import test_gpu_hooks as hooks
+    from ztcp_b200 import kvcache
+    from ztcp_b200.cold_page_spec import ColdPageGeometry
+    from ztcp_b200.hooks import CompactStagingRing, HiCachePageCodec
+    from ztcp_b200.keyring import SessionKeyRing
+    from ztcp_b200.session import ColdPageCodec
+
+    ring = SessionKeyRing(b"h" * 32)
+    hc = HiCachePageCodec(ColdPageCodec(ColdPageGeometry(num_tokens=64, num_kv_heads=8, head_dim=128, rope_dim=64), ring, DEV),
+                          CompactStagingRing(32, 98352))
+    k, v, tables, lens = ref.make_cache([640, 100, 300], 64, 8, 128, BF16, 3, poison=False)
+    P = tables.shape[1]
+    mass = torch.rand(tables.shape, generator=torch.Generator().manual_seed(4)).to(DEV)
+    hashes = torch.arange(3 * P, device=DEV).view(3, P) * 7919 + 11
+    args = ("tenant-h", "s")
+    sel = kvcache.select_cold_pages(mass, tables, lens, page_tokens=64, keep=3)
+    want_starts, n = sel.cold_starts.clone(), int(sel.cold_starts[-1])
+    want = hc.store_cold(sel, k, v, hashes, *args, hooks._aad(ring.next_sequence_nonce("tenant-h", "s", n)))
+    want_k, want_v = (torch.empty((n, 64, 8, 128), dtype=F16, device=DEV) for _ in range(2))
+    assert hc.load(want, want_k, want_v, *args, "model-h", 9).all()
+    side = torch.cuda.Stream(DEV)
+    for stream in (side, side.cuda_stream):
+        torch.cuda.synchronize()
+        long_work(side)
+        late = kvcache.select_cold_pages(mass, tables, lens, page_tokens=64, keep=3, stream=side)
+        view = hc.store_cold(late, k, v, hashes, *args, hooks._aad(ring.next_sequence_nonce("tenant-h", "s", n)), stream=stream)
+        got_k, got_v = torch.empty_like(want_k), torch.empty_like(want_v)
+        assert hc.load(view, got_k, got_v, *args, "model-h", 9).all()
+        assert torch.equal(late.cold_starts, want_starts) and torch.equal(got_k, want_k) and torch.equal(got_v, want_v)
+
+    def refuse(match, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            hc.store_cold(sel._replace(**kw), k, v, hashes, *args, hooks._aad(1))
+
+    refuse("kv_len lies outside its block table", status=torch.tensor([0, kvcache.SEQ_BAD_LENGTH, 0], dtype=torch.int32, device=DEV))
+    refuse("cold_index entries must lie in", cold_index=sel.cold_index + 3 * P)
+    refuse("cold_index entries must lie in", cold_index=sel.cold_index - 3 * P)
+    refuse("cold_starts must end with at most", cold_starts=sel.cold_starts + 3 * P)
+    refuse("cold_starts must end with at most", cold_starts=sel.cold_starts - 3 * P)
+    live = hc.ring.free_slots
+    refuse("block_tables entries must lie in", cold_blocks=sel.cold_blocks + k.shape[0])
+    assert hc.ring.free_slots == live

@@ -26,6 +26,7 @@ import collections
 import torch
 
 from . import errors as _errors
+from .codec import _stream_arg
 from .cold_page_spec import ColdPageAAD
 from .kvcache import ColdSelection
 from .session import ColdPageCodec
@@ -125,20 +126,34 @@ class HiCachePageCodec:
 
     def store_cold(self, sel: ColdSelection, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
                    page_token_hashes_i64: torch.Tensor, tenant_id: str, session_id: str,
-                   aad_template: ColdPageAAD) -> StagingView:
+                   aad_template: ColdPageAAD, stream=None) -> StagingView:
         """``store`` of the pages that ``kvcache.select_cold_pages`` chose, sequence by sequence as in
         ``sel.cold_index``; page_token_hashes_i64 is [sequences, pages] like the block tables.  The pages number
-        ``int(sel.cold_starts[-1])`` (at least one; reserve as many nonces); waits for the selection."""
+        ``int(sel.cold_starts[-1])`` (at least one; reserve as many nonces).  ``stream``: the one that the selection was
+        enqueued on, a torch.cuda.Stream or a raw handle (default: the current stream, as for every other argument); the
+        current stream and the host wait for it.  A selection with a bad length, or whose entries lie outside the pool
+        or the tables, is refused before a page is read."""
         if page_token_hashes_i64.shape != sel.kept_tables.shape:
             raise RuntimeError(f"page_token_hashes must have the block tables' shape {tuple(sel.kept_tables.shape)}")
-        n = int(sel.cold_starts[-1])
+        if stream is not None:
+            torch.cuda.current_stream(self.device).wait_stream(
+                torch.cuda.ExternalStream(_stream_arg(self.device, stream), device=self.device))
+            for t in sel:  # used on the current stream, and perhaps dropped behind this call
+                t.record_stream(torch.cuda.current_stream(self.device))
+        n, bad = torch.stack([sel.cold_starts[-1], sel.status.ne(0).any().to(torch.int32)]).tolist()
+        if bad:
+            raise RuntimeError("the selection holds a sequence whose kv_len lies outside its block table")
         if n == 0:
             raise RuntimeError("the selection holds no cold page")
-        blocks = sel.cold_blocks[:n].long()
-        lo, hi = torch.stack([blocks.min(), blocks.max()]).tolist()
+        if not 0 < n <= sel.cold_index.numel():
+            raise RuntimeError(f"cold_starts must end with at most {sel.cold_index.numel()} pages, got {n}")
+        blocks, index = sel.cold_blocks[:n].long(), sel.cold_index[:n].long()
+        lo, hi, first, last = torch.stack([blocks.min(), blocks.max(), index.min(), index.max()]).tolist()
         if lo < 0 or hi >= k_pool.shape[0]:
             raise RuntimeError(f"block_tables entries must lie in [0, {k_pool.shape[0]})")
-        hashes = page_token_hashes_i64.to(self.device).reshape(-1)[sel.cold_index[:n].long()]
+        if first < 0 or last >= page_token_hashes_i64.numel():
+            raise RuntimeError(f"cold_index entries must lie in [0, {page_token_hashes_i64.numel()})")
+        hashes = page_token_hashes_i64.to(self.device).reshape(-1)[index]
         return self.store(k_pool[blocks], None if v_pool is None else v_pool[blocks], hashes, tenant_id, session_id,
                           aad_template)
 
