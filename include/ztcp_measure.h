@@ -1,10 +1,11 @@
 /*
  * ztcp_measure.h -- measurement entry points of the B200 ZTCP codec library (libztcp_b200.so).
  *
- * Neither has a counterpart in the reference (research/baseline_codec/csrc/fused_cold_page_cpu.cpp has no
- * GPU and no roofline).  They give a benchmark the integer ceilings of the codec's own primitives on the
+ * None has a counterpart in the reference (research/baseline_codec/csrc/fused_cold_page_cpu.cpp has no
+ * GPU and no roofline).  Two give a benchmark the integer ceilings of the codec's own primitives on the
  * GPU at hand, and the split of one codec call's time between its two kernels, so every roofline
- * fraction it reports is measured in the same run.  Not part of the drop-in boundary.
+ * fraction it reports is measured in the same run; one bounds the waits inside kernels.  Not part of the drop-in
+ * boundary.
  */
 #ifndef ZTCP_MEASURE_H
 #define ZTCP_MEASURE_H
@@ -41,6 +42,12 @@ int32_t ztcp_measure_int_peaks(void* scratch, int64_t scratch_bytes, ztcp_int_pe
  * check and before the decrypt kernel (decode) -- and then disarms it.  A call that fails before
  * launching leaves it armed.  event = NULL disarms. */
 int32_t ztcp_mark_phase(void* event);
+
+/* Sets the bound, in SM cycles, of every wait inside the kernels of ztcp_attend_pages and ztcp_page_mass that this
+ * process launches from now on, and returns the one before; 0 or less restores the default of 2e9 (about a second).
+ * A call in which a wait runs out ends, reports ZTCP_SEQ_TIMEOUT for its sequences, and leaves outputs that are not
+ * valid.  For tests of that report. */
+int64_t ztcp_wait_limit(int64_t cycles);
 
 #ifdef __cplusplus
 }

@@ -504,6 +504,91 @@ def test_one_shot_calls_in_a_graph():
             assert torch.equal(g, w)
 
 
+@pytest.fixture()
+def wait_limit():
+    from ztcp_b200 import capi
+
+    yield capi.load().ztcp_wait_limit
+    capi.load().ztcp_wait_limit(0)
+
+
+WAITING = [("attend", 1, 1, 64, None), ("attend", 1, 1, 576, 64), ("attend", 1, 40, 128, None), ("mass", 1, 1, 64, None),
+           ("mass", 1, 40, 64, None), ("mass", 1, 90, 128, None), ("mass", 1, 20, 576, None)]  # by operator and max_q_len
+
+
+@pytest.mark.parametrize("op,G,hint,D,rope", WAITING)
+def test_waits_that_run_out(wait_limit, op, G, hint, D, rope):
+    """With 65,536 sequences each CTA takes milliseconds to find its place on the line, for which its other warps wait:
+    longer than a limit of a few microseconds.  The call reports it and ends; the next one is as ever."""
+    from ztcp_b200 import kvcache
+
+    n = 1 << 16
+    g = torch.Generator(device=DEV).manual_seed(D)
+    rnd = lambda *s: torch.randn(s, generator=g, device=DEV, dtype=torch.float32).to(BF16)  # noqa: E731
+    k = rnd(64, 8, 1, D)
+    v = None if rope else rnd(64, 8, 1, D)
+    q = rnd(n, G, D)
+    tables = torch.randint(0, 64, (n, 1), generator=g, device=DEV, dtype=torch.int32)
+    lens = torch.ones(n, dtype=torch.int32, device=DEV)
+    starts = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    first = tables[:, 0].long()
+    s = (q.double() * k[first, 0].double()).sum(-1) * D ** -0.5  # one key: its score is the log-sum-exp
+    kw = dict(q_starts=starts, max_q_len=hint)
+    if op == "attend":
+        out, lse = torch.empty((n, G, D - (rope or 0)), dtype=BF16, device=DEV), torch.empty((n, G), device=DEV)
+        call = kvcache.prepare_attend(q, k, v, tables, lens, out, lse=lse, rope_dim=rope or 0, **kw)
+    else:
+        out = torch.empty((n, 1), device=DEV)
+        call = kvcache.prepare_page_mass(q, k, tables, lens, s.float(), None, out, **kw)
+    for limit in (1000, 0):
+        wait_limit(limit)
+        out.fill_(9.0)
+        status = call()
+        torch.cuda.synchronize()
+        assert bool((status == (kvcache.SEQ_TIMEOUT if limit else 0)).all())
+    if op == "attend":
+        values = k[first, 0, :, rope:] if rope else v[first, 0]
+        assert torch.equal(out, values.expand_as(out))  # the weight is 1, and the sum
+        assert bool(((lse - s).abs() <= (D + 8) * ref.U32 * (q.double().abs() * k[first, 0].double().abs()).sum(-1)).all())
+    else:  # exp of a score's error and of its rounding
+        bound = (D + 8) * ref.U32 * ((q.double().abs() * k[first, 0].double().abs()).sum(-1) * D ** -0.5 + 1)
+        assert bool(((out - 1).abs() <= 2 * bound).all())
+
+
+@pytest.mark.parametrize("limit", [1, 300, 2000, 6000, 20_000, 100_000])
+def test_waits_that_may_run_out(wait_limit, limit):
+    """Limits about what a call's waits take: all of a call's sequences report it, or none does and the results are right;
+    calls with the default limit on the same workspaces are as before."""
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = [3000, 70, 900, 1], [40, 1, 33, 1]
+    calls = []
+    for H, G, D, rope, m in ((2, 4, 128, None, 40), (2, 4, 64, None, 1), (1, 16, 576, 64, 1), (2, 8, 256, None, 1)):
+        k, v, tables, lens = ref.make_cache(kv, 64, H, D, BF16, 5, mla=rope is not None)
+        ql = q_lens if m > 1 else [1] * 4
+        q = queries(sum(ql), H * G, D, BF16, 6)
+        out, lse = torch.empty((q.shape[0], H * G, D - (rope or 0)), dtype=BF16, device=DEV), torch.empty(q.shape[:2], device=DEV)
+        mass = torch.empty(tables.shape, device=DEV)
+        kw = dict(q_starts=ref.starts_of(ql), max_q_len=m)
+        attend = kvcache.prepare_attend(q, k, v, tables, lens, out, lse=lse, rope_dim=rope or 0, **kw)
+        attend()
+        fixed = lse.clone()
+        calls += [(attend, (out, lse)), (kvcache.prepare_page_mass(q, k, tables, lens, fixed, None, mass, **kw), (mass,))]
+    want = []
+    for call, outs in calls:
+        assert not call().any()
+        want.append([t.clone() for t in outs])
+    for _ in range(5):
+        for (call, outs), w in zip(calls, want):
+            wait_limit(limit)
+            status = call().tolist()
+            assert status in ([kvcache.SEQ_TIMEOUT] * 4, [0] * 4)
+            if status[0] == 0:
+                assert all(torch.equal(a, b) for a, b in zip(outs, w))
+            wait_limit(0)
+            assert not call().any() and all(torch.equal(a, b) for a, b in zip(outs, w))
+
+
 # ---- attention weight per page ----------------------------------------------------------------------------------
 def check_mass(kv, q_lens, T, H, G, D, dtype, *, causal=True, seed=1, decay=0.75, empty=True, bad=()):
     from ztcp_b200 import kvcache

@@ -89,6 +89,13 @@ def test_scale_too_large_for_base_2(lib):
     assert lib.ztcp_last_error().decode() == msg
 
 
+def test_wait_limit(lib):
+    default = 2_000_000_000
+    assert lib.ztcp_wait_limit(500) == default
+    assert lib.ztcp_wait_limit(0) == 500
+    assert lib.ztcp_wait_limit(-1) == default and lib.ztcp_wait_limit(0) == default
+
+
 def test_attend_refusals(lib):
     def refuse(msg, c=None, out=FAKE, status=FAKE, ws=FAKE):
         rc = lib.ztcp_attend_pages(c or cache(), rows(), out, None, status, ws, 1 << 40, None)

@@ -110,7 +110,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kKS = Sh::kKSlots, kTileKeys = Sh::kTileKeys;
   constexpr int kGroupBytes = Sh::kGroupBytes, kKGroups = Sh::kGroups;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int dead_s;
+  __shared__ Waits waits_s;
   __shared__ uint32_t tmem_s;
   __shared__ unsigned s_bad[16];  // a tile's boxes that lie outside the pool
   __shared__ float4 s_max[2][2][N], s_sum[2][N];  // per group (and tile, by turns) and row: one value of each warp
@@ -121,7 +121,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
   __shared__ Job s_jobs[kJobs];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  volatile int* const dead = &dead_s;
+  volatile Waits* const waits = &waits_s;
 
   const uint32_t bars = smem_u32(smem_raw);
   const uint32_t ring = (bars + kBars * 8 + 1023) & ~1023u;
@@ -135,7 +135,8 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
                  summed = meet + 16, read = summed + 8, job_full = read + 8, job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
 
   if (tid == 0) {
-    dead_s = 0;
+    waits_s.limit = c.wait_cycles;
+    waits_s.dead = 0;
     for (int s = 0; s < kSlots; ++s) mbar_init(full(s), 1);
     mbar_init(q_full, 256);
     for (int i = 0; i < 4; ++i) {
@@ -179,7 +180,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     Job job;
     PageRows pages;
     bool ok = true;
-    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, waits, &job)) && job.ta < job.tb) {
       pages.start(job.ta);
       for (int t = job.ta; ok && t < job.tb; ++t) {
         const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
@@ -192,7 +193,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
           const uint32_t slot = pos % kSlots;
           if (pos >= kSlots) {  // the slot's last tile: its K is done with its scores, its V (or shared K) with its products
             const uint32_t was = pos - kSlots, tile = was / kTS;
-            ok = ok && mbar_wait((SHARED || was % kTS >= kKS ? pv_done : s_full) + 8 * (tile & 3), (tile >> 2) & 1, dead);
+            ok = ok && mbar_wait((SHARED || was % kTS >= kKS ? pv_done : s_full) + 8 * (tile & 3), (tile >> 2) & 1, waits);
           }
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
@@ -211,10 +212,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       }
     }
     if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
-    if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
-      int none = 0;
-      for (uint32_t p = pos > kSlots ? pos - kSlots : 0; p < pos; ++p) mbar_wait(full(p % kSlots), (p / kSlots) & 1, &none);
-    }
+    drain_fills(full(0), kSlots, pos);
   } else if (warp == kMmaWarp) {
     // ---- products: one thread ------------------------------------------------------------------------
     if (elect_one()) {
@@ -226,7 +224,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       const uint32_t k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kVLbo), q_lo = desc_lo(qbuf, 16), p_lo = desc_lo(pbuf, Sh::kPBlock);
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t n) {  // the n-th completion (from 0)
-        ok = ok && mbar_wait(bar, n & 1, dead);
+        ok = ok && mbar_wait(bar, n & 1, waits);
         return ok;
       };
       auto scores = [&](uint32_t step) {  // S^T of the CTA's tile `step`
@@ -263,7 +261,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       };
       uint32_t step = 0, items = 0;
       Job job;
-      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, items, dead, &job)) && job.ta < job.tb) {
+      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, items, waits, &job)) && job.ta < job.tb) {
         const int n = job.tb - job.ta;
         if (!wait(q_full, items - 1)) break;
         tc_fence_after();
@@ -278,11 +276,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
         }
         step += n;
       }
-      if (*dead) {  // no product may be in flight when TMEM is freed
-        int none = 0;
-        tc_commit(drain);
-        mbar_wait(drain, 0, &none);
-      }
+      drain_products(drain);
     }
     __syncwarp();
   } else {
@@ -295,19 +289,19 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     const uint32_t pdst = pbuf + wg * Sh::kPBytes + key * 32;
     const int chunks = c.head_dim / 8;
     uint32_t step = 0, mine = 0, meets = 0, nitem = 0;  // tiles of the CTA, of this group, meetings, items
-    auto tile_wait = [&](uint32_t bars, uint32_t tile) { return warp_wait(bars + 8 * (tile & 3), (tile >> 2) & 1, dead); };
+    auto tile_wait = [&](uint32_t bars, uint32_t tile) { return warp_wait(bars + 8 * (tile & 3), (tile >> 2) & 1, waits); };
     // The group's four warps meet.  Not a bar.sync, which no bound could end if a warp had left after a timeout.
     auto meet_warps = [&] {
       __syncwarp();
       if (lane == 0) mbar_arrive(meet + 8 * wg);
-      return warp_wait(meet + 8 * wg, meets++ & 1, dead);
+      return warp_wait(meet + 8 * wg, meets++ & 1, waits);
     };
     // The next item: its rows' places and limits (tables of kTurns items, by turns: a warp may be two items ahead of
     // another), and Q into shared memory.
     Job job;
     uint32_t jobs = 0;
     auto open = [&] {
-      if (!take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) return false;
+      if (!take_job(s_jobs, job_full, job_empty, jobs, lane, waits, &job)) return false;
       if (job.ta == job.tb) return true;
       if (wt < job.rows) {
         const int tok = (job.row + wt) / c.group, gh = job.row + wt - tok * c.group;
@@ -389,7 +383,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
         const bool grow = __any_sync(0xffffffffu, grows);
         // the group's product before has read P and written O; at an item's start, O has been read as well
         if (mine > 0 && !(ok = tile_wait(pv_done, g - 2))) break;
-        if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+        if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, waits))) break;
         if (!fresh && grow) {  // the same in every thread of the group
           tc_fence_after();
 #pragma unroll
@@ -422,7 +416,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
         if (j0 + kTileKeys > it.kv_len && it.kv_len % c.page_tokens != 0) {
           for (int s = SHARED ? 1 : kKS; s < kTS; ++s) {
             const uint32_t pos = g * kTS + s, slot = pos % kSlots;
-            if (!(ok = warp_wait(full(slot), (pos / kSlots) & 1, dead))) break;
+            if (!(ok = warp_wait(full(slot), (pos / kSlots) & 1, waits))) break;
             if (j >= it.kv_len && holds)
               for (int i = 0; i < kKGroups * 8; ++i)
                 asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + slot * Sh::kSlotBytes + (i >> 3) * kGroupBytes + key * 128 + (i & 7) * 16),
@@ -440,7 +434,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
 
       // The groups' maxima and sums meet in shared memory; each group then joins and writes its share of the columns
       // (one block of columns: its share of the rows).
-      if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, dead))) break;
+      if (fresh && nitem > 0 && !(ok = warp_wait(read, (nitem - 1) & 1, waits))) break;
       {
         const float sum = lane_sums<N>(l, lane);
         if (lane < N) reinterpret_cast<float*>(s_sum[wg])[4 * lane + ww] = sum;
@@ -448,7 +442,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(summed);
-      if (!(ok = warp_wait(summed, nitem & 1, dead))) break;
+      if (!(ok = warp_wait(summed, nitem & 1, waits))) break;
       float* const part = P.a.part + (int64_t)(2 * blockIdx.x + (it.inside ? 0 : 1)) * P.a.part_floats;
       if (wt < rows) {
         const float4 u = s_sum[0][wt], v = s_sum[1][wt];
@@ -506,7 +500,7 @@ attend_decode_kernel(const __grid_constant__ DecodeParams P, const __grid_consta
     }
   }
   __syncthreads();
-  if (tid == 0 && *dead) P.a.cuts[blockIdx.x].error = 1;
+  if (tid == 0 && waits->dead) P.a.cuts[blockIdx.x].error = 1;
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Sh::kCols) : "memory");

@@ -29,9 +29,9 @@
 // Work.  As in ztcp_attend.cu the items form one line that the CTAs (one per SM) share evenly, in units of
 // keys x group (Line); attend_merge_kernel joins items that several CTAs share.
 //
-// Waits are bounded: a wait that runs out (ztcp_tc.cuh) sets the CTA's error word, every role leaves
-// its loop, copies and products in flight are waited for (bounded again), TMEM is freed, and the merge kernel
-// reports ZTCP_SEQ_TIMEOUT for every sequence.
+// Waits are bounded: a wait that runs out (ztcp_tc.cuh) sets the CTA's error word, every role leaves its loop, copies
+// and products in flight are waited for (always, and bounded again: a role that has left in time cannot know that another
+// one will run out), TMEM is freed, and the merge kernel reports ZTCP_SEQ_TIMEOUT for every sequence.
 #include "ztcp_tc.cuh"
 
 namespace ztcp {
@@ -62,13 +62,13 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   constexpr int kQHalf = kItemRows * 128;      // and 64 columns of Q
   constexpr int kCols = HALVES * 64;           // head_dim rounded up
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int dead_s;
+  __shared__ Waits waits_s;
   __shared__ uint32_t tmem_s;
   __shared__ Job s_jobs[kJobs];
   __shared__ unsigned s_bad[16];
   const CacheParams& c = P.a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  volatile int* const dead = &dead_s;
+  volatile Waits* const waits = &waits_s;
 
   // barriers first, then the 1,024-byte aligned tiles
   const uint32_t raw = smem_u32(smem_raw);
@@ -82,7 +82,8 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
   static_assert(2 * SLOTS + 16 + 2 * kJobs <= kBars, "barrier slots");
 
   if (tid == 0) {
-    dead_s = 0;
+    waits_s.limit = c.wait_cycles;
+    waits_s.dead = 0;
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 2);
@@ -134,7 +135,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     // Lane p loads box p of V, of 64 columns and one page each, and lane boxes + p that of K.
     auto stage = [&](bool v_on, bool k_on, int32_t row, int32_t head) {
       const uint32_t slot = pos % SLOTS;
-      if (pos >= SLOTS && !warp_wait(empty(slot), (pos / SLOTS - 1) & 1, dead)) return false;
+      if (pos >= SLOTS && !warp_wait(empty(slot), (pos / SLOTS - 1) & 1, waits)) return false;
       if (lane == 0) mbar_expect(full(slot), (v_on ? kTile : 0) + (k_on ? kTile : 0));
       __syncwarp();
       const bool isk = lane >= boxes;
@@ -152,7 +153,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       head1 = head;
       return true;
     };
-    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, dead, &job)) && job.ta < job.tb) {
+    while (ok && (ok = pub.next(c, S, s_jobs, job_full, job_empty, lane, waits, &job)) && job.ta < job.tb) {
       pages.start(job.ta);
       for (int t = job.ta; t < job.tb; ++t) {
         const int32_t row = pages.at(c, P.box, per_tile, job.b, job.kv_len, t, lane);  // pool_rows: zeros
@@ -164,7 +165,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         if (t > job.ta) continue;
         // Q as it lies: tokens x group rows, each half of the columns [256][64] (rows past the item's are other tokens',
         // or left over; nothing of theirs is stored).  The item before needs its own Q for one tile less than V.
-        if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, dead))) break;
+        if (items > 0 && !(ok = warp_wait(q_empty, (items - 1) & 1, waits))) break;
         ++items;
         if (lane == 0) mbar_expect(q_full, HALVES * item_rows * 128);
         __syncwarp();
@@ -175,11 +176,8 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       ok = stage(pos >= 2, false, 0, 0) && stage(true, false, 0, 0);
     }
     if (lane == 0) P.a.cuts[blockIdx.x] = pub.cut;
-    if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
-      int none = 0;
-      for (uint32_t p = pos > SLOTS ? pos - SLOTS : 0; p < pos; ++p) mbar_wait(full(p % SLOTS), (p / SLOTS) & 1, &none);
-      if (items > 0) mbar_wait(q_full, (items - 1) & 1, &none);
-    }
+    drain_fills(full(0), SLOTS, pos);
+    drain_fills(q_full, 1, items);
   } else if (warp >= kMmaWarp) {
     // ---- products of row tile q: one thread ----------------------------------------------------------
     const int q = warp - kMmaWarp;
@@ -196,7 +194,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       int now = 0, next = 0, t = 0;
       bool more = true, ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
-        ok = ok && mbar_wait(bar, parity & 1, dead);
+        ok = ok && mbar_wait(bar, parity & 1, waits);
         return ok;
       };
       Job job;
@@ -204,7 +202,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       while (true) {
         int then = 0;
         if (more && t == job.tb) {
-          if (!(ok = take_job_alone(s_jobs, job_full, job_empty, njobs, dead, &job))) break;
+          if (!(ok = take_job_alone(s_jobs, job_full, job_empty, njobs, waits, &job))) break;
           more = job.ta < job.tb;
           t = job.ta;
           then = kFirst;
@@ -244,9 +242,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         now = next;
         next = then;
       }
-      int none = 0;  // no product may be in flight when TMEM is freed, after a timeout either
-      tc_commit(drain + 8 * q);
-      mbar_wait(drain + 8 * q, 0, &none);
+      drain_products(drain + 8 * q);
     }
     __syncwarp();
   } else {
@@ -258,7 +254,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
     uint32_t ends = 0, prevs = 0;  // items of this row tile, and those of more than one tile
     Job job;
     uint32_t njobs = 0;
-    auto open = [&] { return take_job(s_jobs, job_full, job_empty, njobs, lane, dead, &job); };
+    auto open = [&] { return take_job(s_jobs, job_full, job_empty, njobs, lane, waits, &job); };
     bool ok = open();
     while (ok && job.ta < job.tb) {
       const Job it = job;
@@ -277,7 +273,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       for (int t = it.ta; t < it.tb; ++t, ++step, ++mine) {
         const int j0 = t * kTileKeys;
         const uint32_t buf = mine & 1, ts = tmem + lanes + q * 128 + buf * 64;
-        if (!(ok = warp_wait(s_full + 16 * q + 8 * buf, (mine >> 1) & 1, dead))) break;
+        if (!(ok = warp_wait(s_full + 16 * q + 8 * buf, (mine >> 1) & 1, waits))) break;
         tc_fence_after();
         const unsigned bad = s_bad[step & 15];
         uint32_t x[64];
@@ -336,8 +332,8 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
             const float mn = grow ? mx : m;
             const float f = grow ? fast_exp2(m - mn) : 1.f;  // 0 for the first maximum
             if (t > it.ta) {  // O is this thread's to change between its products
-              if (t + 1 < it.tb) ok = warp_wait(s_full + 16 * q + 8 * (buf ^ 1), ((mine + 1) >> 1) & 1, dead);
-              else ok = warp_wait(pv_prev + 8 * q, prevs & 1, dead);
+              if (t + 1 < it.tb) ok = warp_wait(s_full + 16 * q + 8 * (buf ^ 1), ((mine + 1) >> 1) & 1, waits);
+              else ok = warp_wait(pv_prev + 8 * q, prevs & 1, waits);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -371,7 +367,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         const int end = it.kv_len - j0;
         if (end < kTileKeys && it.kv_len % c.page_tokens != 0) {
           const uint32_t vp = step + 2;
-          if (!(ok = warp_wait(full(vp % SLOTS), (vp / SLOTS) & 1, dead))) break;
+          if (!(ok = warp_wait(full(vp % SLOTS), (vp / SLOTS) & 1, waits))) break;
           if (wg >= end && wg < kTileKeys)
 #pragma unroll
             for (int i = 0; i < HALVES * 8; ++i)
@@ -387,7 +383,7 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
       if (!ok) break;
       if (!(ok = open())) break;
 
-      if (!(ok = warp_wait(pv_last + 8 * q, ends & 1, dead))) break;
+      if (!(ok = warp_wait(pv_last + 8 * q, ends & 1, waits))) break;
       tc_fence_after();
       ++ends;
       prevs += prev;
@@ -430,9 +426,10 @@ attend_tc_kernel(const __grid_constant__ TcParams P, const __grid_constant__ CUt
         }
       }
     }
+    tc_wait_st();  // (a wait that ran out may have left a store of P in flight)
   }
   __syncthreads();
-  if (tid == 0 && *dead) P.a.cuts[blockIdx.x].error = 1;
+  if (tid == 0 && waits->dead) P.a.cuts[blockIdx.x].error = 1;
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

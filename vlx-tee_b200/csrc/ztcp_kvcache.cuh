@@ -11,6 +11,8 @@ namespace ztcp {
 
 int32_t set_last_error(int32_t code, const std::string& msg);  // ztcp_capi.cu
 
+constexpr long long kWaitCycles = 2000000000ll;  // bound of a wait inside a kernel: a second or so
+
 // ------------------------------------------------------------------------------------------------
 // Kernel parameters
 // ------------------------------------------------------------------------------------------------
@@ -33,6 +35,7 @@ struct CacheParams {
   float scale;
   float scale_more;  // what a score of the tensor cores is small by, times the scale
   float scale_log2;  // (scale + scale_more) * log2(e): scores enter exp2
+  int64_t wait_cycles;  // bound of a wait inside a kernel
   int32_t* status;
 };
 

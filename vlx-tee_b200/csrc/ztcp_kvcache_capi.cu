@@ -4,7 +4,10 @@
 #include <math.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "../../include/ztcp_kvcache.h"
+#include "../../include/ztcp_measure.h"
 #include "ztcp_kvcache.cuh"
 
 namespace ztcp {
@@ -19,6 +22,7 @@ using ztcp::set_last_error;
 int32_t invalid(const char* msg) { return set_last_error(ZTCP_EINVAL, msg); }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 constexpr int64_t kInt32Max = 0x7fffffff;
+std::atomic<int64_t> g_wait_cycles{ztcp::kWaitCycles};
 
 int32_t check_pool(const ztcp_geometry& g, int32_t dtype, int64_t pool_pages, const void* k, const void* v) {
   if (!k) return invalid("k_pool must not be NULL");
@@ -96,6 +100,7 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   c->v_dim = c->head_dim - c->v_col;
   c->causal = q->causal != 0;
   const double loss = mean_loss(c->head_dim, k->dtype == ZTCP_DTYPE_BF16);
+  c->wait_cycles = g_wait_cycles.load(std::memory_order_relaxed);
   c->scale = q->scale;
   // (0 times a masked score of -inf would be a NaN, where a scale is so small that its correction rounds to 0)
   c->scale_more = fmaxf((float)(q->scale * loss), FLT_TRUE_MIN);
@@ -157,6 +162,10 @@ int64_t plan(Kernel k, const ztcp::CacheParams& c, const ztcp_queries* q, void* 
 }  // namespace
 
 extern "C" {
+
+int64_t ztcp_wait_limit(int64_t cycles) {
+  return g_wait_cycles.exchange(cycles > 0 ? cycles : ztcp::kWaitCycles, std::memory_order_relaxed);
+}
 
 int64_t ztcp_attend_workspace_bytes(const ztcp_kv_cache* cache, const ztcp_queries* queries) {
   ztcp::CacheParams c;

@@ -87,13 +87,13 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   using Sh = Shape<KG, N>;
   constexpr int kSlots = Sh::kSlots, kTS = Sh::kTileSlots, kQS = Sh::kQSlots, kMmaWarp = Sh::kSumWarps, kTmaWarp = kMmaWarp + 1;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int dead_s;
+  __shared__ Waits waits_s;
   __shared__ uint32_t tmem_s;
   __shared__ Job s_jobs[kJobs];  // row: chunks of the item; whole, inside: not used
   __shared__ unsigned s_bad[16];  // a tile's boxes that lie outside the pool
   const CacheParams& c = P.m.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  volatile int* const dead = &dead_s;
+  volatile Waits* const waits = &waits_s;
   const uint32_t bars = smem_u32(smem_raw);
   const uint32_t ring = (bars + kBars * 8 + 1023) & ~1023u;
   const uint32_t qbuf = ring + kSlots * Sh::kSlotBytes;
@@ -103,7 +103,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   const uint32_t q_full = bars + 2 * kSlots * 8, q_empty = q_full + 16, s_full = q_empty + 16, s_read = s_full + 16, job_full = s_read + 16,
                  job_empty = job_full + 8 * kJobs, drain = job_empty + 8 * kJobs;
   if (tid == 0) {
-    dead_s = 0;
+    waits_s.limit = c.wait_cycles;
+    waits_s.dead = 0;
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
@@ -163,7 +164,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         job->tb = (int32_t)div_pos(pos - start, m.chunks);
       }
       const uint32_t e = n % kJobs;
-      if (n >= kJobs && !warp_wait(job_empty + 8 * e, (n / kJobs - 1) & 1, dead)) return false;
+      if (n >= kJobs && !warp_wait(job_empty + 8 * e, (n / kJobs - 1) & 1, waits)) return false;
       if (lane == 0) {
         s_jobs[e] = *job;
         mbar_arrive(job_full + 8 * e);
@@ -176,7 +177,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     while (ok && (ok = next(&job)) && job.ta < job.tb) {
       auto load_q = [&](int ch) {
         const uint32_t slot = qpos % kQS;
-        if (qpos >= kQS && !warp_wait(q_empty + 8 * slot, (qpos / kQS - 1) & 1, dead)) return false;
+        if (qpos >= kQS && !warp_wait(q_empty + 8 * slot, (qpos / kQS - 1) & 1, waits)) return false;
         if (lane == 0) mbar_expect(q_full + 8 * slot, KG * P.chunk_tokens * P.part_heads * 128);
         const int first_tok = ch / P.parts * P.chunk_tokens;
         __syncwarp();
@@ -197,7 +198,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
 #pragma unroll
         for (int s = 0; s < kTS; ++s, ++kpos) {
           const uint32_t slot = kpos % kSlots;
-          if (kpos >= kSlots && !(ok = warp_wait(empty(slot), (kpos / kSlots - 1) & 1, dead))) break;
+          if (kpos >= kSlots && !(ok = warp_wait(empty(slot), (kpos / kSlots - 1) & 1, waits))) break;
           const int groups = KG - s * Sh::kGroups < Sh::kGroups ? KG - s * Sh::kGroups : Sh::kGroups;
           if (lane == 0) mbar_expect(full(slot), groups * kGroupBytes);
           __syncwarp();
@@ -209,11 +210,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           for (int ch = 0; ok && ch < job.row; ++ch) ok = load_q(ch);
       }
     }
-    if (*dead) {  // after a timeout: no copy may be in flight when the CTA ends
-      int none = 0;
-      for (uint32_t p = kpos > kSlots ? kpos - kSlots : 0; p < kpos; ++p) mbar_wait(full(p % kSlots), (p / kSlots) & 1, &none);
-      for (uint32_t p = qpos > kQS ? qpos - kQS : 0; p < qpos; ++p) mbar_wait(q_full + 8 * (p % kQS), (p / kQS) & 1, &none);
-    }
+    drain_fills(full(0), kSlots, kpos);
+    drain_fills(q_full, kQS, qpos);
   } else if (warp == kMmaWarp) {
     // ---- products: one thread ---------------------------------------------------------------------------
     if (elect_one()) {
@@ -223,11 +221,11 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
       uint32_t kpos = 0, qpos = 0, step = 0, jobs = 0;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t n) {  // the n-th completion (from 0)
-        ok = ok && mbar_wait(bar, n & 1, dead);
+        ok = ok && mbar_wait(bar, n & 1, waits);
         return ok;
       };
       Job job;
-      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, jobs, dead, &job)) && job.ta < job.tb) {
+      while (ok && (ok = take_job_alone(s_jobs, job_full, job_empty, jobs, waits, &job)) && job.ta < job.tb) {
         const int chunks = job.row;
         const int tiles = job.tb - job.ta;
         for (int t = 0; ok && t < tiles; ++t) {
@@ -272,11 +270,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           kpos += kTS;
         }
       }
-      if (*dead) {  // no product may be in flight when TMEM is freed
-        int none = 0;
-        tc_commit(drain);
-        mbar_wait(drain, 0, &none);
-      }
+      drain_products(drain);
     }
     __syncwarp();
   } else if constexpr (Sh::kRows) {
@@ -288,7 +282,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
     bool ok = true;
-    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
+    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, waits, &job)) && job.ta < job.tb) {
       const int chunks = job.row;
       float neg = -INFINITY;  // -lse; -inf where the row adds nothing
       int lim = 0, clear = 0;  // keys that the row sees, and that all of the warp's rows see
@@ -314,7 +308,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           if ((step & 1) != wg) continue;
           some = true;
           if (chunks > 1) load_row(ch);
-          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
+          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, waits))) break;
           ++mine;
           tc_fence_after();
           bad = s_bad[tile & 15];
@@ -388,7 +382,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
     bool ok = true;
-    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, dead, &job)) && job.ta < job.tb) {
+    while (ok && (ok = take_job(s_jobs, job_full, job_empty, jobs, lane, waits, &job)) && job.ta < job.tb) {
       const int chunks = job.row;
       bool none = false;  // a row of the chunk adds nothing
       // -lse of a chunk's rows, -inf where a row adds nothing
@@ -424,7 +418,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           // chunk's tokens first: a key far before the window times a wide group does not fit 32 bits.)
           const int unseen = c.causal ? min(max(j - (job.kv_len - job.q_len + tok0), 0), P.chunk_tokens) : 0;
           const int from = unseen * c.group;
-          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, dead))) break;
+          if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, waits))) break;
           ++mine;
           tc_fence_after();
           there = j < job.kv_len && !(s_bad[tile & 15] >> (key >> P.box.shift) & 1);
@@ -503,7 +497,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     }
   }
   __syncthreads();
-  if (tid == 0) P.m.errors[blockIdx.x] = *dead;
+  if (tid == 0) P.m.errors[blockIdx.x] = waits->dead;
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Sh::kCols) : "memory");

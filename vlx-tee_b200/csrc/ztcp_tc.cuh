@@ -9,7 +9,6 @@ namespace ztcp {
 
 constexpr int kKeys = 128;                           // keys per tile
 constexpr int kGroupBytes = kKeys * 128;             // a tile's 64-column group: 128 rows of 128 bytes
-constexpr long long kWaitCycles = 2000000000ll;      // bound of a wait: a second or so
 
 // Boxes of the pool's TMA loads.
 struct PoolBoxes {
@@ -36,19 +35,30 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       "{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared.b64 P, [%1], %2;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
+// The bound of a CTA's waits, in cycles, and whether one has run out.
+struct Waits {
+  long long limit;
+  int dead;
+};
 // Waits for the phase of this parity.  False when the wait ran out: here, which sets the CTA's dead flag, or in another
 // role.  (A single attempt may be suspended by the hardware for tens of microseconds, so the bound is one of time.)
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile Waits* waits) {
   if (mbar_try(bar, parity)) return true;
   const long long start = clock64();
   while (!mbar_try(bar, parity)) {
-    if (*dead) return false;
-    if (clock64() - start > kWaitCycles) {
-      *dead = 1;
+    if (waits->dead) return false;
+    if (clock64() - start > waits->limit) {
+      waits->dead = 1;
       return false;
     }
   }
   return true;
+}
+// Waits for `n` fills of a ring's slots, the last ones of `pos`, whatever the other roles have come to.  A copy still in
+// flight when its CTA ends would write into the next one's shared memory.
+__device__ __forceinline__ void drain_fills(uint32_t bars, uint32_t slots, uint32_t pos) {
+  Waits none = {kWaitCycles, 0};
+  for (uint32_t p = pos > slots ? pos - slots : 0; p < pos; ++p) mbar_wait(bars + p % slots * 8, (p / slots) & 1, &none);
 }
 // One lane of a converged warp, always the same.  The compiler keeps the operands of what it guards in uniform
 // registers, which tcgen05 instructions read (measured: 39 cycles per small product, against 44 to 53 under lane == 0).
@@ -58,8 +68,8 @@ __device__ __forceinline__ bool elect_one() {
   return p;
 }
 // The same for a whole warp: all lanes go on, or none.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, dead));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile Waits* waits) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, waits));
 }
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
@@ -71,6 +81,12 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, 
 }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Waits for every product that this thread has issued: none may be in flight when TMEM is freed.
+__device__ __forceinline__ void drain_products(uint32_t bar) {
+  Waits none = {kWaitCycles, 0};
+  tc_commit(bar);
+  mbar_wait(bar, 0, &none);
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -313,7 +329,7 @@ struct Publisher {
   Cut cut;
   uint32_t n;  // published so far
   // Publishes the next item (lane 0 of the warp writes) and keeps it in `job`; false after a timeout.
-  __device__ __forceinline__ bool next(const CacheParams& c, const SplitSpan& S, Job* jobs, uint32_t full, uint32_t empty, int lane, volatile int* dead,
+  __device__ __forceinline__ bool next(const CacheParams& c, const SplitSpan& S, Job* jobs, uint32_t full, uint32_t empty, int lane, volatile Waits* waits,
                                        Job* job) {
     Item<KEYS>& it = walk.it;
     const int64_t begin = S.begin(blockIdx.x);
@@ -339,7 +355,7 @@ struct Publisher {
       cut.tiles[1] = it.tb;
     }
     const uint32_t e = n % kJobs;
-    if (n >= kJobs && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * e, (n / kJobs - 1) & 1, dead))) return false;
+    if (n >= kJobs && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * e, (n / kJobs - 1) & 1, waits))) return false;
     if (lane == 0) {
       jobs[e] = *job;
       mbar_arrive(full + 8 * e);
@@ -350,18 +366,18 @@ struct Publisher {
 };
 
 // The other side, for one thread that stands for its warp.
-__device__ __forceinline__ bool take_job_alone(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, volatile int* dead, Job* job) {
+__device__ __forceinline__ bool take_job_alone(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, volatile Waits* waits, Job* job) {
   const uint32_t e = n % kJobs;
-  if (!mbar_wait(full + 8 * e, (n / kJobs) & 1, dead)) return false;
+  if (!mbar_wait(full + 8 * e, (n / kJobs) & 1, waits)) return false;
   *job = jobs[e];
   mbar_arrive(empty + 8 * e);
   ++n;
   return true;
 }
 // The other side: a warp takes the next item (false after a timeout) and frees its place at once.
-__device__ __forceinline__ bool take_job(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, int lane, volatile int* dead, Job* job) {
+__device__ __forceinline__ bool take_job(const Job* jobs, uint32_t full, uint32_t empty, uint32_t& n, int lane, volatile Waits* waits, Job* job) {
   const uint32_t e = n % kJobs;
-  if (!warp_wait(full + 8 * e, (n / kJobs) & 1, dead)) return false;
+  if (!warp_wait(full + 8 * e, (n / kJobs) & 1, waits)) return false;
   *job = jobs[e];
   __syncwarp();
   if (lane == 0) mbar_arrive(empty + 8 * e);

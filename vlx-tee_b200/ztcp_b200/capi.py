@@ -39,7 +39,7 @@ EXPORTED_SYMBOLS = (
     "ztcp_decode_pages_noalloc",
 )
 # every symbol include/ztcp_measure.h declares (measurement entry points, not part of the drop-in boundary)
-MEASURE_SYMBOLS = ("ztcp_measure_int_peaks", "ztcp_mark_phase")
+MEASURE_SYMBOLS = ("ztcp_measure_int_peaks", "ztcp_mark_phase", "ztcp_wait_limit")
 MEASURE_SCRATCH_BYTES = 8 << 20  # ZTCP_MEASURE_SCRATCH_BYTES
 
 
@@ -142,6 +142,8 @@ def load() -> C.CDLL:
     L.ztcp_measure_int_peaks.argtypes = [vp, i64, C.POINTER(IntPeaks)]
     L.ztcp_mark_phase.restype = i32
     L.ztcp_mark_phase.argtypes = [vp]
+    L.ztcp_wait_limit.restype = i64
+    L.ztcp_wait_limit.argtypes = [i64]
     L.ztcp_gather.restype = i32
     L.ztcp_gather.argtypes = [vp, i32, C.POINTER(vp), C.POINTER(i32), C.POINTER(i64), i32, vp]
     _lib = L
