@@ -711,6 +711,75 @@ def test_tiny_scale(q_len):
     ref.assert_close(mass, want, tol, "mass")
 
 
+def one_key_scores(op, T, G, D, dtype, hint, rope, kind, n=4096):
+    """Scores of n sequences of one token: (64-bit ones, the errors of the kernel's).  With one key the log-sum-exp is its
+    score; a page's weight is the exponential of the score's error over a given log-sum-exp."""
+    from ztcp_b200 import kvcache
+
+    g = torch.Generator(device=DEV).manual_seed(D + G)
+    rnd = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    q, key = rnd(n, G, D), rnd(n, D)
+    if kind == "few bits":  # every product and every partial sum is exact
+        q, key = q.sign() * 0.5 * (1 + (q.abs() > 1)), key.sign() * (1 + (key.abs() > 0.7))
+    if kind == "one column":
+        q = torch.zeros_like(q).scatter_(2, torch.randint(0, D, (n, G, 1), generator=g, device=DEV), 1.0) * q
+    if kind == "positive":
+        q, key = q.abs(), key.abs()
+    q, key = q.to(dtype), key.to(dtype)
+    k = torch.zeros((n, T, 1, D), dtype=dtype, device=DEV)
+    k[:, 0, 0] = key
+    tables = torch.arange(n, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    lens = torch.ones(n, dtype=torch.int32, device=DEV)
+    kw = dict(q_starts=torch.arange(n + 1, dtype=torch.int32, device=DEV), max_q_len=hint, scale=1.0)
+    s = torch.einsum("ngd,nd->ng", q.double(), key.double())
+    if op == "attend":
+        out, lse = torch.empty((n, G, D - (rope or 0)), dtype=dtype, device=DEV), torch.empty((n, G), device=DEV)
+        kvcache.attend_pages(q, k, None if rope else k, tables, lens, out, lse=lse, rope_dim=rope or 0, **kw)
+        return s, lse.double() - s
+    errors, lse = [], s.float()
+    for h in range(G):
+        out = torch.empty((n, 1), device=DEV)
+        kvcache.page_mass(q[:, h:h + 1].contiguous(), k, tables, lens, lse[:, h:h + 1].contiguous(), None, out, **kw)
+        errors.append(torch.log(out[:, 0].double()) + lse[:, h].double() - s[:, h])
+    return s, torch.stack(errors, 1)
+
+
+SCORES = [("attend", 8, 4, 64, 1, None), ("attend", 8, 4, 128, 1, None), ("attend", 8, 4, 256, 1, None), ("attend", 8, 4, 576, 1, 64),
+          ("attend", 8, 4, 128, 40, None), ("attend", 5, 4, 128, 1, None), ("attend", 5, 4, 320, 1, 16), ("attend", 5, 4, 576, 1, 64),
+          ("mass", 8, 2, 64, 1, None), ("mass", 8, 2, 128, 1, None), ("mass", 8, 2, 128, 40, None), ("mass", 8, 2, 64, 90, None),
+          ("mass", 8, 2, 128, 90, None), ("mass", 8, 2, 256, 1, None), ("mass", 8, 2, 256, 40, None), ("mass", 8, 2, 576, 1, None),
+          ("mass", 8, 2, 576, 40, None), ("mass", 5, 2, 128, 1, None), ("mass", 5, 2, 576, 1, None)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("op,T,G,D,hint,rope", SCORES)
+def test_exact_scores_stay_exact(op, T, G, D, hint, rope, dtype):
+    """Where every product and partial sum is exact, so is the score: nothing is added to it for what other data would
+    lose.  A page's weight under the score itself as log-sum-exp is then 1, to the bit.  Of the log-sum-exp, the rounded
+    scale * log2(e) and ln 2 are at most a half step off each, the last fma another (with |score| each), and the sum of one
+    weight, whose logarithm is added, two steps of 1."""
+    for kind in ("few bits", "one column"):
+        s, e = one_key_scores(op, T, G, D, dtype, hint, rope, kind)
+        if op == "mass":
+            exact = s.float().double() == s  # (all few-bit ones, and products of two 11-bit numbers)
+            assert bool(exact.all()) and bool((e == 0).all())
+        else:
+            assert bool((e.abs() <= ref.U32 * (3 * s.abs() + 5)).all()), float(((e.abs() - 5 * ref.U32) / s.abs()).max()) / ref.U32
+
+
+@pytest.mark.parametrize("D,hint,times", [(128, 1, 1.5), (128, 90, 1.5), (256, 40, 1.5), (576, 1, 1.5), (576, 40, 3)])
+def test_score_loss_does_not_grow_with_the_columns(D, hint, times):
+    """The tensor cores' accumulator drops the lowest bits of what it holds, for every product that it takes.  Positive
+    data shows it: after each of n products it stands at an even share of the sum, so that the relative loss grows
+    with n.  Page weights give an accumulator four products of 16 columns whatever the head_dim (eight with 32 rows of 576:
+    about twice the loss), as at head_dim 64; one accumulator for 36 products loses 16 times as much."""
+    base_s, base = one_key_scores("mass", 8, 2, 64, F16, hint, None, "positive")
+    s, e = one_key_scores("mass", 8, 2, D, F16, hint, None, "positive")
+    mean = lambda s, e: float(e.sum() / s.sum()) / ref.U32  # noqa: E731
+    # (a half step for the sum of the parts and one for the exponent's rounding, in the mean at most)
+    assert abs(mean(s, e)) <= times * abs(mean(base_s, base)) + 1
+
+
 def test_mass_more_rows_than_tokens():
     check_mass([3, 10], [40, 200], 16, 1, 4, 64, F16)
 

@@ -92,6 +92,7 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
     tmem_ready32(r);
   } else {
     tmem_ld16(addr, r);
+    tmem_ready16(r);
   }
 }
 template <int N>

@@ -33,8 +33,7 @@ struct CacheParams {
   int32_t head_dim, v_dim, v_col;
   int32_t causal;
   float scale;
-  float scale_more;  // what a score of the tensor cores is small by, times the scale
-  float scale_log2;  // (scale + scale_more) * log2(e): scores enter exp2
+  float scale_log2;  // scale * log2(e): scores enter exp2
   int64_t wait_cycles;  // bound of a wait inside a kernel
   int32_t* status;
 };

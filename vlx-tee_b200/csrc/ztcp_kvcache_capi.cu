@@ -1,6 +1,5 @@
 // ztcp_kvcache_capi.cu -- host layer of include/ztcp_kvcache.h: validates arguments and launches the kernels on the
 // caller's stream.  Nothing here allocates memory or synchronizes.
-#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -39,18 +38,6 @@ int32_t check_pool(const ztcp_geometry& g, int32_t dtype, int64_t pool_pages, co
 // A row of 16-bit vectors read 16 bytes at a time.
 bool bad_rows(const void* p, int64_t token_stride, int64_t head_stride) {
   return !aligned(p, 16) || token_stride % 8 != 0 || head_stride % 8 != 0;
-}
-
-// What a score of the tensor cores is small by, relative to itself, in the mean: their accumulator drops what lies below
-// its last bit, once per product of 16 columns.  Measured on normally distributed queries and keys against 64 bits, the
-// same in every kernel here (mma.sync and tcgen05): 0.30 (n + 1) units of 2^-24 after n products in fp16 (0.60, 0.91,
-// 1.52, 2.64, 5.08, 10.8 for n = 1, 2, 4, 8, 16, 36), 0.235 n in bf16, whose products have fewer bits to drop (0.22,
-// 0.49, 0.97, 1.76, 3.69, 8.5).  Exponents of 9 lost 1.4e-6 of their weight to it at a head_dim of 128.  Attention's
-// scale takes it back to within its own rounding; page weights, which nothing rounds to 16 bits, add it in a step of
-// its own.
-double mean_loss(int head_dim, bool bf16) {
-  const int n = (head_dim + 15) / 16;
-  return (bf16 ? 0.235 * n : 0.30 * (n + 1)) * 0x1p-24;
 }
 
 int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CacheParams* c) {
@@ -99,12 +86,9 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   c->v_col = k->v_pool ? 0 : (int32_t)g.rope_dim;
   c->v_dim = c->head_dim - c->v_col;
   c->causal = q->causal != 0;
-  const double loss = mean_loss(c->head_dim, k->dtype == ZTCP_DTYPE_BF16);
   c->wait_cycles = g_wait_cycles.load(std::memory_order_relaxed);
   c->scale = q->scale;
-  // (0 times a masked score of -inf would be a NaN, where a scale is so small that its correction rounds to 0)
-  c->scale_more = fmaxf((float)(q->scale * loss), FLT_TRUE_MIN);
-  c->scale_log2 = (float)(q->scale * (1 + loss) * 1.4426950408889634);
+  c->scale_log2 = (float)(q->scale * 1.4426950408889634);
   if (isinf(c->scale_log2)) return invalid("scale must be positive and finite, times log2(e) too");
   return ZTCP_OK;
 }

@@ -2,8 +2,8 @@
 //
 // Mathematics.  out[b, p] = decay * mass[b, p] + sum over rows r, heads and tokens j of page p of
 // exp(s_rj - lse_r): with the log-sum-exp known, weights need one product and no second pass.  (s - lse is formed by
-// one fma, corrected by a second for the accumulator's mean loss, and then multiplied by log2 e, so that it is rounded
-// as a small number.)
+// one fma and then multiplied by log2 e, so that it is rounded as a small number; a score's products of 64 columns add up
+// in the tensor cores' accumulator, which drops its lowest bits, and these parts in fp32.)
 //
 // Work.  A unit is as many whole pages as fit 64 keys (one, where a page is larger), of one sequence, all KV heads:
 // its sums never cross CTAs, so there are no atomics and results repeat bit for bit.  Units of all sequences form
@@ -141,13 +141,18 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
     if (rg * 16 < rows) {
       const uint32_t kbase = ring + stage * sbytes + kb * 16 * pitch, qbase = ring + stage * sbytes + (kKeys + rg * 16) * pitch;
       float sc[2][4] = {};
-      for (int ks = 0; ks < nks; ++ks) {
-        uint32_t a[4], b[4];
-        ldmatrix4(a, chunk_at(kbase, (lane & 7) + (lane & 8), ks * 2 + (lane >> 4), pitch));
-        // rows 0-7 and 8-15 of the row block, both k halves of each
-        ldmatrix4(b, chunk_at(qbase, (lane & 7) + ((lane >> 1) & 8), ks * 2 + ((lane >> 3) & 1), pitch));
-        mma16816<BF16>(sc[0], a, b[0], b[1]);
-        mma16816<BF16>(sc[1], a, b[2], b[3]);
+      for (int k0 = 0; k0 < nks; k0 += 4) {
+        float part[2][4] = {};
+        for (int ks = k0; ks < min(k0 + 4, nks); ++ks) {
+          uint32_t a[4], b[4];
+          ldmatrix4(a, chunk_at(kbase, (lane & 7) + (lane & 8), ks * 2 + (lane >> 4), pitch));
+          // rows 0-7 and 8-15 of the row block, both k halves of each
+          ldmatrix4(b, chunk_at(qbase, (lane & 7) + ((lane >> 1) & 8), ks * 2 + ((lane >> 3) & 1), pitch));
+          mma16816<BF16>(part[0], a, b[0], b[1]);
+          mma16816<BF16>(part[1], a, b[2], b[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[0][e] += part[0][e], sc[1][e] += part[1][e];
       }
       const int key = cons.unit * P.unit_pages * c.page_tokens + cons.sub * kKeys + kb * 16 + g;
       const bool ok0 = s_there[stage][kb * 16 + g], ok1 = s_there[stage][kb * 16 + g + 8];
@@ -158,8 +163,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) page_mass_kernel(const __gri
           const int r = rg * 16 + n * 8 + 2 * t4 + e;
           const float neg = s_neg[stage][r];
           const int lim = s_lim[stage][r];
-          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale_more, fmaf(sc[n][e], c.scale, neg)) * 1.44269504088896f);
-          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale_more, fmaf(sc[n][2 + e], c.scale, neg)) * 1.44269504088896f);
+          if (ok0 && key < lim) k0 += fast_exp2(fmaf(sc[n][e], c.scale, neg) * 1.44269504088896f);
+          if (ok1 && key + 8 < lim) k1 += fast_exp2(fmaf(sc[n][2 + e], c.scale, neg) * 1.44269504088896f);
         }
     }
 

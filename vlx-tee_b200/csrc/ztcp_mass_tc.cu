@@ -6,21 +6,28 @@
 // are then one segment, whose sum goes to the workspace per KV head.  With 256 rows the product is turned over,
 //   S[2 x 128 rows, 128 keys] = Q K^T   (rows on the lanes)
 // so that a thread's lse is a register (read from shared memory for every column it took the bandwidth that the
-// products need: 87 us against 80, before the join got faster, for windows of 64 tokens of four sequences, 32 heads over 84,800 keys); a warp adds its 32
-// rows up by shuffles, segment by segment.  page_mass_join_kernel adds a page's segments and heads in a fixed order,
-// so there are no atomics and results repeat bit for bit.
+// products need: 87 us against 80, before the join got faster, for windows of 64 tokens of four sequences, 32 heads over
+// 84,800 keys); a warp adds its 32 rows up by shuffles, segment by segment.  page_mass_join_kernel adds a page's segments
+// and heads in a fixed order, so there are no atomics and results repeat bit for bit.
 //
 // Accuracy.  The exponent is formed as fma(s, scale, -lse) -- one rounding of a value that is small wherever the
 // weight is not -- and only then multiplied by log2 e: folding log2 e into the scale would round s * scale * log2 e
-// and lse * log2 e, both of tens, apart from each other.  A second fma adds what the tensor core's accumulator has
-// dropped in the mean (mean_loss): against 64 bits 1.4e-6 of a weight otherwise, 2e-7 with it.
+// and lse * log2 e, both of tens, apart from each other.  The tensor cores' accumulator drops what lies below its last
+// bit, for every product of 16 columns that enters it, so that a long chain makes a score small by as much as the data
+// has bits to drop (8 products: nothing where they are exact, 2.6 units of 2^-24 of the score on normally distributed
+// queries and keys, 8.6 where all are positive; 36 products: 0, 10 and 54).  So an accumulator takes one column group,
+// four products (two groups where TMEM has no more room: head_dim beyond 256 with 32 rows), and the groups add up in
+// fp32: 0, 1.5 and 3.4 units at any head_dim, and page weights within 6e-7 of 64-bit ones in the cases below instead of
+// 1.2e-6.  It costs a second reading of TMEM: windows of 64 tokens 92 us instead of 75, one token each nothing.
 //
 // Work.  An item is one KV head of one sequence, a tile 128 of its keys times as many chunks of N rows as its queries
 // need (N = 16 for one token's group, up to 256 for a window of them); the line of tiles x chunks is shared evenly.
-// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 91 us, 5.5 TB/s, of
-// which 8 us are start and join); for an observation window the exponentials, N x 128 a tile (73 us, of 27 us that the
-// special-function units need; a quarter or 3/8 of them as a polynomial on the FMA pipes, a second warp of products, or
-// loads of the next 32 scores under the arithmetic of these were measured, at 2 to 8 us more).
+// Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 94 us, 5.3 TB/s, of
+// which 8 us are start and join); for an observation window the threads' chains of score loads, exponentials and sums
+// (92 us, of which the special-function units need 27 and the join 13: neither they nor the issue of instructions is
+// half busy).  Measured for windows: steps of one row tile and 128 keys instead of two and 64 the same time; loads of the
+// next 16 scores under the arithmetic of these 1 us less; before, with one accumulator a score, a quarter or 3/8 of the
+// exponentials as a polynomial on the FMA pipes or a second warp of products 2 to 8 us more.
 //
 // Warps.  Groups of four: sums of every other step, a thread per key, no warp waiting for another; then one for the
 // products and one for TMA (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
@@ -45,6 +52,7 @@ struct MassTcParams {
   int32_t seg_shift;     // log2 of the keys of a segment: 32, or a smaller page's
   int32_t segs;          // segments of a sequence in the workspace
   int32_t sums;          // sums of a segment that a step leaves in the workspace
+  int32_t turns;         // step parities that a segment's sums come from, where there are several chunks
 };
 
 template <int KG, int N>
@@ -62,8 +70,15 @@ struct Shape {
   static constexpr int kRoom = (232448 - 4096 - kQSlots * kQBytes - kNegBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 8 ? kRoom : 8;
   static constexpr int kSmem = kBars * 8 + 1024 + kSlots * kSlotBytes + kQSlots * kQBytes + kNegBytes;
-  static constexpr int kCols = 2 * N < 32 ? 32 : 2 * N;     // TMEM: S^T of two steps
-  static_assert(kSlots >= kTileSlots && 2 * kSlots + 9 + 2 * kJobs <= kBars, "shape");
+  // Accumulators of a step: one per column group (two groups where TMEM has no room for more).
+  static constexpr int kPer = !kRows && 2 * N * KG > 512 ? 2 : 1;
+  static constexpr int kAccs = (KG + kPer - 1) / kPer;
+  // Keys of a step: with rows on the lanes, further accumulators take the columns of further keys.
+  static constexpr int kStepKeys = kRows ? kKeys / kAccs : kKeys;
+  static constexpr int kTileSteps = kKeys / kStepKeys;      // per chunk
+  static constexpr int kBuf = kRows ? 256 : kAccs * N;      // columns of a step's scores; TMEM holds two steps'
+  static constexpr int kCols = 2 * kBuf <= 32 ? 32 : 2 * kBuf <= 64 ? 64 : 2 * kBuf <= 128 ? 128 : 2 * kBuf <= 256 ? 256 : 512;
+  static_assert(kSlots >= kTileSlots && 2 * kSlots + 9 + 2 * kJobs <= kBars && 2 * kBuf <= kCols, "shape");
 };
 
 // Tiles and chunks of a sequence.
@@ -79,6 +94,28 @@ __device__ __forceinline__ MassSeq mass_seq(const MassTcParams& P, int b) {
   m.tiles = m.s.q_len > 0 ? (m.s.kv_len + kKeys - 1) / kKeys : 0;
   m.chunks = (m.s.q_len + P.chunk_tokens - 1) / P.chunk_tokens * P.parts;
   return m;
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 32) tmem_ld32(addr, r);
+  else tmem_ld16(addr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_ready(uint32_t* r) {
+  if constexpr (N == 32) tmem_ready32(r);
+  else tmem_ready16(r);
+}
+// x += y, columns of fp32.
+template <int N>
+__device__ __forceinline__ void add_columns(uint32_t* x, const uint32_t* y) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float a, b;
+    unpair(add2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), pair(__uint_as_float(y[i]), __uint_as_float(y[i + 1]))), a, b);
+    x[i] = __float_as_uint(a);
+    x[i + 1] = __float_as_uint(b);
+  }
 }
 
 template <bool BF16, int KG, int N>
@@ -216,7 +253,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     // ---- products: one thread ---------------------------------------------------------------------------
     if (elect_one()) {
       constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
-      const uint32_t qk = inst_desc(BF16, 128, Sh::kRows ? kKeys : N, false, false);
+      const uint32_t qk = inst_desc(BF16, 128, Sh::kRows ? Sh::kStepKeys : N, false, false);
       const uint32_t k_lo = desc_lo(ring, 16), q_lo = desc_lo(qbuf, 16);
       uint32_t kpos = 0, qpos = 0, step = 0, jobs = 0;
       bool ok = true;
@@ -229,40 +266,47 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         const int chunks = job.row;
         const int tiles = job.tb - job.ta;
         for (int t = 0; ok && t < tiles; ++t) {
-          for (int ch = 0; ok && ch < chunks; ++ch, ++step) {
+          for (int ch = 0; ok && ch < chunks; ++ch) {
             const bool fresh = chunks > 1 || t == 0;             // this step's Q is a new one,
             const bool spent = chunks > 1 || t + 1 == tiles;     // and not used again
-            const uint32_t qslot = qpos % kQS, buf = step & 1;
+            const uint32_t qslot = qpos % kQS;
             if (fresh && !wait(q_full + 8 * qslot, qpos / kQS)) break;
-            if (step > 1 && !wait(s_read + 8 * buf, (step >> 1) - 1)) break;
+            for (int part = 0; ok && part < Sh::kTileSteps; ++part, ++step) {
+              const uint32_t buf = step & 1, d = tmem + buf * Sh::kBuf, q = q_lo + qslot * (Sh::kQBytes >> 4);
+              if (step > 1 && !wait(s_read + 8 * buf, (step >> 1) - 1)) break;
 #pragma unroll
-            for (int s = 0; s < kTS; ++s) {
-              const uint32_t pos = kpos + s, slot = pos % kSlots;
-              if (ch == 0 && !wait(full(slot), pos / kSlots)) break;
-              tc_fence_after();
-              const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4), q = q_lo + qslot * (Sh::kQBytes >> 4), d = tmem + buf * N;
-              if constexpr (Sh::kRows) {
-                const bool two = (P.parts == 1 ? (job.q_len - ch * P.chunk_tokens) * (int64_t)c.group : c.group - ch % P.parts * N) > 128;
+              for (int s = 0; s < kTS; ++s) {
+                const uint32_t pos = kpos + s, slot = pos % kSlots;
+                if (ch == 0 && part == 0 && !wait(full(slot), pos / kSlots)) break;
+                tc_fence_after();
+                const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4);
+                bool two = false;  // the chunk's rows fill more than one row tile
+                if constexpr (Sh::kRows)
+                  two = (P.parts == 1 ? (job.q_len - ch * P.chunk_tokens) * (int64_t)c.group : c.group - ch % P.parts * N) > 128;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  if (h == 0 || two)
+                for (int i = 0; i < Sh::kGroups; ++i) {
+                  const int g = s * Sh::kGroups + i;
+                  if (g >= KG) continue;
+                  if constexpr (Sh::kRows) {
 #pragma unroll
-                    for (int k = 0; k < KG * 4; ++k)
-                      mma_ss(d + h * 128, q + (((k >> 2) * N * 128 + h * 128 * 128 + (k & 3) * 32) >> 4), kHi, a + (((k >> 2) * kGroupBytes + (k & 3) * 32) >> 4),
-                             kHi, qk, k > 0);
-              } else
+                    for (int h = 0; h < 2; ++h)
+                      if (h == 0 || two)
 #pragma unroll
-              for (int g = 0; g < Sh::kGroups; ++g)
-                if (s * Sh::kGroups + g < KG)
+                        for (int k = 0; k < 4; ++k)
+                          mma_ss(d + (2 * g + h) * Sh::kStepKeys, q + ((g * N * 128 + h * 128 * 128 + k * 32) >> 4), kHi,
+                                 a + ((i * kGroupBytes + part * Sh::kStepKeys * 128 + k * 32) >> 4), kHi, qk, k > 0);
+                  } else {
 #pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    mma_ss(d, a + ((g * kGroupBytes + k * 32) >> 4), kHi, q + (((s * Sh::kGroups + g) * N * 128 + k * 32) >> 4), kHi, qk,
-                           s * Sh::kGroups + g > 0 || k > 0);
-              if (ch + 1 == chunks) tc_commit(empty(slot));
+                    for (int k = 0; k < 4; ++k)
+                      mma_ss(d + g / Sh::kPer * N, a + ((i * kGroupBytes + k * 32) >> 4), kHi, q + ((g * N * 128 + k * 32) >> 4), kHi, qk,
+                             g % Sh::kPer > 0 || k > 0);
+                  }
+                }
+                if (ch + 1 == chunks && part + 1 == Sh::kTileSteps) tc_commit(empty(slot));
+              }
+              if (ok) tc_commit(s_full + 8 * buf);
             }
-            if (!ok) break;
-            tc_commit(s_full + 8 * buf);
-            if (spent) {
+            if (ok && spent) {
               tc_commit(q_empty + 8 * qslot);
               ++qpos;
             }
@@ -276,8 +320,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
   } else if constexpr (Sh::kRows) {
     // ---- sums: a thread per row -------------------------------------------------------------------------
     const int wg = (warp >> 2) & 1, half = warp >> 3, r = half * 128 + (tid & 127);
-    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N + half * 128;
-    const uint64_t scale2 = pair(c.scale, c.scale), more2 = pair(c.scale_more, c.scale_more), log2e = pair(1.44269504088896f, 1.44269504088896f);
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * Sh::kBuf + half * Sh::kStepKeys;  // the first accumulator
+    const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
     const int tok_in = r / P.part_heads, head_in = r - tok_in * P.part_heads;
     uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
@@ -304,8 +348,9 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         unsigned bad = 0;
         float total = 0.f;  // lane i: the tile's segment i
         bool some = false;
-        for (int ch = 0; ch < chunks; ++ch, ++step) {
-          if ((step & 1) != wg) continue;
+        for (int x = 0; x < chunks * Sh::kTileSteps; ++x, ++step) {
+          if ((step & 1) != wg) continue;  // (two steps a chunk: this group has the tile's keys of half wg)
+          const int ch = x / Sh::kTileSteps, k0 = x % Sh::kTileSteps * Sh::kStepKeys;
           some = true;
           if (chunks > 1) load_row(ch);
           if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, waits))) break;
@@ -323,7 +368,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const uint64_t s = pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-              uint64_t u = mul2(fma2(s, more2, fma2(s, scale2, neg2)), log2e);
+              uint64_t u = mul2(fma2(s, scale2, neg2), log2e);
               float a, b2;
               unpair(u, a, b2);
               u = pair(fast_exp2(a), fast_exp2(b2));
@@ -349,16 +394,24 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           };
           if (any) {
 #pragma unroll 1
-            for (int n0 = 0; n0 < kKeys; n0 += 32) {
+            for (int n0 = 0; n0 < Sh::kStepKeys; n0 += 32) {
               uint32_t x[32];
               tmem_ld32(ts + n0, x);
-              tmem_ready32(x);
-              if (n0 + 32 == kKeys) {  // S has been read
+              if constexpr (Sh::kAccs > 1) {
+                uint32_t y[32];
+                tmem_ld32(ts + 2 * Sh::kStepKeys + n0, y);
+                tmem_ready32(x);
+                tmem_ready32(y);
+                add_columns<32>(x, y);
+              } else {
+                tmem_ready32(x);
+              }
+              if (n0 + 32 == Sh::kStepKeys) {  // S has been read
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_read + 8 * wg);
               }
-              add_block(x, n0);
+              add_block(x, k0 + n0);
             }
           } else {
             __syncwarp();
@@ -367,18 +420,19 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         }
         if (!ok) break;
         const int seg = (j0 >> P.seg_shift) + lane;
-        if (some && lane < kKeys >> P.seg_shift && seg << P.seg_shift < job.kv_len) {
+        const int from = Sh::kTileSteps > 1 ? wg * (Sh::kStepKeys >> P.seg_shift) : 0, segs = Sh::kStepKeys >> P.seg_shift;  // this group's
+        if (some && lane >= from && lane < from + segs && seg << P.seg_shift < job.kv_len) {
           if (bad >> (lane << P.seg_shift >> P.box.shift) & 1) total = 0.f;
-          P.m.part[(((int64_t)((chunks > 1 ? kRowSums * wg : 0) + half * 4 + (warp & 3)) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + seg] = total;
+          P.m.part[(((int64_t)((chunks > 1 && Sh::kTileSteps == 1 ? kRowSums * wg : 0) + half * 4 + (warp & 3)) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + seg] = total;
         }
       }
     }
   } else {
     // ---- sums: a thread per key -------------------------------------------------------------------------
     const int wg = warp >> 2, key = tid & 127;
-    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * N;
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * Sh::kBuf;
     float* const neg = negs + warp * N;
-    const uint64_t scale2 = pair(c.scale, c.scale), more2 = pair(c.scale_more, c.scale_more), log2e = pair(1.44269504088896f, 1.44269504088896f);
+    const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
     uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
     bool ok = true;
@@ -433,8 +487,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
               const float4 w = *reinterpret_cast<const float4*>(neg + n0 + i);
               float a, b2, d, e;
               const uint64_t s = pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), s1 = pair(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-              unpair(mul2(fma2(s, more2, fma2(s, scale2, pair(w.x, w.y))), log2e), a, b2);
-              unpair(mul2(fma2(s1, more2, fma2(s1, scale2, pair(w.z, w.w))), log2e), d, e);
+              unpair(mul2(fma2(s, scale2, pair(w.x, w.y)), log2e), a, b2);
+              unpair(mul2(fma2(s1, scale2, pair(w.z, w.w)), log2e), d, e);
               a = fast_exp2(a);
               b2 = fast_exp2(b2);
               d = fast_exp2(d);
@@ -455,15 +509,34 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(s_read + 8 * wg);
           };
-          if constexpr (N < 64) {
-            uint32_t x[kBlock];
-            if constexpr (N == 16) tmem_ld16(ts, x);
-            else {
-              tmem_ld32(ts, x);
-              tmem_ready32(x);
+          // Columns [n0, n0 + kBlock) of all accumulators, added up; two more of them are loaded at a time.
+          auto load_block = [&](uint32_t* x, int n0) {
+            tmem_load<kBlock>(ts + n0, x);
+            if constexpr (Sh::kAccs == 1) tmem_ready<kBlock>(x);
+#pragma unroll
+            for (int a = 1; a < Sh::kAccs; a += 2) {
+              uint32_t y[kBlock], z[kBlock];
+              tmem_load<kBlock>(ts + a * N + n0, y);
+              if (a + 1 < Sh::kAccs) tmem_load<kBlock>(ts + (a + 1) * N + n0, z);
+              if (a == 1) tmem_ready<kBlock>(x);
+              tmem_ready<kBlock>(y);
+              add_columns<kBlock>(x, y);
+              if (a + 1 < Sh::kAccs) {
+                tmem_ready<kBlock>(z);
+                add_columns<kBlock>(x, z);
+              }
             }
-            release();
-            add_block(x, 0);
+          };
+          if constexpr (N < 64 || Sh::kAccs > 1) {
+            uint32_t x[kBlock];
+#pragma unroll 1
+            for (int n0 = 0; n0 < N; n0 += kBlock) {
+              load_block(x, n0);
+              const bool more = n0 + kBlock < N && n0 + kBlock < valid;
+              if (!more) release();
+              add_block(x, n0);
+              if (!more) break;
+            }
           } else {  // one block's loads under the other's arithmetic
             uint32_t x[32], y[32];
             tmem_ld32(ts, x);
@@ -520,7 +593,7 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
       if (P.m.mass) before = P.m.mass[i];
       if (m.chunks > 0) {
         n = (int)((min((int64_t)c.page_tokens, left) + (1 << P.seg_shift) - 1) >> P.seg_shift);
-        slots = m.chunks > 1 ? 2 : 1;
+        slots = m.chunks > 1 ? P.turns : 1;
       }
     }
   }
@@ -570,6 +643,7 @@ int chunk_rows(const CacheParams& c, int64_t rows) {
   return rows <= 64 || c.head_dim > 128 ? 64 : 256;
 }
 int sums_of(int n) { return n == 256 ? kRowSums : 1; }
+int turns_of(const CacheParams& c, int n) { return n == 256 && c.head_dim > 64 ? 1 : 2; }  // Shape::kTileSteps of 2: 1
 int seg_shift(const CacheParams& c) { return c.page_tokens >= 32 ? 5 : c.page_tokens == 16 ? 4 : 3; }
 int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_tokens >> seg_shift(c); }
 
@@ -578,7 +652,8 @@ int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_t
 bool page_mass_tc_fits(const CacheParams& c) { return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31); }
 
 int64_t page_mass_tc_workspace(const CacheParams& c, int64_t rows, int sms) {  // sums by step parity
-  return (sms + 3) / 4 * 16 + 2 * sums_of(chunk_rows(c, rows)) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+  const int n = chunk_rows(c, rows);
+  return (sms + 3) / 4 * 16 + turns_of(c, n) * sums_of(n) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
 }
 
 bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s) {
@@ -595,6 +670,7 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   P.seg_shift = seg_shift(m.c);
   P.segs = (int32_t)seg_count(m.c);
   P.sums = sums_of(n);
+  P.turns = turns_of(m.c, n);
   CUtensorMap k, q;
   if (!pool_map(&k, m.c.k, m.c, bf16, P.box) || !query_map(&q, m.c, bf16, P.chunk_tokens, P.part_heads)) return false;
   if (bf16) launch_any<true>(P, n, k, q, s);
