@@ -956,6 +956,41 @@ def test_select_page_counts(n, keep):
         assert torch.equal(got.cpu(), torch.tensor(exp, dtype=got.dtype).view(got.shape)), name
 
 
+@pytest.mark.parametrize("n,P", [(511, 9), (512, 9), (513, 9), (1537, 3), (5000, 5), (70_000, 3)])
+def test_select_many_sequences(n, P):
+    """Batches about the size from which the cold lists' starts are added up beforehand, and far beyond."""
+    from ztcp_b200 import kvcache
+
+    g = torch.Generator().manual_seed(n)
+    mass = torch.rand((n, P), generator=g)
+    tables = torch.randint(0, 1 << 20, (n, P), generator=g, dtype=torch.int32)
+    lens = torch.randint(0, P * 16 + 1, (n,), generator=g, dtype=torch.int32)
+    want = ref.select(mass.numpy(), tables, lens.tolist(), 16, 2, 1, 1)
+    sel = kvcache.select_cold_pages(mass.to(DEV), tables.to(DEV), lens.to(DEV), page_tokens=16, keep=2)
+    for got, exp, name in zip(sel, want, sel._fields):
+        assert torch.equal(got.cpu(), torch.tensor(exp, dtype=got.dtype).view(got.shape)), name
+    assert not sel.status.any()
+
+
+def test_select_takes_time_in_proportion():
+    """Every sequence's place was once found by adding up all sequences' pages: 262,144 of them took 180 ms."""
+    from ztcp_b200 import kvcache
+
+    def time(n):
+        mass, tables = torch.rand((n, 2), device=DEV), torch.zeros((n, 2), dtype=torch.int32, device=DEV)
+        lens = torch.full((n,), 32, dtype=torch.int32, device=DEV)
+        run = lambda: kvcache.select_cold_pages(mass, tables, lens, page_tokens=16, keep=1)  # noqa: E731
+        run()
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        run()
+        end.record()
+        torch.cuda.synchronize()
+        return begin.elapsed_time(end)
+
+    assert time(1 << 18) < 60  # (a few ms)
+
+
 def test_select_clamps_lengths():
     from ztcp_b200 import kvcache
 

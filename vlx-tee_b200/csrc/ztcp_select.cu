@@ -63,6 +63,25 @@ __device__ __forceinline__ int sum_before(int x, int* sums, int* total) {
   return before + inc - x;
 }
 
+// Where every sequence's cold pages begin, found beforehand for large batches: each CTA adding up all counts itself takes
+// time in proportion to the batch's square.  Measured with 256 pages a sequence, by each CTA / beforehand: 256 sequences
+// 6.2 / 7.5 us, 512 8.2 / 8.8, 1,024 15.5 / 13.3, 4,096 79 / 38; 262,144 of 4 pages 180 / 2.3 ms.
+constexpr int kManySeqs = 512;
+
+__global__ void __launch_bounds__(1024) select_starts_kernel(const __grid_constant__ ztcp_cold_selection S) {
+  __shared__ int sums[2][32];  // by turns, so that one barrier a step is enough
+  int run = 0;                 // fewer than 2^31 pages in all
+  for (int64_t b0 = 0, turn = 0; b0 < S.n_seqs; b0 += 1024, turn ^= 1) {
+    const int64_t b = b0 + threadIdx.x;
+    const int c = b < S.n_seqs ? pages_of(S, b).count : 0;
+    int total;
+    const int before = sum_before(c, sums[turn], &total);
+    if (b < S.n_seqs) S.cold_starts[b + 1] = run + before + c;
+    run += total;
+  }
+  if (threadIdx.x == 0) S.cold_starts[0] = 0;
+}
+
 template <int BITS>  // of a digit: as many bins as threads
 __global__ void __launch_bounds__(1 << BITS) select_kernel(const __grid_constant__ ztcp_cold_selection S) {
   constexpr int nt = 1 << BITS, kChunk = nt * kPer;
@@ -95,13 +114,15 @@ __global__ void __launch_bounds__(1 << BITS) select_kernel(const __grid_constant
   if (tid == 0) least_s = 0xffffffffu, most_s = 0;
   hist[tid] = 0;
   __syncthreads();
+  const bool many = S.n_seqs > kManySeqs;
+  if (many && tid < 2) offs[tid] = S.cold_starts[tid == 0 ? b : S.n_seqs];
   long long before = 0, all = 0;
-  for (int i = tid; i < S.n_seqs; i += nt) {
+  for (int i = tid; !many && i < S.n_seqs; i += nt) {
     const int c = pages_of(S, i).count;
     all += c;
     if (i < b) before += c;
   }
-  if (tid - (tid & 31) < S.n_seqs) {  // one 64-bit atomic a warp: from every thread they took 4 us (64 sequences)
+  if (!many && tid - (tid & 31) < S.n_seqs) {  // one 64-bit atomic a warp: from every thread they took 4 us (64 sequences)
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
       all += __shfl_xor_sync(0xffffffffu, all, d);
@@ -216,8 +237,10 @@ __global__ void __launch_bounds__(1 << BITS) select_kernel(const __grid_constant
     S.cold_index[i] = -1;
   }
   if (tid == 0) {
-    if (b == 0) S.cold_starts[0] = 0;
-    S.cold_starts[b + 1] = (int32_t)(base + me.count);
+    if (!many) {
+      if (b == 0) S.cold_starts[0] = 0;
+      S.cold_starts[b + 1] = (int32_t)(base + me.count);
+    }
     S.kept_lens[b] = (int32_t)(me.kv_len - me.count * S.page_tokens);
     S.status[b] = S.kv_lens[b] == me.kv_len ? ZTCP_SEQ_OK : ZTCP_SEQ_BAD_LENGTH;
   }
@@ -227,6 +250,7 @@ __global__ void __launch_bounds__(1 << BITS) select_kernel(const __grid_constant
 
 void launch_select(const ztcp_cold_selection& S, cudaStream_t s) {
   const unsigned n = (unsigned)S.n_seqs;
+  if (S.n_seqs > kManySeqs) select_starts_kernel<<<1, 1024, 0, s>>>(S);
   if (S.max_pages <= 256 * kPer) select_kernel<8><<<n, 256, 0, s>>>(S);
   else if (S.max_pages <= 512 * kPer) select_kernel<9><<<n, 512, 0, s>>>(S);
   else select_kernel<10><<<n, 1024, 0, s>>>(S);
