@@ -126,7 +126,8 @@ int32_t ztcp_append_tokens(const ztcp_append* a, int32_t* status, void* stream);
  *     b * max_pages + page; -1 behind the last
  *   kept_tables / kept_mass [n_seqs, max_pages]: the other pages in order, then -1 / 0
  *   kept_lens [n_seqs]: kv_lens minus the cold pages' tokens
- * The outputs overlap neither each other nor the inputs.  A kv_len outside the table is clamped as above. */
+ * The outputs overlap neither each other nor the inputs.  A kv_len outside [0, max_pages * page_tokens] is clamped to
+ * it and reported.  n_seqs * max_pages is below 2^31, and max_pages at most 2^31 - 4096. */
 typedef struct ztcp_cold_selection {
   const float* mass;           /* [n_seqs, max_pages] */
   const int32_t* block_tables; /* [n_seqs, max_pages] */

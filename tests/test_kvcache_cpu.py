@@ -157,6 +157,8 @@ def test_append_refusals(lib, kw, msg):
     (dict(n_seqs=1 << 20, max_pages=1 << 12),
      "selection must hold at least one sequence and page, and fewer than 2^31 pages in all"),
     (dict(page_tokens=0), "selection must hold at least one sequence and page, and fewer than 2^31 pages in all"),
+    (dict(n_seqs=1, max_pages=(1 << 31) - 1), "max_pages beyond 2^31 - 4096"),
+    (dict(n_seqs=1, max_pages=(1 << 31) - 4095), "max_pages beyond 2^31 - 4096"),
     (dict(recent=0), "keep and sink must be non-negative and recent positive"),
     (dict(keep=-1), "keep and sink must be non-negative and recent positive"),
 ])

@@ -266,6 +266,8 @@ int32_t ztcp_select_cold_pages(const ztcp_cold_selection* s, void* stream) {
   if (s->n_seqs <= 0 || s->max_pages <= 0 || s->page_tokens <= 0 || s->page_tokens > (1 << 20) || s->n_seqs > kInt32Max ||
       s->max_pages > kInt32Max || s->n_seqs * s->max_pages > kInt32Max)
     return invalid("selection must hold at least one sequence and page, and fewer than 2^31 pages in all");
+  // (a CTA's steps through a row end on a multiple of 4,096 pages, which has to fit 32 bits)
+  if (s->max_pages > kInt32Max - 4095) return invalid("max_pages beyond 2^31 - 4096");
   if (s->keep < 0 || s->sink < 0 || s->recent < 1) return invalid("keep and sink must be non-negative and recent positive");
   if (s->keep > kInt32Max || s->sink > kInt32Max || s->recent > kInt32Max) return invalid("keep, sink or recent too large");
   ztcp::launch_select(*s, static_cast<cudaStream_t>(stream));
