@@ -52,7 +52,7 @@ typedef struct ztcp_kv_cache {
   int64_t table_stride;
   int64_t max_pages;           /* entries of a row that may be read */
   const int32_t* kv_lens;      /* [n_seqs] */
-  int64_t n_seqs;
+  int64_t n_seqs;              /* 1 to 2^21 */
 } ztcp_kv_cache;
 
 /* The newest tokens' queries, packed: sequence b owns rows [q_starts[b], q_starts[b + 1]).  Its row i is token

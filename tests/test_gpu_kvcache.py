@@ -555,6 +555,32 @@ def test_waits_that_run_out(wait_limit, op, G, hint, D, rope):
         assert bool(((out - 1).abs() <= 2 * bound).all())
 
 
+def test_many_sequences_without_rows():
+    """The largest batch, of sequences without rows but the first and the last: the kernels' waits do not run out."""
+    from ztcp_b200 import kvcache
+
+    n, D = 1 << 21, 64
+    k, v = (queries(64 * 8, 1, D, BF16, s).view(64, 8, 1, D) for s in (1, 2))
+    starts = torch.ones(n + 1, dtype=torch.int32, device=DEV)
+    starts[0], starts[-1] = 0, 301
+    q = queries(301, 1, D, BF16, 3)
+    tables = torch.zeros((n, 1), dtype=torch.int32, device=DEV)
+    lens = torch.full((n,), 8, dtype=torch.int32, device=DEV)
+    out, lse = torch.empty_like(q), torch.empty((301, 1), device=DEV)
+    for hint in (1, 300):
+        out.fill_(9.0)
+        status = kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=starts, max_q_len=hint, causal=False)
+        assert not bool(status.any())
+        want, wl, tol, ltol = ref.attend(cpu(q), cpu(k), cpu(v), cpu(tables[:2]), [8, 8], [1, 300], D ** -0.5, False)
+        ref.assert_close(lse, wl, ltol, "lse")
+        ref.assert_close(out, want, tol, "out")
+        mass = torch.empty((n, 1), device=DEV)
+        assert not bool(kvcache.page_mass(q, k, tables, lens, lse, None, mass, q_starts=starts, max_q_len=hint, causal=False).any())
+        assert not bool(mass[1:-1].any())
+        want, tol = ref.mass(cpu(q), cpu(k), cpu(tables[:2]), [8, 8], [1, 300], cpu(lse), None, 1.0, D ** -0.5, False)
+        ref.assert_close(mass[[0, -1]], want, tol, "mass")
+
+
 @pytest.mark.parametrize("limit", [1, 300, 2000, 6000, 20_000, 100_000])
 def test_waits_that_may_run_out(wait_limit, limit):
     """Limits about what a call's waits take: all of a call's sequences report it, or none does and the results are right;

@@ -89,6 +89,17 @@ def test_scale_too_large_for_base_2(lib):
     assert lib.ztcp_last_error().decode() == msg
 
 
+def test_too_many_sequences(lib):
+    """Beyond 2^21 sequences a kernel's start comes near the bound of its waits."""
+    for n, msg in (((1 << 21) + 1, "more than 2^21 sequences in a batch"), (1 << 24, "more than 2^21 sequences in a batch"),
+                   (-1, "batch must hold at least one sequence")):
+        c, q = cache(n_seqs=n), rows()
+        assert lib.ztcp_attend_pages(c, q, FAKE, None, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
+        assert lib.ztcp_last_error().decode() == msg
+        assert lib.ztcp_page_mass(c, q, FAKE, None, 1.0, FAKE, FAKE, FAKE, 1 << 40, None) == capi.ZTCP_EINVAL
+        assert lib.ztcp_last_error().decode() == msg
+
+
 def test_wait_limit(lib):
     default = 2_000_000_000
     assert lib.ztcp_wait_limit(500) == default

@@ -46,7 +46,10 @@ int32_t to_params(const ztcp_kv_cache* k, const ztcp_queries* q, ztcp::CachePara
   if (rc != ZTCP_OK) return rc;
   const ztcp_geometry& g = k->geom;
   if (g.head_dim > 576) return invalid("head_dim beyond 576");
-  if (k->n_seqs <= 0 || k->n_seqs > (1 << 24)) return invalid("batch must hold at least one sequence");
+  if (k->n_seqs <= 0) return invalid("batch must hold at least one sequence");
+  // A CTA passes over all sequences to find its place on the line of items, and one by one over sequences without rows,
+  // while its other warps wait: 180 ms for 2^20 sequences, of which all but two are empty, and the waits' bound is a second.
+  if (k->n_seqs > (1 << 21)) return invalid("more than 2^21 sequences in a batch");
   if (!k->block_tables || !k->kv_lens) return invalid("block_tables and kv_lens must not be NULL");
   if (k->max_pages <= 0 || k->max_pages > k->table_stride || k->max_pages > (1 << 28))
     return invalid("max_pages must be positive and at most the block tables' row length");
