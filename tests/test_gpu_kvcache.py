@@ -806,6 +806,28 @@ def test_score_loss_does_not_grow_with_the_columns(D, hint, times):
     assert abs(mean(s, e)) <= times * abs(mean(base_s, base)) + 1
 
 
+@pytest.mark.parametrize("kw,fits", [
+    (dict(), True),
+    # a page whose sums, 16 a segment and head, pass 2^31
+    (dict(geom=(1 << 20, 4096, 16), n_seqs=1, max_pages=1), False),
+    # sums of all sequences beyond any memory, their size beyond 64 bits in the second case
+    (dict(geom=(1 << 15, 64, 64), n_seqs=1 << 12, max_pages=1 << 12), False),
+    (dict(geom=(1 << 20, 1 << 9, 16), n_seqs=1 << 21, max_pages=1 << 11), False),
+])
+def test_mass_sums_that_do_not_fit(kw, fits):
+    """Geometries, never launched here, whose segment sums pass 32 bits or a GPU's memory: they go to the kernel that needs
+    no workspace."""
+    from ztcp_b200 import capi, kvcache
+
+    lib = kvcache._load()
+    T, H, D = kw.pop("geom", (64, 8, 128))
+    n, P = kw.get("n_seqs", 4), kw.get("max_pages", 16)
+    c = kvcache._Cache(1 << 16, None, 0, 0, capi.geometry(T, H, D, 0, True), 1, 1 << 16, P, P, 1 << 16, n)
+    q = kvcache._Queries(1 << 16, H * D * 4, D, 1 << 16, n, 4 * H, 64, 0.1, 1)
+    size = lib.ztcp_page_mass_workspace_bytes(c, q)
+    assert size > 16 if fits else size == 16
+
+
 def test_mass_more_rows_than_tokens():
     check_mass([3, 10], [40, 200], 16, 1, 4, 64, F16)
 

@@ -649,11 +649,17 @@ int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_t
 
 }  // namespace
 
-bool page_mass_tc_fits(const CacheParams& c) { return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31); }
-
 int64_t page_mass_tc_workspace(const CacheParams& c, int64_t rows, int sms) {  // sums by step parity
   const int n = chunk_rows(c, rows);
   return (sms + 3) / 4 * 16 + turns_of(c, n) * sums_of(n) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+}
+
+// A sequence's segments and a page's sums have to fit 32 bits (16 sums a segment at most), and all sums a GPU's memory
+// (whose size is formed here in floating point: in 64 bits it could wrap).
+bool page_mass_tc_fits(const CacheParams& c) {
+  const int64_t page_sums = 16 * (int64_t)c.kv_heads * ((c.page_tokens >> seg_shift(c)) + 1);
+  return pages_fit(c, kKeys) && seg_count(c) < ((int64_t)1 << 31) && page_sums < ((int64_t)1 << 31) &&
+         64.0 * c.n_seqs * c.kv_heads * (double)seg_count(c) < 0x1p37;
 }
 
 bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, bool bf16, cudaStream_t s) {
