@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import capi
-from .codec import PreparedCall, _ptr, _require_cuda, _stream_arg, _stream_handle
+from .codec import PreparedCall, _on_device, _ptr, _require_cuda, _stream_arg, _stream_handle
 
 SEQ_OK = 0
 SEQ_BAD_LENGTH = 5  # ZTCP_SEQ_BAD_LENGTH
@@ -228,7 +228,10 @@ class _OwningCall(PreparedCall):
         handle = _stream_arg(self._dev, stream)
         if handle not in self._streams:
             self._meet(handle)
-        return super().__call__(handle)
+        rc = _on_device(self._dev, self._fn, *self._args, handle)
+        if rc != capi.ZTCP_OK:
+            capi.check(rc)
+        return self._result
 
     def _meet(self, handle: int) -> None:
         other = torch.cuda.ExternalStream(handle, device=self._dev)
