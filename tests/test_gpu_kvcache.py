@@ -84,6 +84,23 @@ def test_chunk_head_layouts(H, G):
     check_attend([300, 77, 140], [40, 77, 9], 64, H, G, 128, BF16)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("D,H,G,T,causal", [(256, 2, 4, 64, True), (176, 1, 8, 16, True), (144, 2, 3, 128, False), (208, 1, 1, 40, True),
+                                            (256, 1, 32, 5, True)])
+def test_chunk_wide_heads(D, H, G, T, causal, dtype):
+    """Chunks at head dims that have no chunk kernel: many row blocks of 16 an item's worth each."""
+    check_attend([200, 5, 0, 130, 64, 385], [50, 5, 0, 129, 1, 33], T, H, G, D, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("heads,D,rope,T", [(16, 576, 64, 64), (40, 576, 64, 16), (4, 96, 64, 64), (12, 320, 64, 32), (7, 128, 64, 8),
+                                            (3, 192, 16, 64), (5, 576, 64, 24)])
+def test_single_buffer_chunks(heads, D, rope, T, dtype):
+    """Chunks over latent pages, of more rows than an item holds, at widths from one value group to eight."""
+    check_attend([150, 3, 0, 70], [60, 3, 0, 21], T, 1, heads, D, dtype, mla_rope=rope)
+    check_attend([33, 257], [1, 1], T, 1, heads, D, dtype, mla_rope=rope, decode=True)
+
+
 def test_rows_that_see_nothing():
     # more query rows than tokens: the first rows see nothing; sequences without tokens or without rows between
     check_attend([3, 0, 10, 0, 70], [8, 4, 0, 0, 200], 64, 2, 4, 128, BF16)
@@ -826,6 +843,13 @@ def test_mass_sums_that_do_not_fit(kw, fits):
     q = kvcache._Queries(1 << 16, H * D * 4, D, 1 << 16, n, 4 * H, 64, 0.1, 1)
     size = lib.ztcp_page_mass_workspace_bytes(c, q)
     assert size > 16 if fits else size == 16
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("H,G,D,T", [(1, 16, 576, 64), (1, 40, 576, 16), (2, 4, 256, 64), (1, 3, 320, 32), (2, 2, 176, 40), (2, 8, 128, 64)])
+def test_mass_windows_of_wide_heads(H, G, D, T, dtype):
+    """Windows of several chunks of rows at head dims beyond 128, latent pages among them, and of two 256-row chunks."""
+    check_mass([200, 0, 70, 385], [32, 3, 70, 64], T, H, G, D, dtype, empty=False, bad=[(0, 1), (3, 2)])
 
 
 def test_mass_more_rows_than_tokens():
