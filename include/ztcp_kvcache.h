@@ -18,6 +18,7 @@
  * Every pointer is device memory of the current device.  Lengths, tables and slots are read on the device at
  * every call and checked there before they address memory: a bad one is never followed, and is reported in
  * `status`.
+ * A batch holds at least one sequence, query row or token; an empty one is refused.
  */
 #ifndef ZTCP_KVCACHE_H
 #define ZTCP_KVCACHE_H
@@ -57,7 +58,8 @@ typedef struct ztcp_kv_cache {
 
 /* The newest tokens' queries, packed: sequence b owns rows [q_starts[b], q_starts[b + 1]).  Its row i is token
  * kv_len - q_len + i; with `causal` it sees tokens up to itself, otherwise all of the sequence.  A row that sees
- * nothing gets a zero output and a log-sum-exp of -inf. */
+ * nothing gets a zero output and a log-sum-exp of -inf.  Where starts do not ascend, rows that two sequences claim get the
+ * result of either. */
 typedef struct ztcp_queries {
   const void* q;            /* row r, head h at q + r * token_stride + h * head_stride elements; 16-byte aligned */
   int64_t token_stride;     /* elements, multiples of 8 */

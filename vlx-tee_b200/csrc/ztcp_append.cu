@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ ztc
 // nothing waits for anything but its own copies).  The next token's angles come the same way, its position and slot
 // a token earlier still.  A lane's addresses step from vector to vector and are looked up anew where the kind changes,
 // and with one chunk a lane the norm's weights stay in registers: the instructions are the limit.  Measured:
-// 8,191 tokens of 32 + 8 + 8 vectors of 128 columns, 46.6 us, 4.3 TB/s (57 with addresses and weights looked up for every
-// vector); 4,096 of 16 + 1 of 576, 36.6 us, 4.4 TB/s.
+// 8,191 tokens of 32 + 8 + 8 vectors of 128 columns, neighbours paired, half of the columns rotated, in a graph of calls
+// 46.6 us (57 with addresses and weights looked up for every vector), as a call in a stream 49.1, 4.1 TB/s; 4,096 of 16 + 1 of
+// 576, 36.6 and 38.9 us, 4.2 TB/s; 8,192 of 48 of 128, halves paired, all rotated, 58.
 // CTAs per SM: with halves paired a third one's registers were not enough (spilled; 8,192 tokens 75 us, with two 58).
 template <bool INTER, int CH>
 constexpr int kStreamCtas = CH == 1 && INTER ? 3 : 2;

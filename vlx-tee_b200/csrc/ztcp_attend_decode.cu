@@ -17,10 +17,12 @@
 // thread until the item ends.  O^T is rescaled only when a maximum has grown by more than 2^8 over the one in use.
 // For single-buffer pools V's columns are those of the K tile itself.
 //
-// Measured: 48 sequences of 1,024 to 8,192 tokens, 32/8 heads of 128: 158 us, 5.9 TB/s, of which 8 us are start and join;
-// 32 sequences of 1,000 to 8,100 over a latent cache, 16 heads of 576: 62 us, 2.9 TB/s (48 us of them without any load:
+// Measured: 48 sequences of 1,024 to 8,192 tokens, 32/8 heads of 128: 165 us, 5.7 TB/s, of which 8 us are start and join;
+// 32 sequences of 1,000 to 8,100 over a latent cache, 16 heads of 576: 63 us, 2.8 TB/s (48 us of them without any load:
 // 15 tiles a CTA, of 52 products that take 39 cycles each to issue, do not hide the start, two items' ends and the
-// join); one sequence of 1,021 tokens: 13 us, two launches.
+// join); one sequence of 1,021 tokens: 16 us, two launches.  Chunks that have no kernel of their own come here too, a
+// reading of K and V per 16 rows (latent pages: 32): 512 tokens over 8,192, 16 latent heads of 576 531 us, 32/8 heads of
+// 256 826.
 //
 // Work, joining of shared items and bounded waits as in ztcp_attend_tc.cu.
 #include "ztcp_tc.cuh"

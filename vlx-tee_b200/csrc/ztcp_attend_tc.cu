@@ -22,9 +22,9 @@
 // Bound.  Per 256 x 64 scores the tensor core needs 1,260 cycles (head_dim 128; products of 64 keys read Q at the limit of
 // shared memory's 128 bytes a cycle, else they would need 1,024), the exponentials 1,024 of the special-function units'
 // 16 a cycle, in a thread's chain of score loads, exponentials and P stores that takes 1,590 when both row tiles are in
-// it; together 1,800 were measured.  2,048 new tokens over 32,768 keys, 32 heads of 128: 1,130 us, 940 TFLOP/s (the GPU
-// runs at 1.35 to 1.7 GHz then, as its power allows); five ragged chunks of up to 777 tokens over 800 to 8,192 keys:
-// 240 us, 730 TFLOP/s, join included.
+// it; together 1,800 were measured.  2,048 new tokens over 32,768 keys, 32 heads of 128: 1,160 to 1,190 us, 900 TFLOP/s (the
+// GPU runs at 1.35 to 1.7 GHz then, as its power allows); five ragged chunks of up to 777 tokens over 800 to 8,192 keys:
+// 250 to 258 us, 690 TFLOP/s, join included.
 //
 // Work.  As in ztcp_attend.cu the items form one line that the CTAs (one per SM) share evenly, in units of
 // keys x group (Line); attend_merge_kernel joins items that several CTAs share.

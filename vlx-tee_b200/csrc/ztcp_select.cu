@@ -7,8 +7,9 @@
 // equal to it the first ones that are still wanted.  Counts are integers, so the order of atomics changes nothing.  One
 // CTA per sequence; a thread holds four neighbouring pages, so that up to 4,096 pages are read once and placed by one
 // scan.  A few bytes per page, so the time is that of the passes' barriers, not of memory.
-// Measured: one sequence of 256 pages 4.7 us (an empty kernel takes 2.5), 64 sequences of up to 4,096 pages 10.5; with
-// four passes of 8-bit digits that each read the weights again, and a scan per 1,024 pages, 5.3 and 16.3.
+// Measured in a graph of calls: one sequence of 256 pages 4.7 us (an empty kernel takes 2.5), 64 sequences of up to 4,096
+// pages 10.5 (6.2 and 12.3 as calls in a stream); with four passes of 8-bit digits that each read the weights again, and
+// a scan per 1,024 pages, 5.3 and 16.3.
 #include "ztcp_kvcache.cuh"
 #include "../../include/ztcp_kvcache.h"
 
