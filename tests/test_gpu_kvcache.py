@@ -476,6 +476,37 @@ def test_host_check_reads_in_the_calls_stream():
         kvcache.attend_pages(q[:, :, :64], k, v, tables, lens, out, stream=side)
 
 
+def test_checked_calls_follow_the_current_stream():
+    """A one-shot call whose tables the host checks comes behind the current stream's earlier work, on any stream."""
+    from ztcp_b200 import kvcache
+
+    kv = [700, 65, 900]
+    k, v, tables, lens = ref.make_cache(kv, 64, 2, 128, BF16, 8)
+    q = queries(3, 8, 128, BF16, 9)
+    want, out, lse = torch.empty_like(q), torch.empty_like(q), torch.empty((3, 8), device=DEV)
+    kvcache.attend_pages(q, k, v, tables, lens, want, lse=lse)
+    mass, summed = torch.empty(tables.shape, device=DEV), torch.empty(tables.shape, device=DEV)
+    kvcache.page_mass(q, k, tables, lens, lse, None, mass)
+    late = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(DEV)
+    long_work()
+    out.fill_(7.0)
+    summed.fill_(7.0)
+    late.copy_(q)
+    kvcache.attend_pages(late, k, v, tables, lens, out, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    late.zero_()
+    torch.cuda.synchronize()
+    long_work()
+    summed.fill_(7.0)
+    late.copy_(q)
+    kvcache.page_mass(late, k, tables, lens, lse, None, summed, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(summed, mass)
+
+
 def test_one_shot_calls_in_a_graph():
     """A whole step of one-shot calls, host checks at their default, captured and replayed over new contents."""
     from ztcp_b200 import kvcache

@@ -244,10 +244,11 @@ class _OwningCall(PreparedCall):
         self._streams.add(handle)
 
 
-def _run_once(prepare, first: torch.Tensor | None, stream):
+def _run_once(prepare, first: torch.Tensor | None, stream, checks: bool = False):
     """Prepares and enqueues a call whose own buffers die with it, on `stream` (None: the current one) of the device of
     `first`, an argument.  On another stream than the current one, all of it happens in that stream's order: the host's
-    check reads lengths and tables there, and the buffers are its own.  Whatever the call was given may be dropped at
+    check reads lengths and tables there, and the buffers are its own.  A call that the host checks also follows what the
+    current stream has been given so far (``checks``; its host waits anyhow).  Whatever the call was given may be dropped at
     once, and what it returns is used on the current stream: both are handed back only when both streams are done."""
     if stream is None or not isinstance(first, torch.Tensor) or not first.is_cuda:
         return prepare()(stream)
@@ -255,6 +256,9 @@ def _run_once(prepare, first: torch.Tensor | None, stream):
     if handle == _stream_handle(dev):
         return prepare()(handle)
     here, other = torch.cuda.current_stream(dev), torch.cuda.ExternalStream(handle, device=dev)
+    with torch.cuda.device(dev):
+        if checks and not torch.cuda.is_current_stream_capturing():
+            other.wait_stream(here)
     with torch.cuda.stream(other):
         call = prepare()
         result = call(handle)
@@ -307,7 +311,8 @@ def prepare_attend(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor |
 def attend_pages(q, k_pool, v_pool, block_tables, kv_lens, out, *, stream=None, **kw) -> torch.Tensor:
     """Attention of packed query rows over the sequences' pages, enqueued on `stream` (default: the current
     stream); arguments as for ``prepare_attend``.  Returns status[n] int32 (device)."""
-    return _run_once(lambda: prepare_attend(q, k_pool, v_pool, block_tables, kv_lens, out, **kw), k_pool, stream)
+    return _run_once(lambda: prepare_attend(q, k_pool, v_pool, block_tables, kv_lens, out, **kw), k_pool, stream,
+                     kw.get("check_block_table", True))
 
 
 # ---- attention weight per page ----------------------------------------------------------------------------------
@@ -350,7 +355,8 @@ def prepare_page_mass(q: torch.Tensor, k_pool: torch.Tensor, block_tables: torch
 def page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, *, stream=None, **kw) -> torch.Tensor:
     """Attention weight per page, enqueued on `stream` (default: the current stream); arguments as for
     ``prepare_page_mass``.  Returns status[n] int32 (device)."""
-    return _run_once(lambda: prepare_page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, **kw), k_pool, stream)
+    return _run_once(lambda: prepare_page_mass(q, k_pool, block_tables, kv_lens, lse, mass, out_mass, **kw), k_pool, stream,
+                     kw.get("check_block_table", True))
 
 
 # ---- append -----------------------------------------------------------------------------------------------------
