@@ -883,6 +883,27 @@ def test_mass_windows_of_wide_heads(H, G, D, T, dtype):
     check_mass([200, 0, 70, 385], [32, 3, 70, 64], T, H, G, D, dtype, empty=False, bad=[(0, 1), (3, 2)])
 
 
+@pytest.mark.parametrize("G,D", [(4, 128), (4, 64), (7, 112), (140, 128)])
+def test_mass_items_of_one_and_two_row_tiles(G, D):
+    """Many short items to a CTA, of one row tile and of two, of one chunk and of several, in any order: whichever group of
+    warps an item's first step falls to."""
+    from ztcp_b200 import kvcache
+
+    kv, q_lens = ref.ragged(D + G, 300, 500, 64 if G < 100 else 3)
+    kv = [n + 1 for n in kv]
+    q_lens = [min(m, n) for m, n in zip(q_lens, kv)]
+    k, v, tables, lens = ref.make_large_cache(kv, 16, 1, D, BF16, 9)
+    q = queries(sum(q_lens), G, D, BF16, 8)
+    lse, out = torch.empty(q.shape[:2], device=DEV), torch.empty_like(q)
+    starts = ref.starts_of(q_lens)
+    kvcache.attend_pages(q, k, v, tables, lens, out, lse=lse, q_starts=starts, max_q_len=64)
+    before = torch.rand(tables.shape, device=DEV)
+    mass = torch.empty_like(before)
+    kvcache.page_mass(q, k, tables, lens, lse, before, mass, decay=0.5, q_starts=starts, max_q_len=64)
+    want, tol = ref.mass_large(q, k, tables, kv, q_lens, lse, before, 0.5, D ** -0.5)
+    ref.assert_close(mass, want, tol, "mass")
+
+
 def test_mass_more_rows_than_tokens():
     check_mass([3, 10], [40, 200], 16, 1, 4, 64, F16)
 

@@ -25,9 +25,10 @@
 // Bound: for few rows the reading of K (48 sequences of 1,024 to 8,192 keys, 8 heads, one token each: 94 us, 5.3 TB/s, of
 // which 8 us are start and join); for an observation window the threads' chains of score loads, exponentials and sums
 // (92 us, of which the special-function units need 27 and the join 13: neither they nor the issue of instructions is
-// half busy).  Measured for windows: steps of one row tile and 128 keys instead of two and 64 the same time; loads of the
-// next 16 scores under the arithmetic of these 1 us less; before, with one accumulator a score, a quarter or 3/8 of the
-// exponentials as a polynomial on the FMA pipes or a second warp of products 2 to 8 us more.
+// half busy).  Measured for windows: steps of two row tiles and 64 keys instead of one and 128 the same time (with up to 128
+// rows, 187 us instead of 128: half of the warps have none); loads of the next 16 scores under the arithmetic of these
+// 1 us less; before, with one accumulator a score, a quarter or 3/8 of the exponentials as a polynomial on the FMA pipes
+// or a second warp of products 2 to 8 us more.
 //
 // Warps.  Groups of four: sums of every other step, a thread per key, no warp waiting for another; then one for the
 // products and one for TMA (K tiles page by page through a ring, Q chunks as boxes of tokens x group).  Waits are bounded as in
@@ -40,7 +41,6 @@ namespace ztcp {
 namespace {
 
 constexpr int kBars = 40;
-constexpr int kRowSums = 8;  // sums of a segment that a step with rows on the lanes leaves: one per warp; else one in all
 
 struct MassTcParams {
   MassParams m;
@@ -52,7 +52,7 @@ struct MassTcParams {
   int32_t seg_shift;     // log2 of the keys of a segment: 32, or a smaller page's
   int32_t segs;          // segments of a sequence in the workspace
   int32_t sums;          // sums of a segment that a step leaves in the workspace
-  int32_t turns;         // step parities that a segment's sums come from, where there are several chunks
+  int32_t halves;        // a step is one row tile of a chunk
 };
 
 template <int KG, int N>
@@ -73,9 +73,9 @@ struct Shape {
   // Accumulators of a step: one per column group (two groups where TMEM has no room for more).
   static constexpr int kPer = !kRows && 2 * N * KG > 512 ? 2 : 1;
   static constexpr int kAccs = (KG + kPer - 1) / kPer;
-  // Keys of a step: with rows on the lanes, further accumulators take the columns of further keys.
-  static constexpr int kStepKeys = kRows ? kKeys / kAccs : kKeys;
-  static constexpr int kTileSteps = kKeys / kStepKeys;      // per chunk
+  // With rows on the lanes a second accumulator takes the columns of the second row tile: a step is one row tile then,
+  // and the warps that have the other one where there is one accumulator have the other 64 keys.
+  static constexpr bool kHalves = kRows && kAccs == 2;
   static constexpr int kBuf = kRows ? 256 : kAccs * N;      // columns of a step's scores; TMEM holds two steps'
   static constexpr int kCols = 2 * kBuf <= 32 ? 32 : 2 * kBuf <= 64 ? 64 : 2 * kBuf <= 128 ? 128 : 2 * kBuf <= 256 ? 256 : 512;
   static_assert(kSlots >= kTileSlots && 2 * kSlots + 9 + 2 * kJobs <= kBars && 2 * kBuf <= kCols, "shape");
@@ -94,6 +94,10 @@ __device__ __forceinline__ MassSeq mass_seq(const MassTcParams& P, int b) {
   m.tiles = m.s.q_len > 0 ? (m.s.kv_len + kKeys - 1) / kKeys : 0;
   m.chunks = (m.s.q_len + P.chunk_tokens - 1) / P.chunk_tokens * P.parts;
   return m;
+}
+// Whether chunk ch's rows fill more than one row tile.
+__device__ __forceinline__ bool two_row_tiles(const MassTcParams& P, int N, int q_len, int ch) {
+  return (P.parts == 1 ? (q_len - ch * P.chunk_tokens) * (int64_t)P.m.c.group : P.m.c.group - ch % P.parts * N) > 128;
 }
 
 template <int N>
@@ -253,7 +257,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     // ---- products: one thread ---------------------------------------------------------------------------
     if (elect_one()) {
       constexpr uint32_t kHi = desc_hi(1024, kSwizzle128);
-      const uint32_t qk = inst_desc(BF16, 128, Sh::kRows ? Sh::kStepKeys : N, false, false);
+      const uint32_t qk = inst_desc(BF16, 128, Sh::kRows ? kKeys : N, false, false);
       const uint32_t k_lo = desc_lo(ring, 16), q_lo = desc_lo(qbuf, 16);
       uint32_t kpos = 0, qpos = 0, step = 0, jobs = 0;
       bool ok = true;
@@ -271,30 +275,32 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
             const bool spent = chunks > 1 || t + 1 == tiles;     // and not used again
             const uint32_t qslot = qpos % kQS;
             if (fresh && !wait(q_full + 8 * qslot, qpos / kQS)) break;
-            for (int part = 0; ok && part < Sh::kTileSteps; ++part, ++step) {
+            const bool two = Sh::kRows && two_row_tiles(P, N, job.q_len, ch);
+            const int row_steps = Sh::kHalves && two ? 2 : 1;
+            for (int half = 0; ok && half < row_steps; ++half, ++step) {
               const uint32_t buf = step & 1, d = tmem + buf * Sh::kBuf, q = q_lo + qslot * (Sh::kQBytes >> 4);
               if (step > 1 && !wait(s_read + 8 * buf, (step >> 1) - 1)) break;
 #pragma unroll
               for (int s = 0; s < kTS; ++s) {
                 const uint32_t pos = kpos + s, slot = pos % kSlots;
-                if (ch == 0 && part == 0 && !wait(full(slot), pos / kSlots)) break;
+                if (ch == 0 && half == 0 && !wait(full(slot), pos / kSlots)) break;
                 tc_fence_after();
                 const uint32_t a = k_lo + slot * (Sh::kSlotBytes >> 4);
-                bool two = false;  // the chunk's rows fill more than one row tile
-                if constexpr (Sh::kRows)
-                  two = (P.parts == 1 ? (job.q_len - ch * P.chunk_tokens) * (int64_t)c.group : c.group - ch % P.parts * N) > 128;
 #pragma unroll
                 for (int i = 0; i < Sh::kGroups; ++i) {
                   const int g = s * Sh::kGroups + i;
                   if (g >= KG) continue;
-                  if constexpr (Sh::kRows) {
+                  if constexpr (Sh::kHalves) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                      mma_ss(d + g * kKeys, q + ((g * N * 128 + k * 32) >> 4) + half * (128 * 128 >> 4), kHi, a + ((i * kGroupBytes + k * 32) >> 4), kHi, qk, k > 0);
+                  } else if constexpr (Sh::kRows) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                       if (h == 0 || two)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                          mma_ss(d + (2 * g + h) * Sh::kStepKeys, q + ((g * N * 128 + h * 128 * 128 + k * 32) >> 4), kHi,
-                                 a + ((i * kGroupBytes + part * Sh::kStepKeys * 128 + k * 32) >> 4), kHi, qk, k > 0);
+                          mma_ss(d + h * kKeys, q + ((h * 128 * 128 + k * 32) >> 4), kHi, a + (k * 32 >> 4), kHi, qk, k > 0);
                   } else {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -302,7 +308,7 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
                              g % Sh::kPer > 0 || k > 0);
                   }
                 }
-                if (ch + 1 == chunks && part + 1 == Sh::kTileSteps) tc_commit(empty(slot));
+                if (ch + 1 == chunks && half + 1 == row_steps) tc_commit(empty(slot));
               }
               if (ok) tc_commit(s_full + 8 * buf);
             }
@@ -319,10 +325,10 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
     __syncwarp();
   } else if constexpr (Sh::kRows) {
     // ---- sums: a thread per row -------------------------------------------------------------------------
-    const int wg = (warp >> 2) & 1, half = warp >> 3, r = half * 128 + (tid & 127);
-    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * Sh::kBuf + half * Sh::kStepKeys;  // the first accumulator
+    const int wg = (warp >> 2) & 1, other = warp >> 3;  // 1: the second row tile's warps, or the second 64 keys'
+    const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + wg * Sh::kBuf + other * (Sh::kHalves ? 64 : kKeys);
+    const int from = Sh::kHalves ? other * 64 : 0, keys = Sh::kHalves ? 64 : kKeys;  // this warp's, of a tile
     const uint64_t scale2 = pair(c.scale, c.scale), log2e = pair(1.44269504088896f, 1.44269504088896f);
-    const int tok_in = r / P.part_heads, head_in = r - tok_in * P.part_heads;
     uint32_t step = 0, mine = 0, jobs = 0, tile = 0;
     Job job;
     bool ok = true;
@@ -331,7 +337,8 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
       float neg = -INFINITY;  // -lse; -inf where the row adds nothing
       int lim = 0, clear = 0;  // keys that the row sees, and that all of the warp's rows see
       bool any = false;        // a row of the warp adds something
-      auto load_row = [&](int ch) {
+      auto load_row = [&](int ch, int half) {
+        const int r = half * 128 + (tid & 127), tok_in = r / P.part_heads, head_in = r - tok_in * P.part_heads;
         const int tok = ch / P.parts * P.chunk_tokens + tok_in, g = ch % P.parts * N + head_in;
         neg = -INFINITY;
         if (tok_in < P.chunk_tokens && tok < job.q_len && g < c.group) {
@@ -342,17 +349,23 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         clear = __reduce_min_sync(0xffffffffu, lim);
         any = __any_sync(0xffffffffu, neg != -INFINITY);
       };
-      if (chunks == 1) load_row(0);
+      const bool two = two_row_tiles(P, N, job.q_len, 0);
+      const bool several = chunks > 1 || (Sh::kHalves && two);  // steps a tile
+      // (an only chunk's two row tiles go to the groups by turns, from whichever the item's first step falls to)
+      if (chunks == 1) load_row(0, !Sh::kHalves ? other : two ? (int)(step & 1) ^ wg : 0);
       for (int t = job.ta; ok && t < job.tb; ++t, ++tile) {
         const int j0 = t * kKeys;
         unsigned bad = 0;
         float total = 0.f;  // lane i: the tile's segment i
         bool some = false;
-        for (int x = 0; x < chunks * Sh::kTileSteps; ++x, ++step) {
-          if ((step & 1) != wg) continue;  // (two steps a chunk: this group has the tile's keys of half wg)
-          const int ch = x / Sh::kTileSteps, k0 = x % Sh::kTileSteps * Sh::kStepKeys;
+        int ch = 0, half = 0;
+        for (; ch < chunks; ++step) {
+          const int ch_now = ch, half_now = half;
+          if (Sh::kHalves && half == 0 && (ch == 0 ? two : two_row_tiles(P, N, job.q_len, ch))) half = 1;
+          else half = 0, ++ch;
+          if ((step & 1) != wg) continue;
           some = true;
-          if (chunks > 1) load_row(ch);
+          if (chunks > 1) load_row(ch_now, Sh::kHalves ? half_now : other);
           if (!(ok = warp_wait(s_full + 8 * wg, mine & 1, waits))) break;
           ++mine;
           tc_fence_after();
@@ -394,24 +407,24 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
           };
           if (any) {
 #pragma unroll 1
-            for (int n0 = 0; n0 < Sh::kStepKeys; n0 += 32) {
+            for (int n0 = 0; n0 < keys; n0 += 32) {
               uint32_t x[32];
               tmem_ld32(ts + n0, x);
-              if constexpr (Sh::kAccs > 1) {
+              if constexpr (Sh::kHalves) {
                 uint32_t y[32];
-                tmem_ld32(ts + 2 * Sh::kStepKeys + n0, y);
+                tmem_ld32(ts + kKeys + n0, y);
                 tmem_ready32(x);
                 tmem_ready32(y);
                 add_columns<32>(x, y);
               } else {
                 tmem_ready32(x);
               }
-              if (n0 + 32 == Sh::kStepKeys) {  // S has been read
+              if (n0 + 32 == keys) {  // S has been read
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_read + 8 * wg);
               }
-              add_block(x, k0 + n0);
+              add_block(x, from + n0);
             }
           } else {
             __syncwarp();
@@ -420,10 +433,10 @@ page_mass_tc_kernel(const __grid_constant__ MassTcParams P, const __grid_constan
         }
         if (!ok) break;
         const int seg = (j0 >> P.seg_shift) + lane;
-        const int from = Sh::kTileSteps > 1 ? wg * (Sh::kStepKeys >> P.seg_shift) : 0, segs = Sh::kStepKeys >> P.seg_shift;  // this group's
-        if (some && lane >= from && lane < from + segs && seg << P.seg_shift < job.kv_len) {
+        const int at = lane << P.seg_shift;  // the segment's first key, of the tile's
+        if (some && at >= from && at < from + keys && seg << P.seg_shift < job.kv_len) {
           if (bad >> (lane << P.seg_shift >> P.box.shift) & 1) total = 0.f;
-          P.m.part[(((int64_t)((chunks > 1 && Sh::kTileSteps == 1 ? kRowSums * wg : 0) + half * 4 + (warp & 3)) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + seg] = total;
+          P.m.part[(((int64_t)((several ? P.sums * wg : 0) + (Sh::kHalves ? 0 : other * 4) + (warp & 3)) * c.n_seqs + job.b) * c.kv_heads + job.head) * P.segs + seg] = total;
         }
       }
     }
@@ -593,7 +606,7 @@ __global__ void __launch_bounds__(256) page_mass_join_kernel(const __grid_consta
       if (P.m.mass) before = P.m.mass[i];
       if (m.chunks > 0) {
         n = (int)((min((int64_t)c.page_tokens, left) + (1 << P.seg_shift) - 1) >> P.seg_shift);
-        slots = m.chunks > 1 ? P.turns : 1;
+        slots = m.chunks > 1 || (P.halves && two_row_tiles(P, 256, m.s.q_len, 0)) ? 2 : 1;
       }
     }
   }
@@ -635,23 +648,23 @@ void launch_any(const MassTcParams& P, int n, const CUtensorMap& k, const CUtens
 }
 
 // Rows of a chunk: the smallest of 16, 64 and 256 that holds a sequence's rows; wide heads leave less room for Q.
-// Measured on 48 sequences of 1,024 to 8,192 tokens, 8 KV heads of 128, with 16 / 64 / 256: 4 rows 85.4 / 86.1 / 130 us,
-// 32 rows 150 / 87 / 131, 64 rows 241 / 102 / 132, 128 rows 436 / 208 / 133.
+// Measured on 48 sequences of 1,024 to 8,192 tokens, 8 KV heads of 128, with 16 / 64 / 256: 4 rows 87.5 / 92.0 / 128 us,
+// 32 rows 156 / 90 / 128, 64 rows 251 / 113 / 129, 128 rows 449 / 233 / 129.
 int chunk_rows(const CacheParams& c, int64_t rows) {
   if (rows <= 16) return 16;
   if (c.head_dim > 256) return 32;
   return rows <= 64 || c.head_dim > 128 ? 64 : 256;
 }
-int sums_of(int n) { return n == 256 ? kRowSums : 1; }
-int turns_of(const CacheParams& c, int n) { return n == 256 && c.head_dim > 64 ? 1 : 2; }  // Shape::kTileSteps of 2: 1
+// Shape::kHalves, and the sums of a segment that a step leaves: one per warp with rows on the lanes, else one in all.
+bool halves_of(const CacheParams& c, int n) { return n == 256 && c.head_dim > 64; }
+int sums_of(const CacheParams& c, int n) { return n != 256 ? 1 : halves_of(c, n) ? 4 : 8; }
 int seg_shift(const CacheParams& c) { return c.page_tokens >= 32 ? 5 : c.page_tokens == 16 ? 4 : 3; }
 int64_t seg_count(const CacheParams& c) { return (int64_t)c.max_pages * c.page_tokens >> seg_shift(c); }
 
 }  // namespace
 
 int64_t page_mass_tc_workspace(const CacheParams& c, int64_t rows, int sms) {  // sums by step parity
-  const int n = chunk_rows(c, rows);
-  return (sms + 3) / 4 * 16 + turns_of(c, n) * sums_of(n) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
+  return (sms + 3) / 4 * 16 + 2 * sums_of(c, chunk_rows(c, rows)) * c.n_seqs * (int64_t)c.kv_heads * seg_count(c) * (int64_t)sizeof(float);
 }
 
 // A sequence's segments and a page's sums have to fit 32 bits (16 sums a segment at most), and all sums a GPU's memory
@@ -675,8 +688,8 @@ bool launch_page_mass_tc(MassParams m, int64_t rows, int sms, void* workspace, b
   P.part_heads = m.c.group < n ? m.c.group : n;
   P.seg_shift = seg_shift(m.c);
   P.segs = (int32_t)seg_count(m.c);
-  P.sums = sums_of(n);
-  P.turns = turns_of(m.c, n);
+  P.sums = sums_of(m.c, n);
+  P.halves = halves_of(m.c, n);
   CUtensorMap k, q;
   if (!pool_map(&k, m.c.k, m.c, bf16, P.box) || !query_map(&q, m.c, bf16, P.chunk_tokens, P.part_heads)) return false;
   if (bf16) launch_any<true>(P, n, k, q, s);
